@@ -15,36 +15,44 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffast-math", "
          "-Wno-unused-result", "-DNDEBUG",
          # no SLP vectorizer: it pairs scalar fp32 adds/muls into v_pk_*_f32, which issue slower than the two
          # scalar ops they replace next to MFMA/exp streams (measured on the attention kernels)
-         "-fno-slp-vectorize"]
+         "-fno-slp-vectorize",
+         # no packed fp32 instructions at all: vector types make them without the SLP vectorizer too, and some of their
+         # forms have given wrong results on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# Sources whose kernels see infinities and NaN in earnest (masked keys, empty rows): -ffast-math without the assumption
+# that there are none.
+HONOR_NONFINITE = {"dm_cross.hip", "dm_rope.hip"}
 
 
 def hipcc():
     return shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
-def _compile(src):
+def _compile(src, force=False):
     obj = os.path.join(OBJ, os.path.basename(src) + ".o")
     deps = [src] + [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith(".h")] + [
         os.path.join(os.path.dirname(PKG), "include", "dm_hip.h")]
-    if os.path.exists(obj) and all(os.path.getmtime(obj) > os.path.getmtime(d) for d in deps):
+    if not force and os.path.exists(obj) and all(os.path.getmtime(obj) > os.path.getmtime(d) for d in deps):
         return obj, ""
-    r = subprocess.run([hipcc(), *FLAGS, "-c", src, "-o", obj], capture_output=True, text=True)
+    extra = ["-fno-finite-math-only"] if os.path.basename(src) in HONOR_NONFINITE else []
+    r = subprocess.run([hipcc(), *FLAGS, *extra, "-c", src, "-o", obj], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{r.stdout}\n{r.stderr}")
     return obj, r.stderr
 
 
-def build(verbose=False):
+def build(verbose=False, force=False):
+    """``force``: compile every source, also where an up-to-date object is there."""
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith(".hip"))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        res = list(ex.map(_compile, srcs))
+        res = list(ex.map(lambda src: _compile(src, force), srcs))
     objs = [o for o, _ in res]
     if verbose:
         for _, err in res:
             if err.strip():
                 print(err)
-    if os.path.exists(OUT) and all(os.path.getmtime(OUT) > os.path.getmtime(o) for o in objs):
+    if not force and os.path.exists(OUT) and all(os.path.getmtime(OUT) > os.path.getmtime(o) for o in objs):
         return OUT
     r = subprocess.run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT, *objs],
                        capture_output=True, text=True)
