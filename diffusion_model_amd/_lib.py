@@ -63,6 +63,23 @@ class Cross1Args(C.Structure):
                 ("drop_p", c_float), ("drop_seed", c_ulonglong)]
 
 
+class CrossArgs(C.Structure):
+    _fields_ = [("q", c_void_p), ("ldq", c_long), ("k", c_void_p), ("ldk", c_long), ("v", c_void_p), ("ldv", c_long),
+                ("o", c_void_p), ("ldo", c_long), ("lse", c_void_p), ("d_o", c_void_p), ("lddo", c_long),
+                ("dq", c_void_p), ("lddq", c_long), ("dk", c_void_p), ("lddk", c_long), ("dv", c_void_p), ("lddv", c_long),
+                ("lens", c_void_p), ("mask", c_void_p), ("index", c_void_p),
+                ("B", c_int), ("Bc", c_int), ("heads", c_int), ("kv_heads", c_int), ("Nq", c_int), ("Nk", c_int),
+                ("hd", c_int), ("dtype", c_int), ("scale", c_float), ("drop_p", c_float), ("drop_seed", c_ulonglong),
+                ("workspace", c_void_p), ("ws_bytes", c_long)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_long), ("y", c_void_p), ("ldy", c_long), ("dtype", c_int), ("B", c_int),
+                ("N", c_int), ("heads", c_int), ("hd", c_int), ("rot", c_int), ("pairing", c_int), ("freq", c_void_p),
+                ("axis", c_void_p), ("axes", c_int), ("pos", c_void_p), ("pos_f32", c_int), ("pos_batch_stride", c_long),
+                ("grid", c_int * 3), ("inverse", c_int)]
+
+
 _SIGS = {
     "dm_abi_version": (c_int, []),
     "dm_target_arch": (C.c_char_p, []),
@@ -92,6 +109,11 @@ _SIGS = {
     "dm_cross1_fwd": (c_int, [C.POINTER(Cross1Args), c_void_p]),
     "dm_cross1_bwd": (c_int, [C.POINTER(Cross1Args), c_void_p]),
     "dm_cross1_bwd_workspace_bytes": (c_long, [c_int] * 3),
+    "dm_cross_fwd": (c_int, [C.POINTER(CrossArgs), c_void_p]),
+    "dm_cross_bwd": (c_int, [C.POINTER(CrossArgs), c_void_p]),
+    "dm_cross_fwd_workspace_bytes": (c_long, [C.POINTER(CrossArgs)]),
+    "dm_cross_bwd_workspace_bytes": (c_long, [C.POINTER(CrossArgs)]),
+    "dm_rope": (c_int, [C.POINTER(RopeArgs), c_void_p]),
     "dm_nchw_f32_to_nhwc_bf16": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_long, c_int, c_void_p]),
     "dm_nhwc_to_nchw_f32": (c_int, [c_void_p, c_int, c_long, c_void_p, c_int, c_int, c_int, c_void_p]),
     "dm_cast_f32_to_bf16": (c_int, [c_void_p, c_void_p, c_long, c_void_p]),

@@ -19,9 +19,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffast-math", "
          # no packed fp32 instructions at all: vector types make them without the SLP vectorizer too, and some of their
          # forms have given wrong results on this hardware
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# Sources whose kernels see infinities and NaN in earnest (masked keys, empty rows): -ffast-math without the assumption
-# that there are none.
-HONOR_NONFINITE = {"dm_cross.hip", "dm_rope.hip"}
+# Sources whose kernels see infinities and NaN in earnest (masked keys, empty rows) or reduce angles in 64 bits: no fast math.
+PRECISE = {"dm_cross_fwd.hip", "dm_cross_bwd.hip", "dm_rope.hip"}
 
 
 def hipcc():
@@ -34,7 +33,7 @@ def _compile(src, force=False):
         os.path.join(os.path.dirname(PKG), "include", "dm_hip.h")]
     if not force and os.path.exists(obj) and all(os.path.getmtime(obj) > os.path.getmtime(d) for d in deps):
         return obj, ""
-    extra = ["-fno-finite-math-only"] if os.path.basename(src) in HONOR_NONFINITE else []
+    extra = ["-fno-fast-math"] if os.path.basename(src) in PRECISE else []
     r = subprocess.run([hipcc(), *FLAGS, *extra, "-c", src, "-o", obj], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{r.stdout}\n{r.stderr}")

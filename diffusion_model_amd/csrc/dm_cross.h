@@ -1,0 +1,223 @@
+// Shared pieces of the cross-attention kernels (dm_cross_fwd.hip, dm_cross_bwd.hip).
+//
+// One source serves bf16 and fp32.  Everything runs on the 32x32 MFMA tiles (32x32x16 bf16, four 32x32x2 fp32): in both
+// types a FRAGMENT is 16 bytes per lane, the reduction chunk of one fragment is 32 bytes of a row (16 bf16 or 8 fp32), and
+// lane l holds row l % 32, bytes [16 (l / 32), +16) of the chunk.  For fp32 that assigns the reduction indices to the four
+// MFMAs in another order than memory's, the same for both operands, so the sum is the same.
+//
+// A 32x32 result tile puts column l % 32 and rows 8 i + 4 (l / 32) + r (register 4 i + r) into lane l.  Scores are computed
+// with the softmax axis on the registers (forward, dq) or the lanes (dk, dv), and the probability tile is then, register by
+// register, already the second product's operand over the reduction order "rows 8 i + 4 half + r"; the other operand takes
+// that order through the row addresses of its transposing LDS reads (tr_frag).  No probability passes through LDS.
+#pragma once
+#include "dm_common.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float CR_LOG2E = 1.4426950408889634f;
+constexpr float CR_LN2 = 0.6931471805599453f;
+
+struct CrossParams {
+  const char *q, *k, *v, *d_o;
+  char *o, *dq, *dk, *dv;
+  long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;    // row strides, BYTES
+  float* lse;
+  float* delta;                                       // [B, heads, Nq]: sum_d dO * O (dq kernel -> dk / dv kernel)
+  const int* lens; const unsigned char* mask; const int* index;
+  int B, Bc, H, G, Nq, Nk, hd;
+  float scale;
+  uint32_t seed, thresh; float inv_keep; const uint32_t* seed_ctr;   // dropout (dm_common.h); thresh 0 = none
+  int kb;                      // keys staged per LDS image (a multiple of 64)
+  int iters;                   // query tiles per wave and workgroup
+  int nqb;                     // workgroups along the queries
+  int nsplit, ksplit;          // forward: key splits and keys per split; dk / dv: splits of the query list
+  float* part;                 // split results
+};
+
+// context of a sample, or -1 (no keys)
+__device__ __forceinline__ int context_of(const CrossParams& p, int b) {
+  if (!p.index) return p.Bc == 1 ? 0 : b;
+  const int c = p.index[b];
+  return c >= 0 && c < p.Bc ? c : -1;
+}
+__device__ __forceinline__ int keys_of(const CrossParams& p, int c) {
+  if (c < 0) return 0;
+  const int n = p.lens ? p.lens[c] : p.Nk;
+  return n < 0 ? 0 : (n > p.Nk ? p.Nk : n);
+}
+
+template <typename T> struct Cr;
+template <> struct Cr<bf16> {
+  typedef bf16x8 frag;
+  static constexpr int NF = 2;      // fragments that a 32-row reduction takes
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // operand fragment f of a result tile (its rows are the reduction axis)
+  static __device__ __forceinline__ frag pack(const f32x16& s, int f) {
+    frag r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (bf16)s[8 * f + j];
+    return r;
+  }
+};
+template <> struct Cr<float> {
+  typedef f32x4 frag;
+  static constexpr int NF = 4;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ frag pack(const f32x16& s, int f) {
+    return frag{s[4 * f], s[4 * f + 1], s[4 * f + 2], s[4 * f + 3]};
+  }
+};
+
+// Head width HDP: hd rounded up to 16, 32, 64, 96 or 128; the padding is zero in LDS and in the registers.
+template <typename T, int HDP> struct Geo {
+  static constexpr int RB = HDP * (int)sizeof(T);          // row bytes
+  static constexpr int NC = RB / 32;                       // reduction chunks of a row
+  static constexpr int DT = HDP < 32 ? 1 : HDP / 32;       // 32-channel tiles of a head-dim-major result
+  static constexpr int PPR = RB / 16;                      // 16-byte pieces of a row
+  // LDS row strides.  SR (rows read as operand rows, 16 bytes per lane and row): an odd number of 16-byte units, so that
+  // any 16 consecutive rows start in different banks.  ST (rows read through the transposing loads, 64 bytes of each of
+  // four rows at a time): 4 or 12 units modulo 16; 48 bytes where a row has only 32.
+  static constexpr int SR = RB + 16;
+  static constexpr int units = RB / 16;
+  static constexpr int ST = sizeof(T) == 4 ? RB + 16 : (units < 4 ? 48 : (units == 8 ? 192 : (units == 16 ? 320 : RB)));
+};
+
+template <typename T, int HDP>
+__device__ __forceinline__ typename Cr<T>::frag tr_frag(const char* tile, int stride, int f, int dt, int lane) {
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const int qq = (lane & 15) >> 2, pp = lane & 3, c16 = HDP < 32 ? 0 : (lane >> 4) & 1;
+    const char* a = tile + (16 * f + 4 * h + qq) * stride + dt * 64 + c16 * 32 + pp * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(a + 8 * stride));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    const int d = HDP < 32 ? lane & 15 : lane & 31;
+    const char* a = tile + (8 * f + 4 * h) * stride + (dt * 32 + d) * 4;
+    f32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(a + j * stride);
+    return r;
+  }
+}
+template <typename T>
+__device__ __forceinline__ typename Cr<T>::frag row_frag(const char* tile, int stride, int kc, int lane) {
+  return *reinterpret_cast<const typename Cr<T>::frag*>(tile + (lane & 31) * stride + kc * 32 + (lane >> 5) * 16);
+}
+template <typename T> __device__ __forceinline__ typename Cr<T>::frag zero_frag() {
+  return __builtin_bit_cast(typename Cr<T>::frag, u32x4{0u, 0u, 0u, 0u});
+}
+// the row fragments of one row straight from global memory (zero past the head width, and altogether if !ok)
+template <typename T, int HDP>
+__device__ __forceinline__ void load_frags(const char* row, bool ok, int hdb, int lane,
+                                           typename Cr<T>::frag (&f)[Geo<T, HDP>::NC]) {
+#pragma unroll
+  for (int kc = 0; kc < Geo<T, HDP>::NC; ++kc) {
+    const int off = kc * 32 + (lane >> 5) * 16;
+    f[kc] = ok && off < hdb ? *reinterpret_cast<const typename Cr<T>::frag*>(row + off) : zero_frag<T>();
+  }
+}
+// rows [r0, r0 + n) -> LDS rows 0..n-1; rows past `valid` or masked out, and the padding of a head, become zero
+template <typename T, int HDP>
+__device__ __forceinline__ void stage_rows(char* dst, int stride, const char* src, long ld, int r0, int n, int valid,
+                                           const unsigned char* mask, int hdb, int tid) {
+  constexpr int PPR = Geo<T, HDP>::PPR;
+  for (int i = tid; i < n * PPR; i += 256) {
+    const int r = i / PPR, pc = i % PPR;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (r0 + r < valid && pc * 16 < hdb && (!mask || mask[r0 + r]))
+      v = *reinterpret_cast<const u32x4*>(src + (long)(r0 + r) * ld + pc * 16);
+    *reinterpret_cast<u32x4*>(dst + r * stride + pc * 16) = v;
+  }
+}
+// validity bits of keys [r0, r0 + n): one word per 32 keys
+__device__ __forceinline__ void stage_bits(uint32_t* bits, int r0, int n, int valid, const unsigned char* mask, int tid) {
+  for (int i = tid; i < ((n + 63) & ~63); i += 256) {
+    const bool ok = i < n && r0 + i < valid && (!mask || mask[r0 + i]);
+    const unsigned long long w = __ballot(ok);
+    if ((tid & 63) == 0) { bits[i >> 5] = (uint32_t)w; bits[(i >> 5) + 1] = (uint32_t)(w >> 32); }
+  }
+}
+// x of this lane and of its partner 32 lanes on (in the order of the halves)
+__device__ __forceinline__ void half_swap(float x, float& a, float& b) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned r0 = r[0], r1 = r[1];     // (copied out: a bit cast of a vector's element reads the vector's first)
+  a = __builtin_bit_cast(float, r0);
+  b = __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ float half_max(float x) {
+  float a, b;
+  half_swap(x, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  float a, b;
+  half_swap(x, a, b);
+  return a + b;
+}
+__device__ __forceinline__ int tile_row(int reg, int half) { return 8 * (reg >> 2) + 4 * half + (reg & 3); }
+template <typename T> __device__ __forceinline__ void store4(char* dst, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 2) {
+    const bf16x4 w = {(bf16)a, (bf16)b, (bf16)c, (bf16)d};
+    *reinterpret_cast<bf16x4*>(dst) = w;
+  } else {
+    *reinterpret_cast<f32x4*>(dst) = f32x4{a, b, c, d};
+  }
+}
+// Consecutive workgroups go to the eight XCDs in turn; this gives each XCD a contiguous run of logical ids, so that the
+// workgroups that share cache lines (the narrow heads of one query block) and keys share an L2.
+__device__ __forceinline__ uint32_t xcd_contiguous(uint32_t id, uint32_t n) {
+  const uint32_t per = n >> 3;
+  return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+// ---------------------------------------------------------------- host side
+inline int cross_hdp(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 96 ? 96 : 128))); }
+
+inline bool cross_sizes_ok(const dm_cross_args* a) {
+  return a && a->B > 0 && a->Bc > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->Nq > 0 &&
+         a->Nk >= 0 && a->hd >= 8 && a->hd <= 128 && a->hd % 8 == 0 && (a->dtype == 0 || a->dtype == 1) &&
+         (long)a->B * a->heads * a->Nq < (1L << 40) && a->Nq < (1 << 30) && a->Nk < (1 << 30);
+}
+inline int cross_fill(CrossParams& p, const dm_cross_args* a, bool bwd) {
+  DM_REQUIRE(cross_sizes_ok(a));
+  DM_REQUIRE(a->index || a->Bc == a->B || a->Bc == 1);
+  DM_REQUIRE(a->q && a->o && a->lse && (a->Nk == 0 || (a->k && a->v)));
+  DM_REQUIRE(a->scale > 0.f && a->scale < 1e30f && a->drop_p >= 0.f && a->drop_p < 1.f);
+  const long e = a->dtype == 0 ? 2 : 4;
+  const long qw = (long)a->heads * a->hd, kw = (long)a->kv_heads * a->hd;
+  auto rows_ok = [&](const void* ptr, long ld, long width) { return (uintptr_t)ptr % 16 == 0 && ld * e % 16 == 0 && ld >= width; };
+  DM_REQUIRE(rows_ok(a->q, a->ldq, qw) && rows_ok(a->o, a->ldo, qw));
+  DM_REQUIRE(a->Nk == 0 || (rows_ok(a->k, a->ldk, kw) && rows_ok(a->v, a->ldv, kw)));
+  if (bwd) {
+    DM_REQUIRE(a->d_o && a->dq && rows_ok(a->d_o, a->lddo, qw) && rows_ok(a->dq, a->lddq, qw));
+    DM_REQUIRE(a->Nk == 0 || (a->dk && a->dv && rows_ok(a->dk, a->lddk, kw) && rows_ok(a->dv, a->lddv, kw)));
+  }
+  p.q = (const char*)a->q; p.k = (const char*)a->k; p.v = (const char*)a->v; p.d_o = (const char*)a->d_o;
+  p.o = (char*)a->o; p.dq = (char*)a->dq; p.dk = (char*)a->dk; p.dv = (char*)a->dv;
+  p.ldq = a->ldq * e; p.ldk = a->ldk * e; p.ldv = a->ldv * e; p.ldo = a->ldo * e;
+  p.lddo = a->lddo * e; p.lddq = a->lddq * e; p.lddk = a->lddk * e; p.lddv = a->lddv * e;
+  p.lse = a->lse; p.lens = a->lens; p.mask = a->mask; p.index = a->index;
+  p.B = a->B; p.Bc = a->Bc; p.H = a->heads; p.G = a->kv_heads; p.Nq = a->Nq; p.Nk = a->Nk; p.hd = a->hd;
+  p.scale = a->scale;
+  uint32_t t15 = a->drop_p > 0.f ? (uint32_t)((double)a->drop_p * 32768.0 + 0.5) : 0u;   // as dm_attn_fwd
+  if (t15 > 32767u) t15 = 32767u;
+  p.thresh = 2u * t15;
+  p.inv_keep = 32768.f / (32768.f - (float)t15);
+  p.seed = dm_seed32(a->drop_seed);
+  p.seed_ctr = a->drop_p > 0.f ? dm_dropout_counter() : nullptr;
+  return DM_OK;
+}
+
+}  // namespace

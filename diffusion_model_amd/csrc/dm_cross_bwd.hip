@@ -1,0 +1,405 @@
+// Attention to an encoder's states of another length, backward (include/dm_hip.h: dm_cross_bwd).
+//
+//   P = exp2(c S - lse log2(e)),  dP = dO V^T,  dS = P (dP - delta),  delta = sum_d dO * O,
+//   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
+// dQ runs with the queries on the lanes (as the forward), dK / dV with the keys on the lanes; each probability tile is then
+// already the operand of the product that reduces over its rows.
+#include "dm_cross.h"
+
+namespace {
+
+// ---------------------------------------------------------------- dQ (and delta)
+template <typename T, int HDP, bool RES, bool DROP>
+__global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
+  typedef Geo<T, HDP> Gm;
+  typedef typename Cr<T>::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* sK = smem;
+  char* sV = sK + p.kb * Gm::SR;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(sV + p.kb * Gm::SR);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int h = id % p.H;
+  id /= p.H;
+  const int qb = id % p.nqb, b = id / p.nqb;
+  const int ctx = context_of(p, b), kn = keys_of(p, ctx);
+  const int hdb = p.hd * (int)sizeof(T), g = h / (p.H / p.G);
+  const long krow = (long)(ctx < 0 ? 0 : ctx) * p.Nk;
+  const char* kbase = p.k + krow * p.ldk + g * hdb;
+  const char* vbase = p.v + krow * p.ldv + g * hdb;
+  const unsigned char* mask = p.mask ? p.mask + krow : nullptr;
+  const float c = p.scale * CR_LOG2E;
+  const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
+  frag qf[Gm::NC], df[Gm::NC];
+  f32x16 acc[Gm::DT];
+  float L2 = 0.f, delta = 0.f;
+  uint32_t rs = 0;
+  auto begin = [&](int q) {
+    const bool ok = q < p.Nq;
+    const long tok = (long)b * p.Nq + q, row = ((long)b * p.H + h) * p.Nq + q;
+    load_frags<T, HDP>(p.q + tok * p.ldq + h * hdb, ok, hdb, lane, qf);
+    load_frags<T, HDP>(p.d_o + tok * p.lddo + h * hdb, ok, hdb, lane, df);
+    frag of[Gm::NC];
+    load_frags<T, HDP>(p.o + tok * p.ldo + h * hdb, ok, hdb, lane, of);
+    float s = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < Gm::NC; ++kc)
+#pragma unroll
+      for (int j = 0; j < (int)(16 / sizeof(T)); ++j) s += (float)df[kc][j] * (float)of[kc][j];
+    delta = half_sum(s);
+    L2 = ok ? p.lse[row] * CR_LOG2E : 0.f;
+    if (ok && half == 0) p.delta[row] = delta;
+    if (DROP) rs = dm_drop_row(seed, (uint32_t)row);
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  };
+  auto stage = [&](int from, int n) {
+    stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, kn, mask, hdb, tid);
+    stage_rows<T, HDP>(sV, Gm::SR, vbase, p.ldv, from, n, kn, mask, hdb, tid);
+    stage_bits(bits, from, n, kn, mask, tid);
+  };
+  auto sweep = [&](int from, int tiles) {
+    for (int t = 0; t < tiles; ++t) {
+      const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
+      if (w == 0) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+#pragma unroll
+      for (int kc = 0; kc < Gm::NC; ++kc) {
+        s = Cr<T>::mma(row_frag<T>(sK + t * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s);
+        dp = Cr<T>::mma(row_frag<T>(sV + t * 32 * Gm::SR, Gm::SR, kc, lane), df[kc], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -L2));
+      if (DROP) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t key = from + t * 32 + tile_row(i, half), z = dm_drop_bits(rs, key >> 1);
+          dp[i] = dm_keep16(z, 0, p.thresh) ? dp[i] * p.inv_keep : 0.f;
+          dp[i + 1] = dm_keep16(z, 1, p.thresh) ? dp[i + 1] * p.inv_keep : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
+      if (w != 0xFFFFFFFFu) {
+        const uint32_t mine = w >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = (mine >> tile_row(i, 0)) & 1u ? s[i] : 0.f;
+      }
+#pragma unroll
+      for (int f = 0; f < Cr<T>::NF; ++f) {
+        const frag sf = Cr<T>::pack(s, f);
+#pragma unroll
+        for (int d = 0; d < Gm::DT; ++d)
+          acc[d] = Cr<T>::mma(tr_frag<T, HDP>(sK + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, acc[d]);
+      }
+    }
+  };
+  auto finish = [&](int q) {
+    if (q >= p.Nq) return;
+    char* dst = p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = d * 32 + 8 * i + 4 * half;
+        if (col < p.hd)
+          store4<T>(dst + col * sizeof(T), acc[d][4 * i] * p.scale, acc[d][4 * i + 1] * p.scale, acc[d][4 * i + 2] * p.scale, acc[d][4 * i + 3] * p.scale);
+      }
+  };
+  const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
+  if (RES) {
+    const int n = (kn + 31) & ~31;
+    stage(0, n);
+    __syncthreads();
+    for (int it = 0; it < p.iters; ++it) {
+      const int q = q0 + it * 128;
+      if (q - (lane & 31) >= p.Nq) break;
+      begin(q);
+      sweep(0, n >> 5);
+      finish(q);
+    }
+  } else {
+    begin(q0);
+    for (int from = 0; from < kn; from += p.kb) {
+      const int n = min(p.kb, (kn - from + 31) & ~31);
+      __syncthreads();
+      stage(from, n);
+      __syncthreads();
+      sweep(from, n >> 5);
+    }
+    finish(q0);
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+// A workgroup owns 128 keys (32 per wave, on the lanes) of one (context, key / value head) and walks a share of the
+// context's query list: every sample that uses the context, every query head of the group, 64 queries at a time.  The
+// blocks of that list go to the p.nsplit shares in turn, each share leaves one fp32 partial, and cross_sum_kernel adds
+// them in order: no atomics, the same inputs give the same bits.
+constexpr int QS = 64;
+
+template <typename T, int HDP, bool DROP>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && HDP > 64) ? 1 : 2) void cross_dkv_kernel(const CrossParams p) {
+  typedef Geo<T, HDP> Gm;
+  typedef typename Cr<T>::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* sQ = smem;
+  char* sD = sQ + QS * Gm::SR;
+  float* sL = reinterpret_cast<float*>(sD + QS * Gm::SR);
+  float* sDelta = sL + QS;
+  uint32_t* sRow = reinterpret_cast<uint32_t*>(sDelta + QS);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int nkb = (p.Nk + 127) / 128;
+  uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int g = id % p.G;
+  id /= p.G;
+  const int kblk = id % nkb;
+  id /= nkb;
+  const int split = id % p.nsplit, ctx = id / p.nsplit;
+  const int kn = keys_of(p, ctx), hdb = p.hd * (int)sizeof(T), HG = p.H / p.G;
+  const int key = kblk * 128 + wave * 32 + (lane & 31);
+  const long krow = (long)ctx * p.Nk + key;
+  const bool valid = key < kn && (!p.mask || p.mask[krow]);
+  const bool active = __any(valid);
+  const float c = p.scale * CR_LOG2E;
+  const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
+  frag kf[Gm::NC], vf[Gm::NC];
+  load_frags<T, HDP>(p.k + krow * p.ldk + g * hdb, valid, hdb, lane, kf);
+  load_frags<T, HDP>(p.v + krow * p.ldv + g * hdb, valid, hdb, lane, vf);
+  f32x16 dk[Gm::DT], dv[Gm::DT];
+#pragma unroll
+  for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
+
+  const int nqc = (p.Nq + QS - 1) / QS;
+  const uint32_t per = (uint32_t)HG * nqc;       // blocks of 64 queries per sample
+  auto block_of = [&](int b, int hh, int qc) {
+    const int h = g * HG + hh, r0 = qc * QS;
+    const long tok = (long)b * p.Nq, row = ((long)b * p.H + h) * p.Nq;
+    __syncthreads();
+    stage_rows<T, HDP>(sQ, Gm::SR, p.q + tok * p.ldq + h * hdb, p.ldq, r0, QS, p.Nq, nullptr, hdb, tid);
+    stage_rows<T, HDP>(sD, Gm::SR, p.d_o + tok * p.lddo + h * hdb, p.lddo, r0, QS, p.Nq, nullptr, hdb, tid);
+    if (tid < QS) {
+      const int q = r0 + tid;
+      const float l = q < p.Nq ? p.lse[row + q] * CR_LOG2E : INFINITY;
+      sL[tid] = l == -INFINITY ? INFINITY : l;      // no probability for queries past the end
+      sDelta[tid] = q < p.Nq ? p.delta[row + q] : 0.f;
+      if (DROP) sRow[tid] = dm_drop_row(seed, (uint32_t)(row + q));
+    }
+    __syncthreads();
+    if (!active) return;
+    for (int t = 0; t < QS / 32; ++t) {
+      if (r0 + t * 32 >= p.Nq) break;
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+#pragma unroll
+      for (int kc = 0; kc < Gm::NC; ++kc) {
+        s = Cr<T>::mma(row_frag<T>(sQ + t * 32 * Gm::SR, Gm::SR, kc, lane), kf[kc], s);
+        dp = Cr<T>::mma(row_frag<T>(sD + t * 32 * Gm::SR, Gm::SR, kc, lane), vf[kc], dp);
+      }
+      f32x16 pd;      // what multiplies dO: the probability, dropped
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(sL + t * 32 + 8 * i + 4 * half);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sDelta + t * 32 + 8 * i + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + r], c, -l4[r]));
+          float z = 1.f;
+          if (DROP) z = dm_keep16(dm_drop_bits(sRow[t * 32 + 8 * i + 4 * half + r], (uint32_t)key >> 1), (uint32_t)key, p.thresh) ? p.inv_keep : 0.f;
+          pd[4 * i + r] = DROP ? pr * z : pr;
+          s[4 * i + r] = pr * ((DROP ? dp[4 * i + r] * z : dp[4 * i + r]) - d4[r]);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < Cr<T>::NF; ++f) {
+        const frag pf = Cr<T>::pack(pd, f), sf = Cr<T>::pack(s, f);
+#pragma unroll
+        for (int d = 0; d < Gm::DT; ++d) {
+          dv[d] = Cr<T>::mma(tr_frag<T, HDP>(sD + t * 32 * Gm::SR, Gm::SR, f, d, lane), pf, dv[d]);
+          dk[d] = Cr<T>::mma(tr_frag<T, HDP>(sQ + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, dk[d]);
+        }
+      }
+    }
+  };
+  // the samples that use this context, in order; the j-th one's blocks are numbered from j * per
+  uint32_t phase = (uint32_t)split;          // first block of the next sample that is this share's
+  auto sample = [&](int b) {
+    uint32_t u = phase;
+    for (; u < per; u += p.nsplit) block_of(b, u / nqc, u % nqc);
+    phase = u - per;
+  };
+  if (kblk * 128 < kn) {
+    if (!p.index) {
+      if (p.Bc == 1) for (int b = 0; b < p.B; ++b) sample(b);
+      else sample(ctx);
+    } else {
+      for (int b0 = 0; b0 < p.B; b0 += 64) {
+        unsigned long long hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
+        while (hit) {
+          const int b = b0 + __builtin_ctzll(hit);
+          hit &= hit - 1;
+          sample(b);
+        }
+      }
+    }
+  }
+  if (key >= p.Nk) return;
+  const float osc = valid ? p.scale : 0.f;
+  if (p.nsplit > 1) {
+    const long n = (long)p.Bc * p.Nk * p.G * p.hd;
+    float* dst = p.part + (long)split * 2 * n + (krow * p.G + g) * p.hd;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = d * 32 + 8 * i + 4 * half;
+        if (col < p.hd) {
+          *reinterpret_cast<f32x4*>(dst + col) = valid ? f32x4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
+          *reinterpret_cast<f32x4*>(dst + n + col) = valid ? f32x4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]} : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+    return;
+  }
+  char* ok = p.dk + krow * p.lddk + g * hdb;
+  char* ov = p.dv + krow * p.lddv + g * hdb;
+#pragma unroll
+  for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = d * 32 + 8 * i + 4 * half;
+      if (col >= p.hd) continue;
+      if (valid) {
+        store4<T>(ok + col * sizeof(T), dk[d][4 * i] * osc, dk[d][4 * i + 1] * osc, dk[d][4 * i + 2] * osc, dk[d][4 * i + 3] * osc);
+        store4<T>(ov + col * sizeof(T), dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]);
+      } else {
+        store4<T>(ok + col * sizeof(T), 0.f, 0.f, 0.f, 0.f);
+        store4<T>(ov + col * sizeof(T), 0.f, 0.f, 0.f, 0.f);
+      }
+    }
+}
+
+// adds the shares of dK / dV in order: thread = 4 channels of one key
+template <typename T>
+__global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p) {
+  const long n = (long)p.Bc * p.Nk * p.G * p.hd;
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * n) return;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < p.nsplit; ++k) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + (long)k * 2 * n + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += a[j];
+  }
+  const bool is_v = i >= n;
+  const long e = is_v ? i - n : i, w = (long)p.G * p.hd, row = e / w, col = e - row * w;
+  const float f = is_v ? 1.f : p.scale;
+  store4<T>((is_v ? p.dv + row * p.lddv : p.dk + row * p.lddk) + col * (long)sizeof(T), s[0] * f, s[1] * f, s[2] * f, s[3] * f);
+}
+
+constexpr int LDS_IMAGE = 80 * 1024;
+
+struct BwdPlan { int kb, iters, nqb, nsplit; bool res; long delta_bytes, ws; };
+int row_bytes(const dm_cross_args* a) { return cross_hdp(a->hd) * (a->dtype == 0 ? 2 : 4) + 16; }
+BwdPlan bwd_plan(const dm_cross_args* a) {
+  BwdPlan f{};
+  const long groups = ((long)a->Nq + 127) / 128, blocks = groups * a->B * a->heads;
+  const int image = (LDS_IMAGE - 512) / (2 * row_bytes(a)) / 64 * 64;
+  const int need = (a->Nk + 63) & ~63;
+  f.res = need <= image;
+  f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
+  f.iters = 1;
+  if (f.res) {
+    long it = blocks / 1536;
+    if (it > 8) it = 8;
+    if (it > groups) it = groups;
+    f.iters = it < 1 ? 1 : (int)it;
+  }
+  f.nqb = (int)((groups + f.iters - 1) / f.iters);
+  f.delta_bytes = (((long)a->B * a->heads * a->Nq + 3) & ~3L) * 4;
+  // shares of a context's query list: enough workgroups for four per CU, at least four blocks of queries each
+  const long owners = (long)a->Bc * a->kv_heads * ((a->Nk + 127) / 128);
+  const long list = (long)((a->B + a->Bc - 1) / a->Bc) * (a->heads / a->kv_heads) * ((a->Nq + QS - 1) / QS);
+  long ns = owners > 0 ? 1024 / owners : 1;
+  if (ns > list / 4) ns = list / 4;
+  f.nsplit = ns < 1 ? 1 : (int)ns;
+  f.ws = f.delta_bytes + (f.nsplit > 1 ? (long)f.nsplit * 2 * a->Bc * a->Nk * a->kv_heads * a->hd * 4 : 0);
+  return f;
+}
+
+template <typename T, int HDP, bool RES, bool DROP>
+int launch_dq(const CrossParams& p, hipStream_t st) {
+  auto kern = cross_dq_kernel<T, HDP, RES, DROP>;
+  static unsigned long long attr_devs = 0ull;
+  if (dm_first_on_device(attr_devs) &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
+    return DM_ERR_LAUNCH;
+  const size_t lds = (size_t)p.kb * 2 * Geo<T, HDP>::SR + (p.kb / 32 + 2) * 4;
+  const long blocks = (long)p.B * p.nqb * p.H;
+  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
+  DM_LAUNCH_CHECK();
+  return DM_OK;
+}
+template <typename T, int HDP, bool DROP>
+int launch_dkv(const CrossParams& p, hipStream_t st) {
+  auto kern = cross_dkv_kernel<T, HDP, DROP>;
+  const int lds = QS * 2 * Geo<T, HDP>::SR + QS * 12;
+  static unsigned long long attr_devs = 0ull;
+  if (dm_first_on_device(attr_devs) &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return DM_ERR_LAUNCH;
+  const long blocks = (long)p.Bc * p.nsplit * ((p.Nk + 127) / 128) * p.G;
+  if (blocks == 0) return DM_OK;
+  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
+  DM_LAUNCH_CHECK();
+  if (p.nsplit > 1) {
+    const long n = (long)2 * p.Bc * p.Nk * p.G * (p.hd >> 2), jb = (n + 255) / 256;
+    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((cross_sum_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
+    DM_LAUNCH_CHECK();
+  }
+  return DM_OK;
+}
+template <typename T, int HDP, bool DROP> int run_bwd(const CrossParams& p, bool res, hipStream_t st) {
+  const int rc = res ? launch_dq<T, HDP, true, DROP>(p, st) : launch_dq<T, HDP, false, DROP>(p, st);
+  if (rc != DM_OK) return rc;
+  static const DmVariantName nm("cross_bwd<%s,%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP);
+  dm_set_variant(nm.s);
+  return launch_dkv<T, HDP, DROP>(p, st);
+}
+template <typename T, int HDP> int pick_bwd(const CrossParams& p, bool res, hipStream_t st) {
+  return p.thresh ? run_bwd<T, HDP, true>(p, res, st) : run_bwd<T, HDP, false>(p, res, st);
+}
+template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t st) {
+  switch (cross_hdp(p.hd)) {
+    case 16: return pick_bwd<T, 16>(p, res, st);
+    case 32: return pick_bwd<T, 32>(p, res, st);
+    case 64: return pick_bwd<T, 64>(p, res, st);
+    case 96: return pick_bwd<T, 96>(p, res, st);
+    default: return pick_bwd<T, 128>(p, res, st);
+  }
+}
+
+}  // namespace
+
+extern "C" long dm_cross_bwd_workspace_bytes(const dm_cross_args* a) { return cross_sizes_ok(a) ? bwd_plan(a).ws : 0; }
+
+extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
+  CrossParams p{};
+  const int rc = cross_fill(p, a, true);
+  if (rc != DM_OK) return rc;
+  const BwdPlan f = bwd_plan(a);
+  DM_REQUIRE(a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0);
+  p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb; p.nsplit = f.nsplit;
+  p.delta = (float*)a->workspace;
+  p.part = (float*)((char*)a->workspace + f.delta_bytes);
+  return a->dtype == 0 ? pick_width<bf16>(p, f.res, (hipStream_t)stream) : pick_width<float>(p, f.res, (hipStream_t)stream);
+}

@@ -1,0 +1,322 @@
+// Attention to an encoder's states of another length, forward (include/dm_hip.h: dm_cross_fwd).
+//
+//   S^T = K Q^T (keys on the rows of the tile, queries on the lanes), P = exp2(c S - c m), c = scale log2(e), m the running
+//   maximum of the lane's query;  O^T += V^T P^T;  l += sum P;  o = O / l, lse = scale m + ln l.
+// The row sum takes the fp32 probabilities before they are rounded for the second product, so lse is an fp32 value.
+#include "dm_cross.h"
+
+namespace {
+
+template <typename T, int HDP> struct FwdState {
+  f32x16 acc[Geo<T, HDP>::DT];
+  float m, l;
+};
+
+// NT tiles of 32 keys (LDS rows t0..) against the wave's 32 queries
+template <typename T, int HDP, int NT, bool DROP>
+__device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>& st, const char* sK, const char* sV,
+                                         const uint32_t* bits, int t0, int key0, float c,
+                                         const typename Cr<T>::frag (&qf)[Geo<T, HDP>::NC], uint32_t rs, int lane) {
+  typedef Geo<T, HDP> Gm;
+  const int half = lane >> 5;
+  uint32_t w[NT], any = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    w[t] = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t0 + t]);
+    any |= w[t];
+  }
+  if (any == 0) return;
+  f32x16 s[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < Gm::NC; ++kc)
+      s[t] = Cr<T>::mma(row_frag<T>(sK + (t0 + t) * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s[t]);
+    if (w[t] != 0xFFFFFFFFu) {
+      const uint32_t mine = w[t] >> (4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = (mine >> tile_row(i, 0)) & 1u ? s[t][i] : -INFINITY;
+    }
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+  mx = half_max(mx);
+  // the reference maximum moves only when a block exceeds it by more than 2^8 in the probability: exact all the same
+  // (numerator and denominator share it), and the common block rescales nothing
+  const bool up = (mx - st.m) * c > 8.f;
+  if (__any(up)) {
+    const float alpha = up ? __builtin_amdgcn_exp2f((st.m - mx) * c) : 1.f;
+    st.m = up ? mx : st.m;
+    st.l *= alpha;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[d][i] *= alpha;
+  }
+  const float mc = st.m == -INFINITY ? 0.f : st.m * c;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -mc));
+      st.l += s[t][i];
+    }
+    if (DROP) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t key = key0 + t * 32 + tile_row(i, half), z = dm_drop_bits(rs, key >> 1);
+        if (!dm_keep16(z, 0, p.thresh)) s[t][i] = 0.f;
+        if (!dm_keep16(z, 1, p.thresh)) s[t][i + 1] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < Cr<T>::NF; ++f) {
+      const typename Cr<T>::frag pf = Cr<T>::pack(s[t], f);
+#pragma unroll
+      for (int d = 0; d < Gm::DT; ++d)
+        st.acc[d] = Cr<T>::mma(tr_frag<T, HDP>(sV + (t0 + t) * 32 * Gm::ST, Gm::ST, f, d, lane), pf, st.acc[d]);
+    }
+  }
+}
+
+template <typename T, int HDP>
+__device__ __forceinline__ void fwd_finish(const CrossParams& p, const FwdState<T, HDP>& st, int b, int h, int q, int split,
+                                           float c, int lane) {
+  typedef Geo<T, HDP> Gm;
+  const int half = lane >> 5;
+  const float l = half_sum(st.l);
+  const float mc = st.m == -INFINITY ? 0.f : st.m * c;
+  if (q >= p.Nq) return;
+  const long row = ((long)b * p.H + h) * p.Nq + q;
+  if (p.nsplit > 1) {
+    const long rows = (long)p.B * p.H * p.Nq;
+    float* o = p.part + (split * rows + row) * p.hd;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = d * 32 + 8 * i + 4 * half;
+        if (col < p.hd) *reinterpret_cast<f32x4*>(o + col) = f32x4{st.acc[d][4 * i], st.acc[d][4 * i + 1], st.acc[d][4 * i + 2], st.acc[d][4 * i + 3]};
+      }
+    if (half == 0) {
+      float* ml = p.part + p.nsplit * rows * p.hd + (split * rows + row) * 2;
+      ml[0] = mc;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : p.inv_keep / l;
+  char* o = p.o + ((long)b * p.Nq + q) * p.ldo + h * p.hd * (long)sizeof(T);
+#pragma unroll
+  for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = d * 32 + 8 * i + 4 * half;
+      if (col < p.hd)
+        store4<T>(o + col * sizeof(T), st.acc[d][4 * i] * inv, st.acc[d][4 * i + 1] * inv, st.acc[d][4 * i + 2] * inv, st.acc[d][4 * i + 3] * inv);
+    }
+  if (half == 0) p.lse[row] = l == 0.f ? -INFINITY : (mc + log2f(l)) * CR_LN2;
+}
+
+// A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
+// LDS image, which is staged once for all the tiles; otherwise images of p.kb keys follow each other (iters is 1).
+template <typename T, int HDP, bool RES, bool DROP>
+__global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) {
+  typedef Geo<T, HDP> Gm;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* sK = smem;
+  char* sV = sK + p.kb * Gm::SR;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(sV + p.kb * Gm::ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int h = id % p.H;
+  id /= p.H;
+  const int qb = id % p.nqb;
+  id /= p.nqb;
+  const int split = id % p.nsplit, b = id / p.nsplit;
+  const int ctx = context_of(p, b), kn = keys_of(p, ctx);
+  const int k0 = p.nsplit > 1 ? split * p.ksplit : 0;
+  const int k1 = p.nsplit > 1 ? min(kn, k0 + p.ksplit) : kn;
+  const int hdb = p.hd * (int)sizeof(T), g = h / (p.H / p.G);
+  const long krow = (long)(ctx < 0 ? 0 : ctx) * p.Nk;
+  const char* kbase = p.k + krow * p.ldk + g * hdb;
+  const char* vbase = p.v + krow * p.ldv + g * hdb;
+  const unsigned char* mask = p.mask ? p.mask + krow : nullptr;
+  const float c = p.scale * CR_LOG2E;
+  const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
+
+  FwdState<T, HDP> st;
+  typename Cr<T>::frag qf[Gm::NC];
+  uint32_t rs = 0;
+  auto begin = [&](int q) {
+    load_frags<T, HDP>(p.q + ((long)b * p.Nq + q) * p.ldq + h * hdb, q < p.Nq, hdb, lane, qf);
+    if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q));
+    st.m = -INFINITY;
+    st.l = 0.f;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[d][i] = 0.f;
+  };
+  auto stage = [&](int from, int n) {
+    stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, k1, mask, hdb, tid);
+    stage_rows<T, HDP>(sV, Gm::ST, vbase, p.ldv, from, n, k1, mask, hdb, tid);
+    stage_bits(bits, from, n, k1, mask, tid);
+  };
+  auto sweep = [&](int from, int tiles) {
+    int t = 0;
+    for (; t + 2 <= tiles; t += 2) fwd_step<T, HDP, 2, DROP>(p, st, sK, sV, bits, t, from + t * 32, c, qf, rs, lane);
+    if (t < tiles) fwd_step<T, HDP, 1, DROP>(p, st, sK, sV, bits, t, from + t * 32, c, qf, rs, lane);
+  };
+  const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
+  if (RES) {
+    const int n = max(0, (k1 - k0 + 31) & ~31);
+    stage(k0, n);
+    __syncthreads();
+    for (int it = 0; it < p.iters; ++it) {
+      const int q = q0 + it * 128;
+      if (q - (lane & 31) >= p.Nq) break;      // (wave-uniform)
+      begin(q);
+      sweep(k0, n >> 5);
+      fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
+    }
+  } else {
+    begin(q0);
+    for (int from = k0; from < k1; from += p.kb) {
+      const int n = min(p.kb, (k1 - from + 31) & ~31);
+      __syncthreads();
+      stage(from, n);
+      __syncthreads();
+      sweep(from, n >> 5);
+    }
+    fwd_finish<T, HDP>(p, st, b, h, q0, split, c, lane);
+  }
+}
+
+// joins the key splits: thread = (row, 4 channels)
+template <typename T>
+__global__ __launch_bounds__(256) void cross_join_kernel(const CrossParams p) {
+  const long rows = (long)p.B * p.H * p.Nq;
+  const int per = p.hd >> 2;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const long row = i / per;
+  const int col = (int)(i - row * per) * 4;
+  const float* ml = p.part + p.nsplit * rows * p.hd + row * 2;
+  float m = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s)
+    if (ml[s * rows * 2 + 1] != 0.f) m = fmaxf(m, ml[s * rows * 2]);
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float ls = ml[s * rows * 2 + 1];
+    if (ls == 0.f) continue;
+    const float w = __builtin_amdgcn_exp2f(ml[s * rows * 2] - m);
+    l += w * ls;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * p.hd + col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += w * a[j];
+  }
+  const float inv = l == 0.f ? 0.f : p.inv_keep / l;
+  const long bh = row / p.Nq, q = row - bh * p.Nq, b = bh / p.H;
+  const int h = (int)(bh - b * p.H);
+  store4<T>(p.o + (b * p.Nq + q) * p.ldo + (h * p.hd + col) * (long)sizeof(T), o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (col == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * CR_LN2;
+}
+
+constexpr int LDS_IMAGE = 80 * 1024;     // two workgroups per CU
+
+int key_bytes(const dm_cross_args* a) {
+  const int hdp = cross_hdp(a->hd);
+#define DM_KEYB(HDP) if (hdp == HDP) return a->dtype == 0 ? Geo<bf16, HDP>::SR + Geo<bf16, HDP>::ST : Geo<float, HDP>::SR + Geo<float, HDP>::ST
+  DM_KEYB(16); DM_KEYB(32); DM_KEYB(64); DM_KEYB(96); DM_KEYB(128);
+#undef DM_KEYB
+  return 0;
+}
+
+struct FwdPlan { int nsplit, ksplit, kb, iters, nqb; bool res; long ws; };
+FwdPlan fwd_plan(const dm_cross_args* a) {
+  FwdPlan f{};
+  const long groups = ((long)a->Nq + 127) / 128;              // workgroups along the queries at one tile per wave
+  const long blocks = groups * a->B * a->heads;
+  // few rows: the keys are split (at least 128 each) until there are about four workgroups per CU
+  long ns = 1;
+  if (blocks < 512 && a->Nk >= 256) {
+    ns = (1024 + blocks - 1) / blocks;
+    if (ns > a->Nk / 128) ns = a->Nk / 128;
+  }
+  f.ksplit = ns > 1 ? (int)((((long)a->Nk + ns - 1) / ns + 63) & ~63L) : a->Nk;
+  f.nsplit = ns > 1 ? (a->Nk + f.ksplit - 1) / f.ksplit : 1;
+  const int kbytes = key_bytes(a);
+  const int image = (LDS_IMAGE - 512) / kbytes / 64 * 64;     // keys per LDS image
+  const int need = (f.ksplit + 63) & ~63;
+  f.res = need <= image;
+  f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
+  // resident keys serve several query tiles per wave, as long as there are about six workgroups per CU
+  f.iters = 1;
+  if (f.res) {
+    long it = blocks * f.nsplit / 1536;
+    if (it > 8) it = 8;
+    if (it > groups) it = groups;
+    f.iters = it < 1 ? 1 : (int)it;
+  }
+  f.nqb = (int)((groups + f.iters - 1) / f.iters);
+  f.ws = f.nsplit > 1 ? (long)f.nsplit * a->B * a->heads * a->Nq * (a->hd + 2) * 4 : 0;
+  return f;
+}
+
+template <typename T, int HDP, bool RES, bool DROP>
+int launch_fwd(const CrossParams& p, hipStream_t st) {
+  auto kern = cross_fwd_kernel<T, HDP, RES, DROP>;
+  static unsigned long long attr_devs = 0ull;
+  if (dm_first_on_device(attr_devs) &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
+    return DM_ERR_LAUNCH;
+  const size_t lds = (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST) + (p.kb / 32 + 2) * 4;
+  const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
+  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, RES ? "resident" : "streamed");
+  dm_set_variant(nm.s);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
+  DM_LAUNCH_CHECK();
+  if (p.nsplit > 1) {
+    const long n = (long)p.B * p.H * p.Nq * (p.hd >> 2), jb = (n + 255) / 256;
+    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((cross_join_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
+    DM_LAUNCH_CHECK();
+  }
+  return DM_OK;
+}
+template <typename T, int HDP> int pick_fwd(const CrossParams& p, bool res, hipStream_t st) {
+  if (res) return p.thresh ? launch_fwd<T, HDP, true, true>(p, st) : launch_fwd<T, HDP, true, false>(p, st);
+  return p.thresh ? launch_fwd<T, HDP, false, true>(p, st) : launch_fwd<T, HDP, false, false>(p, st);
+}
+template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t st) {
+  switch (cross_hdp(p.hd)) {
+    case 16: return pick_fwd<T, 16>(p, res, st);
+    case 32: return pick_fwd<T, 32>(p, res, st);
+    case 64: return pick_fwd<T, 64>(p, res, st);
+    case 96: return pick_fwd<T, 96>(p, res, st);
+    default: return pick_fwd<T, 128>(p, res, st);
+  }
+}
+
+}  // namespace
+
+extern "C" long dm_cross_fwd_workspace_bytes(const dm_cross_args* a) { return cross_sizes_ok(a) ? fwd_plan(a).ws : 0; }
+
+extern "C" int dm_cross_fwd(const dm_cross_args* a, dm_stream_t stream) {
+  CrossParams p{};
+  const int rc = cross_fill(p, a, false);
+  if (rc != DM_OK) return rc;
+  const FwdPlan f = fwd_plan(a);
+  DM_REQUIRE(f.ws == 0 || (a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0));
+  p.nsplit = f.nsplit; p.ksplit = f.ksplit; p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb;
+  p.part = (float*)a->workspace;
+  return a->dtype == 0 ? pick_width<bf16>(p, f.res, (hipStream_t)stream) : pick_width<float>(p, f.res, (hipStream_t)stream);
+}

@@ -5,13 +5,14 @@ contiguous; slices along the channel dim are allowed (pixel stride = stride(-2))
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, ConvArgs, Cross1Args, GemmArgs, WgradArgs, check
+from ._lib import AttnArgs, ConvArgs, Cross1Args, CrossArgs, GemmArgs, RopeArgs, WgradArgs, check
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -715,6 +716,204 @@ def cross1_bwd(dy, v, w_out, heads, *, dw_out=None, drop_p=0.0, drop_seed=0):
     a.workspace, a.ws_bytes = _p(ws), ws.numel()
     check(_lib.lib().dm_cross1_bwd(C.byref(a), _stream()), "dm_cross1_bwd")
     return dv
+
+
+# --------------------------------------------------------------------------- rotary positions
+class RopePlan:
+    """What rope() needs beside the data: per channel pair its axis and its frequency, in turns per unit of position
+    (64 bits).  Made once by rope_plan() and kept, like the weights of the projection whose heads it rotates."""
+
+    __slots__ = ("head_dim", "axes", "rot", "theta", "pairing", "freq", "axis")
+
+    def __init__(self, head_dim, axes, theta, pairing, freq, axis):
+        self.head_dim, self.axes, self.rot, self.theta, self.pairing = head_dim, axes, sum(axes), theta, pairing
+        self.freq, self.axis = freq, axis
+
+
+def rope_plan(head_dim: int, axes, *, theta: float = 10000.0, pairing: str = "interleaved", device=None) -> RopePlan:
+    """``axes``: the channels of a head that each position axis rotates (time, height, width; one to three even numbers
+    whose sum is at most ``head_dim`` -- the channels behind them are left as they are).  Pair i of an axis with d channels
+    turns by theta^(-2i/d) radians per unit of position.  ``pairing``: "interleaved" (channels 2p and 2p+1) or "half"
+    (channels p and p + R/2 of the R rotated ones)."""
+    axes = tuple(int(d) for d in axes)
+    if not 1 <= len(axes) <= 3 or any(d < 2 or d % 2 for d in axes):
+        raise ValueError(f"rope_plan: one to three axes of an even number of channels, got {axes}")
+    if head_dim % 2 or not sum(axes) <= head_dim <= 2048:
+        raise ValueError(f"rope_plan: head_dim must be even, at most 2048 and hold the axes' {sum(axes)} channels, got {head_dim}")
+    if pairing not in ("interleaved", "half"):
+        raise ValueError(f"rope_plan: pairing must be 'interleaved' or 'half', got {pairing!r}")
+    if not 0.0 < theta < float("inf"):
+        raise ValueError("rope_plan: theta must be positive")
+    freq = torch.tensor([theta ** (-2.0 * i / d) / (2.0 * math.pi) for d in axes for i in range(d // 2)], dtype=torch.float64)
+    axis = torch.tensor([a for a, d in enumerate(axes) for _ in range(d // 2)], dtype=torch.int32)
+    dev = torch.device("cuda" if device is None else device)
+    return RopePlan(int(head_dim), axes, float(theta), pairing, freq.to(dev), axis.to(dev))
+
+
+def rope(x, heads: int, plan: RopePlan, *, grid=None, positions=None, inverse: bool = False, out=None):
+    """Rotary positions on every head of x [B, N, heads * head_dim] (dm_rope, include/dm_hip.h); bf16 or fp32, rows may be
+    strided: the query and key slices of a fused projection are rotated in one call as x = qkv[..., :2C] with 2 * heads.
+    Where the tokens sit: ``grid`` = the extents of the plan's axes, tokens in row-major order; or ``positions``, int32 or
+    float32 [N, axes] or [B, N, axes] (crops, packed images, text tokens).  ``inverse=True`` turns back, which is the backward:
+    dx = rope(dy, ..., inverse=True).  ``out`` may be x itself."""
+    if x.dim() != 3 or x.dtype not in (BF16, F32):
+        raise ValueError("rope: x must be a bf16 or float32 tensor [B, N, heads * head_dim]")
+    B, N, Cc = x.shape
+    if heads < 1 or Cc != heads * plan.head_dim:
+        raise ValueError(f"rope: {Cc} channels are not {heads} heads of {plan.head_dim}")
+    if Cc >= 65536:
+        raise ValueError("rope: at most 65535 channels")
+    nax = len(plan.axes)
+    if (grid is None) == (positions is None):
+        raise ValueError("rope: give either grid or positions")
+    if grid is not None:
+        grid = tuple(int(n) for n in grid)
+        if len(grid) != nax or any(n < 1 for n in grid) or math.prod(grid) != N:
+            raise ValueError(f"rope: grid {grid} does not place {N} tokens on {nax} axes")
+    else:
+        if positions.dtype not in (torch.int32, F32) or not positions.is_contiguous():
+            raise ValueError("rope: positions must be contiguous int32 or float32")
+        if tuple(positions.shape) not in ((N, nax), (B, N, nax)):
+            raise ValueError(f"rope: positions must be [{N}, {nax}] or [{B}, {N}, {nax}], got {tuple(positions.shape)}")
+    if out is None:
+        out = torch.empty((B, N, Cc), dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("rope: out must have x's shape and type")
+    _same_device("rope", x, out, plan.freq, plan.axis, positions)
+    if x.numel() == 0:
+        return out
+    a = RopeArgs()
+    a.x, a.ldx, a.y, a.ldy = _p(x), _act(x, "x"), _p(out), _act(out, "out")
+    a.dtype, a.B, a.N, a.heads, a.hd, a.rot = int(_is32(x)), B, N, heads, plan.head_dim, plan.rot
+    a.pairing, a.freq, a.axis, a.axes = int(plan.pairing == "half"), _p(plan.freq), _p(plan.axis), nax
+    if positions is not None:
+        a.pos, a.pos_f32 = _p(positions), int(positions.dtype == F32)
+        a.pos_batch_stride = N * nax if positions.dim() == 3 else 0
+    else:
+        for i, n in enumerate(grid):
+            a.grid[i] = n
+    a.inverse = int(inverse)
+    check(_lib.lib().dm_rope(C.byref(a), _stream()), "dm_rope")
+    return out
+
+
+def _same_device(what: str, *tensors) -> None:
+    """Every operand on the current HIP device: kernels go to that device's current stream."""
+    if _FORCED_STREAM[0] is None:
+        for t in tensors:
+            if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
+                raise ValueError(f"{what}: every tensor must be on the current GPU, got {t.device}")
+
+
+# --------------------------------------------------------------------------- attention to encoder states
+def _cross_args(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed):
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in (BF16, F32):
+        raise ValueError(f"{what}: q must be [B, Nq, heads * hd] and k, v [Bc, Nk, kv_heads * hd], bf16 or float32")
+    if k.dtype != q.dtype or v.dtype != q.dtype or v.shape != k.shape:
+        raise ValueError(f"{what}: k and v must have one shape, and q's type")
+    kv_heads = heads if kv_heads is None else kv_heads
+    B, Nq, Cq = q.shape
+    Bc, Nk, Ck = k.shape
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or Cq % heads or Ck * heads != Cq * kv_heads:
+        raise ValueError(f"{what}: {Cq} / {Ck} channels do not make {heads} query heads on {kv_heads} key / value heads")
+    hd = Cq // heads
+    if hd % 8 or not 8 <= hd <= 128:
+        raise ValueError(f"{what}: head width {hd} is not a multiple of 8 up to 128")
+    if index is None and Bc not in (1, B):
+        raise ValueError(f"{what}: {Bc} contexts for {B} samples need an index")
+    if Bc == 0 and B > 0:
+        raise ValueError(f"{what}: no context")
+    for t, name, shape, types in ((lens, "lens", (Bc,), (torch.int32,)), (index, "index", (B,), (torch.int32,)),
+                                  (mask, "mask", (Bc, Nk), (torch.bool, torch.uint8))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype not in types or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous {types[0]} tensor of shape {shape}")
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"{what}: scale must be positive")
+    if not 0.0 <= drop_p < 1.0:
+        raise ValueError(f"{what}: drop_p must be in [0, 1)")
+    _same_device(what, q, k, v, lens, mask, index)
+    a = CrossArgs()
+    a.B, a.Bc, a.heads, a.kv_heads, a.Nq, a.Nk, a.hd, a.dtype = B, Bc, heads, kv_heads, Nq, Nk, hd, int(_is32(q))
+    a.scale, a.drop_p, a.drop_seed = scale, float(drop_p), int(drop_seed)
+    a.lens, a.mask, a.index = _p(lens), _p(mask), _p(index)
+    a.q, a.ldq = _rows16(what, "q", q)
+    if Nk:
+        (a.k, a.ldk), (a.v, a.ldv) = _rows16(what, "k", k), _rows16(what, "v", v)
+    return a
+
+
+def _rows16(what, name, t):
+    if t.numel() == 0:
+        return None, t.shape[-1]
+    ld = _act(t, name)
+    if t.data_ptr() % 16 or ld * t.element_size() % 16:
+        raise ValueError(f"{what}: the rows of {name} must be 16-byte aligned")
+    return _p(t), ld
+
+
+def _cross_out(what, name, t, like):
+    if t is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{what}: {name} must have the shape {tuple(like.shape)} and the operands' type")
+    _same_device(what, t)
+    return t
+
+
+def cross_fwd(q, k, v, heads: int, *, kv_heads: Optional[int] = None, lens=None, mask=None, index=None,
+              scale: Optional[float] = None, drop_p: float = 0.0, drop_seed: int = 0, out=None):
+    """Attention of q [B, Nq, heads*hd] to an encoder's states k, v [Bc, Nk, kv_heads*hd] -> (o [B, Nq, heads*hd],
+    lse [B, heads, Nq] fp32) (dm_cross_fwd, include/dm_hip.h); bf16 or fp32, views into fused buffers are fine.
+    ``lens`` int32 [Bc]: the first lens[c] states of context c are valid; ``mask`` bool [Bc, Nk]: True where valid (both:
+    their intersection); what invalid states hold does not matter, and a sample without any valid state gets o = 0 and
+    lse = -inf.  ``index`` int32 [B]: the context of each sample (without it: one each, or Bc == 1 for all); an index
+    outside [0, Bc) means no states.  ``kv_heads``: key / value heads, each shared by heads / kv_heads query heads."""
+    a = _cross_args("cross_fwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed)
+    out = _cross_out("cross_fwd", "out", out, q)
+    lse = torch.empty((a.B, heads, a.Nq), dtype=F32, device=q.device)
+    if out.numel() == 0:
+        return out, lse
+    a.o, a.ldo = _rows16("cross_fwd", "out", out)
+    a.lse = _p(lse)
+    L = _lib.lib()
+    nb = L.dm_cross_fwd_workspace_bytes(C.byref(a))
+    if nb:
+        # a block of its own per call, not the shared workspace(): the allocator orders it on this stream, and graphs
+        # captured from two calls never share it
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+        a.workspace, a.ws_bytes = _p(ws), nb
+    check(L.dm_cross_fwd(C.byref(a), _stream()), "dm_cross_fwd")
+    return out, lse
+
+
+def cross_bwd(q, k, v, o, lse, d_o, heads: int, *, kv_heads: Optional[int] = None, lens=None, mask=None, index=None,
+              scale: Optional[float] = None, drop_p: float = 0.0, drop_seed: int = 0, dq=None, dk=None, dv=None):
+    """Backward of cross_fwd with the same options: (dq, dk, dv) in q's, k's and v's shapes.  dk and dv are sums over the
+    query heads of a group and over the samples that share a context, in a fixed order; rows of invalid states are zero."""
+    a = _cross_args("cross_bwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed)
+    for t, name in ((o, "o"), (d_o, "d_o")):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"cross_bwd: {name} must have q's shape and type")
+    if tuple(lse.shape) != (a.B, heads, a.Nq) or lse.dtype != F32 or not lse.is_contiguous():
+        raise ValueError("cross_bwd: lse must be cross_fwd's")
+    _same_device("cross_bwd", o, d_o, lse)
+    dq = _cross_out("cross_bwd", "dq", dq, q)
+    dk, dv = _cross_out("cross_bwd", "dk", dk, k), _cross_out("cross_bwd", "dv", dv, v)
+    if q.numel() == 0:
+        return dq, dk.zero_(), dv.zero_()
+    a.o, a.ldo = _rows16("cross_bwd", "o", o)
+    a.d_o, a.lddo = _rows16("cross_bwd", "d_o", d_o)
+    a.dq, a.lddq = _rows16("cross_bwd", "dq", dq)
+    a.dk, a.lddk = _rows16("cross_bwd", "dk", dk)
+    a.dv, a.lddv = _rows16("cross_bwd", "dv", dv)
+    a.lse = _p(lse)
+    L = _lib.lib()
+    nb = L.dm_cross_bwd_workspace_bytes(C.byref(a))
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+    a.workspace, a.ws_bytes = _p(ws), nb
+    check(L.dm_cross_bwd(C.byref(a), _stream()), "dm_cross_bwd")
+    return dq, dk, dv
 
 
 # --------------------------------------------------------------------------- layout / elementwise

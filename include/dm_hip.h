@@ -34,7 +34,8 @@ typedef void* dm_stream_t;
 /* ABI version / arch string ("gfx950").  Version 2 (round 2): dm_conv_args / dm_wgrad_args grew the trailing
  * norm_scale / norm_shift fields.  Version 3: dm_attn_args grew the trailing workspace / ws_bytes fields and
  * dm_attn_bwd_workspace_bytes, dm_film_fwd / dm_film_bwd were added.  Version 4 (round 3): the fp32 compute mode (the *_f32
- * entry points at the end of this header); nothing older changed.  Callers built against an older version must be rebuilt. */
+ * entry points at the end of this header); nothing older changed; dm_cross_* and dm_rope were added to it since.  Callers
+ * built against an older version must be rebuilt. */
 int dm_abi_version(void);
 const char* dm_target_arch(void);
 /* Text of the HIP error behind the calling thread's last DM_ERR_LAUNCH ("" if none). */
@@ -230,6 +231,62 @@ typedef struct dm_cross1_args {
 int dm_cross1_fwd(const dm_cross1_args* args, dm_stream_t stream);
 int dm_cross1_bwd(const dm_cross1_args* args, dm_stream_t stream);
 long dm_cross1_bwd_workspace_bytes(int B, int heads, int C);
+
+/* ------------------------------------------------------------------ attention to an encoder's states of another length
+ * o = softmax(scale q k^T over the VALID keys) v for queries [B, Nq] and states [Bc, Nk] (reference unet.py:141-220, where
+ * every token of every sample counts; here each context has its own valid length and, optionally, a mask with holes).
+ *   - head h of heads reads key / value head h / (heads / kv_heads) (kv_heads = heads: one each).
+ *   - context of sample b: index ? index[b] : (Bc == 1 ? 0 : b).  An index outside [0, Bc) means a sample without keys.
+ *     Samples may share a context: its keys and values exist once, its gradients are the sums over the samples.
+ *   - key j of context c is valid iff j < lens[c] (NULL: Nk; values are clamped to [0, Nk]) and mask[c][j] != 0 (NULL: all).
+ *     What invalid rows of k and v hold does not matter (NaN and infinities included).
+ *   - a query with no valid key: o = 0, lse = -infinity, and no gradient flows.
+ * hd: a multiple of 8 up to 128.  Rows of every activation are 16-byte aligned.  Scores, softmax statistics and accumulators
+ * are fp32; with dtype 0 the probabilities (and in the backward the score gradients) are rounded to bf16 for the second
+ * matrix product, like the inputs.  Dropout words as dm_attn_fwd's for 64- and 128-wide heads. */
+typedef struct dm_cross_args {
+  const void* q; long ldq;        /* [B, Nq, heads*hd] */
+  const void* k; long ldk;        /* [Bc, Nk, kv_heads*hd] */
+  const void* v; long ldv;
+  void* o; long ldo;              /* [B, Nq, heads*hd]: written by the forward, read by the backward */
+  float* lse;                     /* [B, heads, Nq] natural log of sum exp(scale*s); as o */
+  const void* d_o; long lddo;     /* backward only */
+  void* dq; long lddq; void* dk; long lddk; void* dv; long lddv;   /* written whole: rows of invalid keys are zero */
+  const int* lens;                /* [Bc] or NULL */
+  const unsigned char* mask;      /* [Bc, Nk] contiguous, or NULL */
+  const int* index;               /* [B] or NULL */
+  int B, Bc, heads, kv_heads, Nq, Nk, hd;
+  int dtype;                      /* 0: bf16, 1: fp32 (every activation and gradient) */
+  float scale;
+  float drop_p; unsigned long long drop_seed;
+  void* workspace; long ws_bytes; /* >= dm_cross_fwd_workspace_bytes / dm_cross_bwd_workspace_bytes; 16-byte aligned */
+} dm_cross_args;
+/* Scratch for these sizes (0: none needed); only B, Bc, heads, kv_heads, Nq, Nk, hd and dtype are read. */
+long dm_cross_fwd_workspace_bytes(const dm_cross_args* args);
+long dm_cross_bwd_workspace_bytes(const dm_cross_args* args);
+int dm_cross_fwd(const dm_cross_args* args, dm_stream_t stream);
+int dm_cross_bwd(const dm_cross_args* args, dm_stream_t stream);
+
+/* ------------------------------------------------------------------ rotary positions
+ * Rotary embedding with up to three position axes on every head of x [B, N, heads*hd] (an image or video's query / key
+ * projection before dm_attn_fwd, reference unet.py:119-126, which has no positions): pair p turns by
+ * position[axis[p]] * freq[p] TURNS (freq = theta^(-2i/d) / (2 pi), doubles); channels >= rot are copied.  Angles are reduced
+ * in 64 bits.  inverse: the opposite angle, which is the backward.  y may be x itself. */
+typedef struct dm_rope_args {
+  const void* x; long ldx;        /* [B*N] rows of heads*hd */
+  void* y; long ldy;
+  int dtype;                      /* 0: bf16, 1: fp32 */
+  int B, N, heads, hd, rot;       /* hd and rot even, heads*hd < 65536 */
+  int pairing;                    /* 0: channels (2p, 2p+1); 1: (p, p + rot/2) */
+  const double* freq;             /* [rot/2] device */
+  const int* axis;                /* [rot/2] device, values in [0, axes) */
+  int axes;                       /* 1..3 */
+  const void* pos;                /* int32 or fp32 [N, axes] (pos_batch_stride 0) or [B, N, axes] (N*axes), device; or NULL */
+  int pos_f32; long pos_batch_stride;
+  int grid[3];                    /* pos NULL: token n sits at its row-major place in grid[0..axes), product N */
+  int inverse;
+} dm_rope_args;
+int dm_rope(const dm_rope_args* args, dm_stream_t stream);
 
 /* ------------------------------------------------------------------ layout / elementwise */
 /* NCHW fp32 -> NHWC bf16, channels zero-padded to Cpad (UNET.forward entry, unet.py:344). */

@@ -1,0 +1,136 @@
+"""CPU: what the rotary and cross-attention front-ends refuse, and that the C entries refuse it too (no launch is made: every
+case here is turned away before one)."""
+import ctypes
+
+import pytest
+import torch
+
+from diffusion_model_amd import _lib
+from diffusion_model_amd import kernels as K
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def plan(hd=32, axes=(16, 16), **kw):
+    return K.rope_plan(hd, axes, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("hd,axes,kw", [
+    (32, (), {}), (32, (8, 8, 8, 8), {}), (32, (15,), {}), (32, (0, 16), {}), (32, (32, 2), {}), (33, (16,), {}),
+    (2050, (16,), {}), (32, (16,), dict(pairing="other")), (32, (16,), dict(theta=0.0)), (32, (16,), dict(theta=float("inf")))])
+def test_rope_plan_refusals(hd, axes, kw):
+    with pytest.raises(ValueError):
+        plan(hd, axes, **kw)
+
+
+def test_rope_plan_values():
+    import math
+    p = plan(40, (4, 6), theta=100.0)
+    want = [100.0 ** (-2 * i / d) / (2 * math.pi) for d in (4, 6) for i in range(d // 2)]
+    assert p.freq.tolist() == want and p.axis.tolist() == [0, 0, 1, 1, 1] and p.rot == 10
+
+
+X = torch.zeros(2, 6, 64)
+
+
+@pytest.mark.parametrize("x,heads,kw", [
+    (X[0], 2, dict(grid=(2, 3))), (X.half(), 2, dict(grid=(2, 3))), (X, 3, dict(grid=(2, 3))), (X, 0, dict(grid=(2, 3))),
+    (X, 2, {}), (X, 2, dict(grid=(2, 3), positions=torch.zeros(6, 2))), (X, 2, dict(grid=(2, 4))), (X, 2, dict(grid=(6,))),
+    (X, 2, dict(grid=(-2, -3))), (X, 2, dict(positions=torch.zeros(6, 3))), (X, 2, dict(positions=torch.zeros(3, 6, 2))),
+    (X, 2, dict(positions=torch.zeros(6, 2, dtype=torch.int64))), (X, 2, dict(positions=torch.zeros(2, 6).T)),
+    (X, 2, dict(grid=(2, 3), out=torch.zeros(2, 6, 32))), (X, 2, dict(grid=(2, 3), out=X.to(BF16))),
+    (torch.zeros(1, 1, 65536), 2048, dict(grid=(1, 1))),
+    (X, 2, dict(grid=(2, 3)))])                       # the last one: everything fits, but no tensor is on the GPU
+def test_rope_refusals(x, heads, kw):
+    with pytest.raises(ValueError):
+        K.rope(x, heads, plan(), **kw)
+
+
+Q, KV = torch.zeros(2, 5, 64), torch.zeros(2, 7, 64)
+
+
+@pytest.mark.parametrize("q,k,v,heads,kw", [
+    (Q[0], KV, KV, 2, {}), (Q, KV[0], KV[0], 2, {}), (Q.half(), KV.half(), KV.half(), 2, {}), (Q.to(BF16), KV, KV, 2, {}),
+    (Q, KV, KV[:, :5], 2, {}), (Q, KV, KV.to(BF16), 2, {}), (Q, KV, KV, 3, {}), (Q, KV, KV, 0, {}), (Q, KV, KV, 2, dict(kv_heads=1)),
+    (Q, KV, KV, 4, dict(kv_heads=3)), (Q, KV, KV, 2, dict(kv_heads=0)),
+    (Q, KV, KV, 16, {}),                                                               # head width 4
+    (torch.zeros(2, 5, 272), torch.zeros(2, 7, 272), torch.zeros(2, 7, 272), 2, {}),   # head width 136
+    (torch.zeros(4, 5, 64), KV, KV, 2, {}),                                            # 2 contexts for 4 samples
+    (Q, KV[:0], KV[:0], 2, dict(index=torch.zeros(2, dtype=torch.int32))),
+    (Q, KV, KV, 2, dict(lens=torch.zeros(2))), (Q, KV, KV, 2, dict(lens=torch.zeros(3, dtype=torch.int32))),
+    (Q, KV, KV, 2, dict(index=torch.zeros(2, dtype=torch.int64))), (Q, KV, KV, 2, dict(index=torch.zeros(1, dtype=torch.int32))),
+    (Q, KV, KV, 2, dict(mask=torch.zeros(2, 7))), (Q, KV, KV, 2, dict(mask=torch.zeros(7, 2, dtype=torch.bool).T)),
+    (Q, KV, KV, 2, dict(mask=torch.zeros(2, 1, 7, dtype=torch.bool))),
+    (Q, KV, KV, 2, dict(scale=0.0)), (Q, KV, KV, 2, dict(scale=-1.0)), (Q, KV, KV, 2, dict(scale=float("nan"))),
+    (Q, KV, KV, 2, dict(drop_p=1.0)), (Q, KV, KV, 2, dict(drop_p=-0.1)),
+    (Q, KV, KV, 2, {})])                              # the last one: everything fits, but no tensor is on the GPU
+def test_cross_refusals(q, k, v, heads, kw):
+    with pytest.raises(ValueError):
+        K.cross_fwd(q, k, v, heads, **kw)
+    with pytest.raises(ValueError):
+        K.cross_bwd(q, k, v, q, torch.zeros(q.shape[0], max(heads, 1), q.shape[1] if q.dim() > 2 else 1), q, heads, **kw)
+
+
+def cross_struct(**kw):
+    """Arguments that a launch would take, with addresses that are never read (every test changes one to be refused)."""
+    a = _lib.CrossArgs()
+    for n in ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv", "workspace"):
+        setattr(a, n, 4096)
+    for n in ("ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv"):
+        setattr(a, n, 64)
+    a.B = a.Bc = 2
+    a.heads = a.kv_heads = 2
+    a.Nq, a.Nk, a.hd, a.dtype, a.scale, a.ws_bytes = 5, 7, 32, 0, 0.2, 1 << 30
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(B=0), dict(Bc=0), dict(Bc=1, B=2, index=None, k=None), dict(B=3), dict(heads=3), dict(kv_heads=0), dict(Nq=0), dict(Nk=-1),
+    dict(hd=4), dict(hd=36), dict(hd=136), dict(dtype=2), dict(scale=0.0), dict(scale=float("nan")), dict(drop_p=1.0),
+    dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(lse=None), dict(q=4098), dict(ldq=63), dict(ldq=32), dict(ldk=60)])
+def test_cross_entry_points_refuse(kw):
+    L = _lib.lib()
+    a = cross_struct(**kw)
+    assert L.dm_cross_fwd(ctypes.byref(a), None) == -1
+    assert L.dm_cross_bwd(ctypes.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(d_o=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(lddq=60), dict(workspace=None),
+                                dict(ws_bytes=4), dict(workspace=4100)])
+def test_cross_backward_entry_point_refuses(kw):
+    assert _lib.lib().dm_cross_bwd(ctypes.byref(cross_struct(**kw)), None) == -1
+
+
+def test_cross_workspace_bytes():
+    L = _lib.lib()
+    assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(cross_struct())) == 0
+    assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(cross_struct(Nq=1, Nk=4096))) > 0     # few rows: keys are split
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct())) >= 2 * 2 * 5 * 4
+    assert L.dm_cross_fwd_workspace_bytes(None) == 0 and L.dm_cross_fwd(None, None) == -1 and L.dm_cross_bwd(None, None) == -1
+    few = cross_struct(Nq=1, Nk=4096, workspace=None)
+    assert L.dm_cross_fwd(ctypes.byref(few), None) == -1
+
+
+def rope_struct(**kw):
+    a = _lib.RopeArgs()
+    a.x = a.y = a.freq = a.axis = 4096
+    a.ldx = a.ldy = 64
+    a.B, a.N, a.heads, a.hd, a.rot, a.axes = 2, 6, 2, 32, 32, 2
+    a.grid[0], a.grid[1] = 2, 3
+    for n, v in kw.items():
+        if n == "grid":
+            for i, g in enumerate(v):
+                a.grid[i] = g
+        else:
+            setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=None), dict(y=None), dict(freq=None), dict(axis=None), dict(B=0), dict(N=0), dict(heads=0), dict(hd=0), dict(hd=31),
+    dict(rot=0), dict(rot=34), dict(rot=15), dict(axes=0), dict(axes=4), dict(dtype=2), dict(pairing=2), dict(ldx=32), dict(ldy=63),
+    dict(grid=(2, 4)), dict(grid=(0, 3)), dict(grid=(-2, -3)), dict(grid=(1 << 30, 1 << 30)), dict(heads=2048)])
+def test_rope_entry_point_refuses(kw):
+    assert _lib.lib().dm_rope(ctypes.byref(rope_struct(**kw)), None) == -1

@@ -1,0 +1,368 @@
+"""GPU: attention to an encoder's states of another length (dm_cross_fwd / dm_cross_bwd) against the definition in 64 bits.
+
+Tolerances (u = 2^-24; ub = 2^-8 for bf16 operands, 0 for fp32), per element, from the reference's own intermediate values:
+  score         ds = (hd + 4) u scale |q| |k|  (products and sums of a dot product) + 4 u (1 + |s| + |s - m|)  (the base-2
+                argument of the exponential and the exponential itself);  a probability is off by a factor 1 +- e,
+                e = 2 max(ds) + (Nk + 4) u  (its own score, the row sum), and by ub once more where it is rounded
+  o             ub |o| + (e + ub + (Nk + 4) u) sum p |v|
+  lse           max(ds) + (Nk + 8) u + 4 u |lse|
+  dS            p [ddelta + (hd + 4) u |dO| |v|] + (e + ub) |dS|,  ddelta = sum |dO| tol(o) + (hd + 4) u sum |dO| |o|
+  dq, dk, dv    ub |result| + the tolerance of dS (of p) through |k| (|q|, |dO|) + n u of the n-term sum of magnitudes
+Everything is doubled once for second-order terms."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def K():
+    from diffusion_model_amd import kernels
+    return kernels
+
+
+def valid_rows(c, Nk, lens, mask):
+    if c is None:
+        return torch.zeros(0, dtype=torch.long)
+    n = Nk if lens is None else max(0, min(Nk, int(lens[c])))
+    r = torch.arange(n)
+    return r if mask is None else r[mask[c, :n].bool()]
+
+
+def reference(q, k, v, heads, kv_heads, lens=None, mask=None, index=None, scale=None, d_o=None, keep=None):
+    """Values and tolerances in 64 bits.  keep: optional [B, H, Nq, Nk] multiplier of the probabilities (dropout)."""
+    ub = 2.0 ** -8 if q.dtype == BF16 else 0.0
+    B, Nq, Cq = q.shape
+    Bc, Nk, _ = k.shape
+    hd = Cq // heads
+    scale = hd ** -0.5 if scale is None else scale
+    q, k, v = q.double(), k.double(), v.double()
+    val = dict(o=torch.zeros_like(q), lse=torch.full((B, heads, Nq), -math.inf, dtype=torch.float64), dq=torch.zeros_like(q),
+               dk=torch.zeros_like(k), dv=torch.zeros_like(k))
+    tol = {n: torch.zeros_like(t) for n, t in val.items()}
+    mag = dict(dk=torch.zeros_like(k), dv=torch.zeros_like(k))
+    terms = torch.zeros(Bc)
+    for b in range(B):
+        c = (0 if Bc == 1 else b) if index is None else int(index[b])
+        c = c if 0 <= c < Bc else None
+        rows = valid_rows(c, Nk, lens, mask)
+        if rows.numel() == 0:
+            continue
+        n = rows.numel()
+        for h in range(heads):
+            hs = slice(h * hd, (h + 1) * hd)
+            gs = slice((h // (heads // kv_heads)) * hd, (h // (heads // kv_heads) + 1) * hd)
+            qh, kh, vh = q[b, :, hs], k[c, rows][:, gs], v[c, rows][:, gs]
+            s = qh @ kh.T * scale
+            m = s.amax(-1, keepdim=True)
+            lse = torch.logsumexp(s, -1, keepdim=True)
+            p = torch.exp(s - lse)
+            z = torch.ones_like(p) if keep is None else keep[b, h][:, rows].double()
+            err_s = (hd + 4) * U * scale * (qh.abs() @ kh.abs().T) + 4 * U * (1 + s.abs() + (s - m).abs())
+            e = 2 * err_s.amax(-1, keepdim=True) + (n + 4) * U
+            o = (p * z) @ vh
+            t_o = ub * o.abs() + (e + ub + (n + 4) * U) * ((p * z) @ vh.abs())
+            val["o"][b, :, hs], tol["o"][b, :, hs] = o, 2 * t_o
+            val["lse"][b, h] = lse[:, 0]
+            tol["lse"][b, h] = 2 * (err_s.amax(-1) + (n + 8) * U + 4 * U * lse[:, 0].abs())
+            if d_o is None:
+                continue
+            g = d_o[b, :, hs].double()
+            dp, delta = g @ vh.T * z, (g * o).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            t_delta = (g.abs() * t_o).sum(-1, keepdim=True) + (hd + 4) * U * (g.abs() * o.abs()).sum(-1, keepdim=True)
+            t_ds = p * (t_delta + (hd + 4) * U * (g.abs() @ vh.abs().T) * z) + (e + ub) * ds.abs()
+            t_p = (e + ub) * p * z
+            val["dq"][b, :, hs] = ds @ kh * scale
+            tol["dq"][b, :, hs] = 2 * (ub * val["dq"][b, :, hs].abs() + scale * ((t_ds + (n + 4) * U * ds.abs()) @ kh.abs()))
+            for j, name, left, t_left, right in ((0, "dk", ds * scale, t_ds * scale, qh), (1, "dv", p * z, t_p, g)):
+                full, t_full, m_full = (torch.zeros(Nk, hd, dtype=torch.float64) for _ in range(3))
+                full[rows], t_full[rows], m_full[rows] = left.T @ right, t_left.T @ right.abs(), left.abs().T @ right.abs()
+                val[name][c, :, gs] += full
+                tol[name][c, :, gs] += t_full
+                mag[name][c, :, gs] += m_full
+            terms[c] += Nq
+    for name in ("dk", "dv"):
+        t = terms.double()[:, None, None]
+        tol[name] = 2 * (tol[name] + (t + 8) * U * mag[name] + ub * val[name].abs())
+    return val, tol
+
+
+def check(name, got, val, tol):
+    got, want, t = got.double().cpu(), val[name], tol[name]
+    fin = torch.isfinite(want)
+    assert torch.equal(got[~fin], want[~fin]), name
+    err = (got[fin] - want[fin]).abs()
+    assert bool((err <= t[fin]).all()), f"{name}: worst excess {float((err - t[fin]).max()):.3e}, worst error {float(err.max()):.3e}"
+
+
+def inputs(dtype, B, Bc, Nq, Nk, H, G, hd, lens, mask, index, seed=0, sharp=1.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype)
+    q, k, v, d_o = r(B, Nq, H * hd), r(Bc, Nk, G * hd), r(Bc, Nk, G * hd), r(B, Nq, H * hd)
+    if sharp != 1.0:
+        q = (q.float() * sharp).to(dtype)
+    L = M = I = None
+    if lens:
+        L = torch.randint(0, Nk + 1, (Bc,), generator=g, dtype=torch.int32)
+        L[0] = 0 if lens == "empty" else Nk
+        if Bc > 1:
+            L[1] = 1
+    if mask:
+        M = torch.rand(Bc, Nk, generator=g) < 0.7
+        if Bc > 1:
+            M[Bc - 1] = False
+    if index:
+        I = torch.randint(0, Bc, (B,), generator=g, dtype=torch.int32)
+    return q, k, v, d_o, L, M, I
+
+
+def poison(k, v, lens, mask):
+    """NaN and infinities in every state that does not count."""
+    k, v = k.clone(), v.clone()
+    for c in range(k.shape[0]):
+        bad = torch.ones(k.shape[1], dtype=torch.bool)
+        bad[valid_rows(c, k.shape[1], lens, mask)] = False
+        k[c, bad], v[c, bad] = float("nan"), float("inf")
+    return k, v
+
+
+def cuda(*ts):
+    return [None if t is None else t.cuda() for t in ts]
+
+
+CASES = [
+    # B, Bc, Nq, Nk, H, G, hd, lens, mask, index
+    (2, 2, 1, 1, 1, 1, 8, None, False, False),               # one query, one state
+    (3, 3, 1, 700, 2, 1, 64, "ragged", False, False),        # one query, the keys split over workgroups
+    (1, 1, 5, 2100, 2, 2, 40, None, True, False),            # few queries, long states, holes
+    (4, 4, 33, 77, 4, 4, 32, "empty", False, False),         # one context without states
+    (2, 2, 129, 64, 8, 8, 16, None, False, False),
+    (3, 3, 100, 65, 2, 2, 24, "empty", True, False),         # lengths and holes together; one context masked whole
+    (2, 2, 40, 31, 6, 2, 80, "ragged", False, False),        # heads shared by three
+    (2, 2, 70, 300, 4, 1, 96, None, True, False),
+    (2, 2, 65, 200, 2, 2, 128, "ragged", False, False),
+    (1, 1, 260, 129, 3, 1, 104, None, False, False),
+    (7, 3, 50, 45, 2, 2, 32, "ragged", False, True),         # samples share contexts
+    (66, 2, 9, 20, 2, 1, 16, "ragged", True, True),          # more samples than one wave scans at a time
+    (5, 1, 40, 33, 2, 2, 8, None, False, False),             # one context for all
+    (2, 2, 17, 600, 2, 2, 128, "ragged", True, False),       # more keys than one image holds
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Bc,Nq,Nk,H,G,hd,lens,mask,index", CASES)
+def test_cross_forward_and_backward(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, dtype):
+    kn = K()
+    q, k, v, d_o, L, M, I = inputs(dtype, B, Bc, Nq, Nk, H, G, hd, lens, mask, index)
+    val, tol = reference(q, k, v, H, G, L, M, I, d_o=d_o)
+    kp, vp = poison(k, v, L, M)
+    dq_, dk_, dv_, do_, dL, dM, dI = cuda(q, kp, vp, d_o, L, M, I)
+    kw = dict(kv_heads=G, lens=dL, mask=dM, index=dI)
+    o, lse = kn.cross_fwd(dq_, dk_, dv_, H, **kw)
+    check("o", o, val, tol)
+    check("lse", lse, val, tol)
+    first = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    for name, t in zip(("dq", "dk", "dv"), first):
+        check(name, t, val, tol)
+    again = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))      # fixed summation order
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_cross_scale_and_large_scores(dtype):
+    """A scale of the caller's, and scores far apart: the running maximum moves from block to block."""
+    kn = K()
+    q, k, v, d_o, *_ = inputs(dtype, 1, 1, 70, 400, 2, 2, 32, None, False, False, seed=3, sharp=6.0)
+    val, tol = reference(q, k, v, 2, 2, scale=0.9, d_o=d_o)
+    q, k, v, d_o = cuda(q, k, v, d_o)
+    o, lse = kn.cross_fwd(q, k, v, 2, scale=0.9)
+    check("o", o, val, tol)
+    check("lse", lse, val, tol)
+    for name, t in zip(("dq", "dk", "dv"), kn.cross_bwd(q, k, v, o, lse, d_o, 2, scale=0.9)):
+        check(name, t, val, tol)
+
+
+def test_cross_strided_views_and_untouched_neighbours():
+    """k and v from one fused projection, q from a wider buffer, every result into a slice: the rest stays as it was."""
+    kn = K()
+    B, Nq, Nk, H, hd = 2, 50, 40, 4, 16
+    C = H * hd
+    q, k, v, d_o, L, _, _ = inputs(BF16, B, B, Nq, Nk, H, H, hd, "ragged", False, False, seed=5)
+    val, tol = reference(q, k, v, H, H, L, d_o=d_o)
+    big = torch.full((B, Nq, 3 * C), 7.0, dtype=BF16, device="cuda")
+    big[..., C:2 * C] = q.cuda()
+    kv = torch.cat([k, v], -1).cuda()
+    ob, dqb = torch.full_like(big, 5.0), torch.full_like(big, 5.0)
+    dkv = torch.full((B, Nk, 3 * C), 5.0, dtype=BF16, device="cuda")
+    args = (big[..., C:2 * C], kv[..., :C], kv[..., C:])
+    o, lse = kn.cross_fwd(*args, H, lens=L.cuda(), out=ob[..., C:2 * C])
+    check("o", o, val, tol)
+    dq, dk, dv = kn.cross_bwd(*args, o, lse, d_o.cuda(), H, lens=L.cuda(), dq=dqb[..., :C], dk=dkv[..., :C], dv=dkv[..., 2 * C:])
+    for name, t in (("dq", dqb[..., :C]), ("dk", dkv[..., :C]), ("dv", dkv[..., 2 * C:])):
+        check(name, t, val, tol)
+    for rest in (ob[..., :C], ob[..., 2 * C:], dqb[..., C:], dkv[..., C:2 * C]):
+        assert bool((rest == 5.0).all())
+
+
+def test_cross_index_outside_the_contexts_and_odd_lengths():
+    """An index outside [0, Bc) means no states; lengths outside [0, Nk] are clamped."""
+    kn = K()
+    q, k, v, d_o, *_ = inputs(F32, 5, 3, 20, 33, 2, 2, 16, None, False, False, seed=6)
+    index = torch.tensor([2, -1, 0, 3, 2], dtype=torch.int32)
+    lens = torch.tensor([100, 5, -7], dtype=torch.int32)
+    val, tol = reference(q, k, v, 2, 2, lens, None, index, d_o=d_o)
+    assert not bool(torch.isfinite(val["lse"][[0, 1, 3, 4]]).any()) and bool(torch.isfinite(val["lse"][2]).all())
+    q, k, v, d_o, lens, index = cuda(q, k, v, d_o, lens, index)
+    o, lse = kn.cross_fwd(q, k, v, 2, lens=lens, index=index)
+    check("o", o, val, tol)
+    check("lse", lse, val, tol)
+    for name, t in zip(("dq", "dk", "dv"), kn.cross_bwd(q, k, v, o, lse, d_o, 2, lens=lens, index=index)):
+        check(name, t, val, tol)
+
+
+def test_cross_no_states_and_empty_batches():
+    kn = K()
+    q = torch.randn(2, 7, 32, device="cuda")
+    k = torch.empty(2, 0, 32, device="cuda")
+    o, lse = kn.cross_fwd(q, k, k, 2)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    dq, dk, dv = kn.cross_bwd(q, k, k, o, lse, q, 2)
+    assert bool((dq == 0).all()) and dk.shape == k.shape
+    k = torch.randn(2, 5, 32, device="cuda")
+    none = q[:, :0].contiguous()
+    o, lse = kn.cross_fwd(none, k, k, 2)
+    assert o.shape == (2, 0, 32) and lse.shape == (2, 2, 0)
+    dq, dk, dv = kn.cross_bwd(none, k, k, o, lse, none, 2)
+    assert bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+def test_cross_nan_in_a_valid_state_reaches_only_its_sample():
+    kn = K()
+    q, k, v, *_ = inputs(BF16, 2, 2, 40, 50, 2, 2, 32, None, False, False, seed=8)
+    v[0, 3, 0] = float("nan")
+    o, lse = kn.cross_fwd(*cuda(q, k, v), 2)
+    assert bool(torch.isnan(o[0, :, 0]).all()) and bool(torch.isfinite(o[1]).all()) and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd,Nk", [(128, 100), (64, 50)])
+def test_cross_dropout(hd, Nk, dtype):
+    """The keep mask is read off with unit values (o = P Z / keep), is a fair draw, and the same seed then gives the
+    forward and the backward of exactly that mask."""
+    kn = K()
+    B, Nq, H, p = 2, 150, 2, 0.25
+    q, k, v, d_o, L, _, _ = inputs(dtype, B, B, Nq, Nk, H, H, hd, "ragged", False, False, seed=9)
+    L[:] = Nk
+    eye = torch.zeros(B, Nk, H, hd)
+    eye[:, torch.arange(Nk), :, torch.arange(Nk)] = 1.0
+    qd, kd, vd, dd, Ld = cuda(q, k, v, d_o, L)
+    o, _ = kn.cross_fwd(qd, kd, eye.reshape(B, Nk, -1).to(dtype).cuda(), H, lens=Ld, drop_p=p, drop_seed=77)
+    keep = (o.float().cpu().reshape(B, Nq, H, hd).permute(0, 2, 1, 3)[..., :Nk] > 0).double()
+    n = keep.numel()
+    assert abs(float(keep.mean()) - (1 - p)) < 5 * math.sqrt(p * (1 - p) / n)       # five standard deviations
+    keep = keep / (1.0 - round(p * 32768) / 32768)
+    val, tol = reference(q, k, v, H, H, L, d_o=d_o, keep=keep)
+    o, lse = kn.cross_fwd(qd, kd, vd, H, lens=Ld, drop_p=p, drop_seed=77)
+    check("o", o, val, tol)
+    check("lse", lse, val, tol)
+    for name, t in zip(("dq", "dk", "dv"), kn.cross_bwd(qd, kd, vd, o, lse, dd, H, lens=Ld, drop_p=p, drop_seed=77)):
+        check(name, t, val, tol)
+    other, _ = kn.cross_fwd(qd, kd, vd, H, lens=Ld, drop_p=p, drop_seed=78)
+    assert not torch.equal(other, o)
+
+
+def test_cross_gradients_against_differences():
+    """fp32, along random directions: (f(x + eps d) - f(x - eps d)) / 2 eps.  eps = 1e-2: the third-order term is about
+    eps^2 / 6 of the directional derivative's scale, the roundings about |f| 2^-22 / eps."""
+    kn = K()
+    q, k, v, w, L, M, I = inputs(F32, 3, 2, 12, 20, 2, 1, 16, "ragged", True, True, seed=11)
+    M[:] = True
+    M[0, 4] = False
+    dw, dL, dM, dI = cuda(w, L, M, I)
+    kw = dict(kv_heads=1, lens=dL, mask=dM, index=dI)
+    f = lambda a, b, c: float((kn.cross_fwd(a.cuda(), b.cuda(), c.cuda(), 2, **kw)[0].double() * dw.double()).sum())
+    qd, kd, vd = cuda(q, k, v)
+    o, lse = kn.cross_fwd(qd, kd, vd, 2, **kw)
+    grads = [t.double().cpu() for t in kn.cross_bwd(qd, kd, vd, o, lse, dw, 2, **kw)]
+    g = torch.Generator().manual_seed(12)
+    for i in range(3):
+        d = torch.randn((q, k, v)[i].shape, generator=g)
+        eps = 1e-2
+        hi, lo = [list((q, k, v)) for _ in range(2)]
+        hi[i], lo[i] = hi[i] + eps * d, lo[i] - eps * d
+        num = (f(*hi) - f(*lo)) / (2 * eps)
+        want = float((grads[i] * d.double()).sum())
+        size = float((grads[i].abs() * d.abs().double()).sum())
+        assert abs(num - want) < 2e-3 * size + 1e-3, (i, num, want)
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_cross_captured_replays(few):
+    """Forward and backward in one HIP graph, replayed with other inputs and other lengths, eager calls in between."""
+    kn = K()
+    shape = (2, 2, 3, 900, 2, 2, 64) if few else (4, 2, 200, 70, 4, 2, 32)
+    B, Bc, Nq, Nk, H, G, hd = shape
+    q, k, v, d_o, L, M, I = cuda(*inputs(BF16, *shape, "ragged", True, Bc != B))
+    kw = dict(kv_heads=G, lens=L, mask=M, index=I)
+
+    def step():
+        o, lse = kn.cross_fwd(q, k, v, H, **kw)
+        return (o, lse, *kn.cross_bwd(q, k, v, o, lse, d_o, H, **kw))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        fresh = cuda(*inputs(BF16, *shape, "empty" if i % 2 else "ragged", True, Bc != B, seed=20 + i))
+        for t, n in zip((q, k, v, d_o, L, M, I), fresh):
+            if t is not None:
+                t.copy_(n)
+        eager = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
+
+
+def test_cross_two_streams_at_once():
+    """Two calls that need scratch, on two streams, many times: each has its own."""
+    kn = K()
+    sets = [cuda(*inputs(BF16, 2, 2, 4, 1500, 2, 2, 64, None, False, False, seed=s))[:4] for s in (1, 2)]
+
+    def both(q, k, v, d_o):
+        o, lse = kn.cross_fwd(q, k, v, 2)
+        return (o, lse, *kn.cross_bwd(q, k, v, o, lse, d_o, 2))
+
+    want = [both(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(both(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
+
+
+def test_cross_states_past_32_bits():
+    """Rows of k and v whose byte offsets pass 2^32."""
+    kn = K()
+    Nk, ld = 600, 1 << 22
+    base = torch.empty(1, Nk, ld, dtype=BF16, device="cuda")      # 4.7 GiB
+    q, k, v, d_o, *_ = inputs(BF16, 1, 1, 20, Nk, 1, 1, 32, None, False, False, seed=13)
+    kd, vd = base[..., :32], base[..., 64:96]
+    kd.copy_(k)
+    vd.copy_(v)
+    val, tol = reference(q, k, v, 1, 1, d_o=d_o)
+    qd, dd = cuda(q, d_o)
+    o, lse = kn.cross_fwd(qd, kd, vd, 1)
+    check("o", o, val, tol)
+    for name, t in zip(("dq", "dk", "dv"), kn.cross_bwd(qd, kd, vd, o, lse, dd, 1, dk=base[..., 128:160], dv=base[..., 192:224])):
+        check(name, t, val, tol)

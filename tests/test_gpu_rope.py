@@ -1,0 +1,170 @@
+"""GPU: rotary positions with several axes (dm_rope) against the definition in 64 bits.
+
+Tolerance.  With u = 2^-24: the reduced angle (a fraction of a turn in [-1/2, 1/2]) is rounded once to fp32, which moves the
+angle by at most pi u; sincospif is within 2 ulp, 2u at most in absolute terms; a product pair and its sum round three times.
+|error| <= (pi + 2 + 3) u (|a| + |b|) < 10 u (|a| + |b|) for fp32, plus half a step (2^-8 relative) of a bf16 result."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+
+
+def K():
+    from diffusion_model_amd import kernels
+    return kernels
+
+
+def positions_of(grid):
+    return torch.stack(torch.meshgrid(*[torch.arange(n) for n in grid], indexing="ij"), -1).reshape(-1, len(grid))
+
+
+def reference(x, heads, hd, axes, pairing, pos, theta=10000.0, inverse=False):
+    """(rotated, |a| + |b| per element) in 64 bits; pos [N, A] or [B, N, A]."""
+    B, N, _ = x.shape
+    h = x.double().cpu().reshape(B, N, heads, hd)
+    R = sum(axes)
+    ang = torch.cat([pos[..., i:i + 1].double() * torch.tensor([theta ** (-2.0 * j / d) for j in range(d // 2)], dtype=torch.float64)
+                     for i, d in enumerate(axes)], -1)
+    ang = ang.reshape(-1, N, 1, R // 2)
+    c, s = torch.cos(ang), torch.sin(ang) * (-1.0 if inverse else 1.0)
+    ia = torch.arange(R // 2) * 2 if pairing == "interleaved" else torch.arange(R // 2)
+    ib = ia + 1 if pairing == "interleaved" else ia + R // 2
+    y, mag = h.clone(), torch.zeros_like(h)
+    a, b = h[..., ia], h[..., ib]
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    mag[..., ia] = mag[..., ib] = a.abs() + b.abs()
+    return y.reshape(B, N, -1), mag.reshape(B, N, -1)
+
+
+def check(y, ref, mag, dtype):
+    tol = 10 * U32 * mag + (2.0 ** -8 * ref.abs() if dtype == torch.bfloat16 else 0.0)
+    err = (y.double().cpu() - ref).abs()
+    assert bool((err <= tol * (1 + 1e-6)).all()), float((err - tol).max())
+
+
+CASES = [
+    # heads, hd, axes, pairing, grid, B
+    (16, 32, (16, 16), "interleaved", (24, 24), 2),
+    (16, 32, (16, 16), "half", (5, 7), 3),
+    (16, 16, (8, 8), "interleaved", (1, 1), 1),           # one token
+    (16, 8, (4, 4), "half", (6, 6), 2),                   # half a head is four channels
+    (2, 128, (32, 48, 48), "half", (3, 5, 7), 1),
+    (3, 128, (44, 42, 42), "interleaved", (4, 3, 5), 2),
+    (5, 40, (16, 16), "half", (11, 3), 2),                # part of the head, an odd head count
+    (5, 40, (10, 6), "interleaved", (11, 3), 2),          # the rotated width ends inside a 16-byte piece
+    (1, 6, (2,), "interleaved", (13,), 2),
+    (3, 10, (4, 2), "half", (4, 4), 2),                   # nothing is aligned
+    (1, 2, (2,), "half", (1,), 5),
+    (1, 2048, (2048,), "half", (3,), 1),
+    (12, 64, (64,), "interleaved", (1025,), 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,hd,axes,pairing,grid,B", CASES)
+def test_rope_grid_and_inverse(heads, hd, axes, pairing, grid, B, dtype):
+    k = K()
+    N = math.prod(grid)
+    g = torch.Generator().manual_seed(heads * 131 + hd)
+    x = torch.randn(B, N, heads * hd, generator=g).to(dtype)
+    plan = k.rope_plan(hd, axes, pairing=pairing, device="cuda")
+    for inverse in (False, True):
+        y = k.rope(x.cuda(), heads, plan, grid=grid, inverse=inverse)
+        check(y, *reference(x, heads, hd, axes, pairing, positions_of(grid), inverse=inverse), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["int", "float", "per_sample"])
+def test_rope_positions(kind, dtype):
+    k = K()
+    B, N, heads, hd, axes = 3, 37, 4, 48, (16, 24)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(B, N, heads * hd, generator=g).to(dtype)
+    if kind == "int":
+        pos = torch.randint(-100000, 1000000, (N, 2), generator=g, dtype=torch.int32)    # far positions keep their fraction
+    else:
+        pos = torch.randn((B, N, 2) if kind == "per_sample" else (N, 2), generator=g) * 3000.0
+    plan = k.rope_plan(hd, axes, theta=500.0, device="cuda")
+    y = k.rope(x.cuda(), heads, plan, positions=pos.cuda())
+    check(y, *reference(x, heads, hd, axes, "interleaved", pos, theta=500.0), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rope_in_place_on_a_fused_projection(dtype):
+    """The query and key slices of a fused buffer in one call; the values behind them stay as they were."""
+    k = K()
+    B, grid, heads, hd = 2, (6, 5), 8, 16
+    C = heads * hd
+    qkv = torch.randn(B, 30, 3 * C, generator=torch.Generator().manual_seed(1)).to(dtype)
+    dev = qkv.cuda()
+    plan = k.rope_plan(hd, (8, 8), device="cuda")
+    qk = dev[..., :2 * C]
+    assert k.rope(qk, 2 * heads, plan, grid=grid, out=qk) is qk
+    check(dev[..., :2 * C], *reference(qkv[..., :2 * C], 2 * heads, hd, (8, 8), "interleaved", positions_of(grid)), dtype)
+    assert torch.equal(dev[..., 2 * C:].cpu(), qkv[..., 2 * C:])
+
+
+def test_rope_unaligned_view_and_special_values():
+    """A slice that starts off a 16-byte boundary; infinities and NaN stay in their own pairs, and channels behind the
+    rotated width are copied bit for bit."""
+    k = K()
+    base = torch.randn(1, 9, 2 * 24 + 3, generator=torch.Generator().manual_seed(2), dtype=torch.float32).cuda()
+    x = base[..., 3:]
+    x[0, 2, 17], x[0, 3, 20] = float("inf"), float("nan")
+    plan = k.rope_plan(24, (8, 8), device="cuda")
+    y = k.rope(x, 2, plan, grid=(3, 3))
+    ref, mag = reference(torch.nan_to_num(x, nan=0.0, posinf=0.0), 2, 24, (8, 8), "interleaved", positions_of((3, 3)))
+    keep = torch.ones_like(ref, dtype=torch.bool)
+    keep[0, 2, 17] = keep[0, 3, 20] = False
+    check(torch.where(keep.cuda(), y, torch.zeros_like(y)), torch.where(keep, ref, torch.zeros_like(ref)), mag, torch.float32)
+    assert float(y[0, 2, 17]) == float("inf") and math.isnan(float(y[0, 3, 20]))
+
+
+def test_rope_backward_is_the_gradient():
+    """<rope(x), w> has the gradient rope(w, inverse): against differences along random directions, in fp32."""
+    k = K()
+    g = torch.Generator().manual_seed(3)
+    x, w, d = (torch.randn(1, 20, 2 * 32, generator=g) for _ in range(3))
+    plan = k.rope_plan(32, (16, 16), pairing="half", device="cuda")
+    f = lambda t: float((k.rope(t.cuda(), 2, plan, grid=(4, 5)).double().cpu() * w.double()).sum())
+    grad = k.rope(w.cuda(), 2, plan, grid=(4, 5), inverse=True).double().cpu()
+    # linear in x: a difference of any width is exact but for the roundings of 1280 terms of size <= ~10
+    num = (f(x + d) - f(x - d)) / 2.0
+    assert abs(num - float((grad * d.double()).sum())) < 1280 * 10 * 16 * U32
+
+
+def test_rope_captured_and_on_another_stream():
+    k = K()
+    plan = k.rope_plan(32, (16, 16), device="cuda")
+    x = torch.randn(2, 64, 16 * 32, device="cuda").to(torch.bfloat16)
+    want = k.rope(x, 16, plan, grid=(8, 8))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = k.rope(x, 16, plan, grid=(8, 8))
+    s.synchronize()
+    assert torch.equal(y, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = k.rope(x, 16, plan, grid=(8, 8))
+    for i in range(3):
+        x.copy_(torch.randn(2, 64, 16 * 32, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, k.rope(x, 16, plan, grid=(8, 8)))
+
+
+def test_rope_rows_past_32_bits():
+    """Rows whose byte offsets pass 2^32."""
+    k = K()
+    ld = 1 << 21
+    base = torch.empty(1, 1100, ld, dtype=torch.bfloat16, device="cuda")     # 4.3 GiB
+    x = base[..., 64:64 + 64]
+    src = torch.randn(1, 1100, 64, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    x.copy_(src)
+    plan = k.rope_plan(32, (32,), device="cuda")
+    k.rope(x, 2, plan, grid=(1100,), out=x)
+    check(x, *reference(src, 2, 32, (32,), "interleaved", positions_of((1100,))), torch.bfloat16)
