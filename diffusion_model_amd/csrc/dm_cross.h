@@ -12,7 +12,7 @@
 #pragma once
 #include "dm_common.h"
 
-namespace {
+namespace dm_cross {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -140,13 +140,33 @@ __device__ __forceinline__ void stage_rows(char* dst, int stride, const char* sr
     *reinterpret_cast<u32x4*>(dst + r * stride + pc * 16) = v;
   }
 }
-// validity bits of keys [r0, r0 + n): one word per 32 keys
-__device__ __forceinline__ void stage_bits(uint32_t* bits, int r0, int n, int valid, const unsigned char* mask, int tid) {
+// Validity of keys [r0, r0 + n): one word per 32 keys (empty tiles are skipped) and, per key, what its score starts from:
+// 0 or -infinity.  A score tile always starts its accumulators from the latter: four broadcast LDS reads per tile, where
+// clearing the registers or masking the scores would be 16 to 64 vector instructions of a loop that is bound by them.
+__device__ __forceinline__ void stage_valid(uint32_t* bits, float* bias, int r0, int n, int valid, const unsigned char* mask, int tid) {
   for (int i = tid; i < ((n + 63) & ~63); i += 256) {
     const bool ok = i < n && r0 + i < valid && (!mask || mask[r0 + i]);
     const unsigned long long w = __ballot(ok);
     if ((tid & 63) == 0) { bits[i >> 5] = (uint32_t)w; bits[(i >> 5) + 1] = (uint32_t)(w >> 32); }
+    if (i < n) bias[i] = ok ? 0.f : -INFINITY;
   }
+}
+// start of a score tile whose rows are the 32 keys of `bias`
+__device__ __forceinline__ f32x16 score_init(const float* bias, int half) {
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 b = *reinterpret_cast<const f32x4*>(bias + 8 * i + 4 * half);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[4 * i + r] = b[r];
+  }
+  return s;
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.f;
+  return s;
 }
 // x of this lane and of its partner 32 lanes on (in the order of the halves)
 __device__ __forceinline__ void half_swap(float x, float& a, float& b) {
@@ -173,6 +193,49 @@ template <typename T> __device__ __forceinline__ void store4(char* dst, float a,
     *reinterpret_cast<bf16x4*>(dst) = w;
   } else {
     *reinterpret_cast<f32x4*>(dst) = f32x4{a, b, c, d};
+  }
+}
+// Orders this wave's LDS accesses for the compiler (the hardware keeps one wave's in order): what a lane wrote before is
+// what the others read after.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// A head-dim-major result tile (columns = rows of dst, this lane's row given; 32 channels from col0) times f, 16 bytes of
+// bf16 per store: the two halves of a wave exchange registers so that each lane has 8 consecutive channels.
+template <typename T>
+__device__ __forceinline__ void store_tile(char* row, const f32x16& a, float f, int col0, int hd, bool ok, int half) {
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    if (col0 + 16 * pair >= hd) break;
+    const int col = col0 + 16 * pair + 8 * half;
+    if constexpr (sizeof(T) == 2) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bf16x2 lo = {(bf16)(a[8 * pair + 2 * j] * f), (bf16)(a[8 * pair + 2 * j + 1] * f)};
+        const bf16x2 hi = {(bf16)(a[8 * pair + 4 + 2 * j] * f), (bf16)(a[8 * pair + 5 + 2 * j] * f)};
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+        w[j] = r[0];
+        w[2 + j] = r[1];
+      }
+      if (ok && col < hd) *reinterpret_cast<u32x4*>(row + col * 2) = w;
+    } else {
+      f32x4 x, y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float lo = a[8 * pair + j] * f, hi = a[8 * pair + 4 + j] * f;
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+        const unsigned r0 = r[0], r1 = r[1];
+        x[j] = __builtin_bit_cast(float, r0);
+        y[j] = __builtin_bit_cast(float, r1);
+      }
+      if (ok && col < hd) {
+        *reinterpret_cast<f32x4*>(row + col * 4) = x;
+        *reinterpret_cast<f32x4*>(row + col * 4 + 16) = y;
+      }
+    }
   }
 }
 // Consecutive workgroups go to the eight XCDs in turn; this gives each XCD a contiguous run of logical ids, so that the
@@ -220,4 +283,9 @@ inline int cross_fill(CrossParams& p, const dm_cross_args* a, bool bwd) {
   return DM_OK;
 }
 
-}  // namespace
+// ---------------------------------------------------------------- the one-kernel backward of few keys (dm_cross_few.hip)
+struct FewPlan { int kt, iters, nqb; bool direct; long ws; };
+bool few_plan(const dm_cross_args* a, FewPlan& f);          // false: these sizes take the two kernels of dm_cross_bwd.hip
+int few_launch(const CrossParams& p, const FewPlan& f, int dtype, hipStream_t st);
+
+}  // namespace dm_cross

@@ -8,6 +8,8 @@
 
 namespace {
 
+using namespace dm_cross;
+
 // ---------------------------------------------------------------- dQ (and delta)
 template <typename T, int HDP, bool RES, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
@@ -16,7 +18,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
   char* sV = sK + p.kb * Gm::SR;
-  uint32_t* bits = reinterpret_cast<uint32_t*>(sV + p.kb * Gm::SR);
+  float* bias = reinterpret_cast<float*>(sV + p.kb * Gm::SR);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(bias + p.kb);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
@@ -47,7 +50,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
 #pragma unroll
       for (int j = 0; j < (int)(16 / sizeof(T)); ++j) s += (float)df[kc][j] * (float)of[kc][j];
     delta = half_sum(s);
-    L2 = ok ? p.lse[row] * CR_LOG2E : 0.f;
+    L2 = ok ? p.lse[row] * CR_LOG2E : INFINITY;
+    if (L2 == -INFINITY) L2 = INFINITY;        // no probability without a finite score, nor past the last query
     if (ok && half == 0) p.delta[row] = delta;
     if (DROP) rs = dm_drop_row(seed, (uint32_t)row);
 #pragma unroll
@@ -58,15 +62,13 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
   auto stage = [&](int from, int n) {
     stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, kn, mask, hdb, tid);
     stage_rows<T, HDP>(sV, Gm::SR, vbase, p.ldv, from, n, kn, mask, hdb, tid);
-    stage_bits(bits, from, n, kn, mask, tid);
+    stage_valid(bits, bias, from, n, kn, mask, tid);
   };
   auto sweep = [&](int from, int tiles) {
     for (int t = 0; t < tiles; ++t) {
       const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
       if (w == 0) continue;
-      f32x16 s, dp;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+      f32x16 s = score_init(bias + t * 32, half), dp = zero16();      // (masked keys: exp2(-inf) = 0)
 #pragma unroll
       for (int kc = 0; kc < Gm::NC; ++kc) {
         s = Cr<T>::mma(row_frag<T>(sK + t * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s);
@@ -84,11 +86,6 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
-      if (w != 0xFFFFFFFFu) {
-        const uint32_t mine = w >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (mine >> tile_row(i, 0)) & 1u ? s[i] : 0.f;
-      }
 #pragma unroll
       for (int f = 0; f < Cr<T>::NF; ++f) {
         const frag sf = Cr<T>::pack(s, f);
@@ -99,16 +96,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
     }
   };
   auto finish = [&](int q) {
-    if (q >= p.Nq) return;
     char* dst = p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb;
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = d * 32 + 8 * i + 4 * half;
-        if (col < p.hd)
-          store4<T>(dst + col * sizeof(T), acc[d][4 * i] * p.scale, acc[d][4 * i + 1] * p.scale, acc[d][4 * i + 2] * p.scale, acc[d][4 * i + 3] * p.scale);
-      }
+    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, acc[d], p.scale, d * 32, p.hd, q < p.Nq, half);
   };
   const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
   if (RES) {
@@ -310,7 +300,7 @@ int row_bytes(const dm_cross_args* a) { return cross_hdp(a->hd) * (a->dtype == 0
 BwdPlan bwd_plan(const dm_cross_args* a) {
   BwdPlan f{};
   const long groups = ((long)a->Nq + 127) / 128, blocks = groups * a->B * a->heads;
-  const int image = (LDS_IMAGE - 512) / (2 * row_bytes(a)) / 64 * 64;
+  const int image = (LDS_IMAGE - 64) / (2 * row_bytes(a) + 5) / 64 * 64;
   const int need = (a->Nk + 63) & ~63;
   f.res = need <= image;
   f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
@@ -322,6 +312,7 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
     f.iters = it < 1 ? 1 : (int)it;
   }
   f.nqb = (int)((groups + f.iters - 1) / f.iters);
+  f.iters = (int)((groups + f.nqb - 1) / f.nqb);
   f.delta_bytes = (((long)a->B * a->heads * a->Nq + 3) & ~3L) * 4;
   // shares of a context's query list: enough workgroups for four per CU, at least four blocks of queries each
   const long owners = (long)a->Bc * a->kv_heads * ((a->Nk + 127) / 128);
@@ -340,7 +331,7 @@ int launch_dq(const CrossParams& p, hipStream_t st) {
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = (size_t)p.kb * 2 * Geo<T, HDP>::SR + (p.kb / 32 + 2) * 4;
+  const size_t lds = (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4;
   const long blocks = (long)p.B * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
@@ -390,12 +381,23 @@ template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t
 
 }  // namespace
 
-extern "C" long dm_cross_bwd_workspace_bytes(const dm_cross_args* a) { return cross_sizes_ok(a) ? bwd_plan(a).ws : 0; }
+extern "C" long dm_cross_bwd_workspace_bytes(const dm_cross_args* a) {
+  if (!dm_cross::cross_sizes_ok(a)) return 0;
+  dm_cross::FewPlan few;
+  return dm_cross::few_plan(a, few) ? few.ws : bwd_plan(a).ws;
+}
 
 extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
   CrossParams p{};
   const int rc = cross_fill(p, a, true);
   if (rc != DM_OK) return rc;
+  FewPlan few;
+  if (few_plan(a, few)) {
+    DM_REQUIRE(few.ws == 0 || (a->workspace && a->ws_bytes >= few.ws && (uintptr_t)a->workspace % 16 == 0));
+    p.iters = few.iters; p.nqb = few.nqb; p.nsplit = few.direct ? 0 : 1;
+    p.part = (float*)a->workspace;
+    return few_launch(p, few, a->dtype, (hipStream_t)stream);
+  }
   const BwdPlan f = bwd_plan(a);
   DM_REQUIRE(a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0);
   p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb; p.nsplit = f.nsplit;

@@ -1,0 +1,315 @@
+// Backward of the attention to encoder states for few keys (up to 96 at the narrow heads: a caption's 77 tokens): one pass.
+//
+// With so few keys a wave holds ALL probabilities and score gradients of its 32 queries in registers (queries on the lanes,
+// KT tiles of 32 keys), so the scores are computed once -- two kernels, one per operand side, would compute them twice --
+// and delta = sum_k P dP comes from the very values it is subtracted from: O is not read, and its rounding to bf16 is in no
+// gradient.  dS^T is directly the operand of dQ^T = K^T dS^T.  dV and dK reduce over the queries, so P and dS go through a
+// small LDS tile of the wave's own (written [query][key], read transposed), against dO and Q from a second one.  The waves
+// of a workgroup keep dK and dV in registers over all their query tiles, add them up in wave order at the end, and leave
+// one fp32 partial per workgroup, which cross_gather_kernel sums in a fixed order: no atomics.
+#include "dm_cross.h"
+
+namespace {
+
+using namespace dm_cross;
+
+template <typename T> constexpr int patch_stride() { return sizeof(T) == 2 ? 72 : 144; }   // 32 keys + padding: writes without conflicts
+template <typename T, int HDP> constexpr int wave_lds() { return 2 * 32 * Geo<T, HDP>::ST + 2 * 32 * patch_stride<T>(); }
+template <typename T, int HDP, int KT> constexpr int few_lds() {
+  const int keys = KT * 32 * (2 * Geo<T, HDP>::SR + 4) + 32, loop = keys + 4 * wave_lds<T, HDP>();
+  const int sums = 2 * KT * 32 * (HDP + 4) * 4;
+  return loop > sums ? loop : sums;
+}
+
+// waves per SIMD that the registers allow (dK and dV alone take 32 KT HDP / 32)
+template <typename T, int HDP, int KT> constexpr int few_waves() {
+  return sizeof(T) == 2 ? (HDP <= 32 || (HDP == 64 && KT == 1) ? 2 : 1) : (HDP <= 32 && KT == 1 ? 2 : 1);
+}
+
+template <typename T> __device__ __forceinline__ void put_tile(char* patch, const f32x16& s, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    store4<T>(patch + (lane & 31) * patch_stride<T>() + (8 * i + 4 * (lane >> 5)) * (int)sizeof(T), s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+}
+
+template <typename T, int HDP, int KT, bool DROP>
+__global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kernel(const CrossParams p) {
+  typedef Geo<T, HDP> Gm;
+  typedef typename Cr<T>::frag frag;
+  constexpr int PS = patch_stride<T>(), NF = Cr<T>::NF;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* sK = smem;
+  char* sV = sK + KT * 32 * Gm::SR;
+  float* bias = reinterpret_cast<float*>(sV + KT * 32 * Gm::SR);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(bias + KT * 32);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  char* sQ = reinterpret_cast<char*>(bits + 8) + wave * wave_lds<T, HDP>();
+  char* sD = sQ + 32 * Gm::ST;
+  char* sP = sD + 32 * Gm::ST;
+  char* sS = sP + 32 * PS;
+  uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int h = id % p.H;
+  id /= p.H;
+  const int qb = id % p.nqb, b = id / p.nqb;
+  const int ctx = context_of(p, b), kn = keys_of(p, ctx);
+  const int hdb = p.hd * (int)sizeof(T), g = h / (p.H / p.G);
+  const long krow = (long)(ctx < 0 ? 0 : ctx) * p.Nk;
+  const unsigned char* mask = p.mask ? p.mask + krow : nullptr;
+  const float c = p.scale * CR_LOG2E;
+  const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
+  const long tok = (long)b * p.Nq, row = ((long)b * p.H + h) * p.Nq;
+
+  frag qf[Gm::NC], df[Gm::NC];
+  float L2;
+  auto fetch = [&](int q) {
+    const bool ok = q < p.Nq;
+    load_frags<T, HDP>(p.q + (tok + q) * p.ldq + h * hdb, ok, hdb, lane, qf);
+    load_frags<T, HDP>(p.d_o + (tok + q) * p.lddo + h * hdb, ok, hdb, lane, df);
+    L2 = ok ? p.lse[row + q] : INFINITY;
+  };
+  const int q0 = (qb * p.iters * 4 + wave) * 32 + (lane & 31);
+  fetch(q0);
+  stage_rows<T, HDP>(sK, Gm::SR, p.k + krow * p.ldk + g * hdb, p.ldk, 0, KT * 32, kn, mask, hdb, tid);
+  stage_rows<T, HDP>(sV, Gm::SR, p.v + krow * p.ldv + g * hdb, p.ldv, 0, KT * 32, kn, mask, hdb, tid);
+  stage_valid(bits, bias, 0, KT * 32, kn, mask, tid);
+  __syncthreads();
+  uint32_t w[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t) w[t] = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
+  f32x16 dk[KT][Gm::DT], dv[KT][Gm::DT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d) { dk[t][d] = zero16(); dv[t][d] = zero16(); }
+
+  for (int it = 0; it < p.iters; ++it) {
+    const int q = q0 + it * 128;
+    if (q - (lane & 31) >= p.Nq) break;        // (wave-uniform)
+    // a query past the end, and one without a finite score, has no probabilities
+    const float lse2 = L2 == -INFINITY ? INFINITY : L2 * CR_LOG2E;
+#pragma unroll
+    for (int kc = 0; kc < Gm::NC; ++kc) {
+      *reinterpret_cast<frag*>(sQ + (lane & 31) * Gm::ST + kc * 32 + half * 16) = qf[kc];
+      *reinterpret_cast<frag*>(sD + (lane & 31) * Gm::ST + kc * 32 + half * 16) = df[kc];
+    }
+    f32x16 pr[KT], dp[KT];
+    uint32_t keep[KT];
+    float delta = 0.f;
+    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q)) : 0u;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if (w[t] == 0) continue;
+      f32x16 s = score_init(bias + t * 32, half), e = zero16();
+#pragma unroll
+      for (int kc = 0; kc < Gm::NC; ++kc) {
+        s = Cr<T>::mma(row_frag<T>(sK + t * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s);
+        e = Cr<T>::mma(row_frag<T>(sV + t * 32 * Gm::SR, Gm::SR, kc, lane), df[kc], e);
+      }
+      if (DROP) {
+        keep[t] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t z = dm_drop_bits(rs, (uint32_t)(t * 32 + tile_row(i, half)) >> 1);
+          const bool k0 = dm_keep16(z, 0, p.thresh), k1 = dm_keep16(z, 1, p.thresh);
+          keep[t] |= (k0 ? 1u : 0u) << i | (k1 ? 2u : 0u) << i;
+          e[i] = k0 ? e[i] * p.inv_keep : 0.f;
+          e[i + 1] = k1 ? e[i + 1] * p.inv_keep : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
+        delta = __builtin_fmaf(s[i], e[i], delta);
+      }
+      pr[t] = s;
+      dp[t] = e;
+    }
+    delta = half_sum(delta);
+    if (it + 1 < p.iters) fetch(q + 128);      // the next tile's rows fly during the products below
+    wave_lds_order();
+    f32x16 dq[Gm::DT];
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d) dq[d] = zero16();
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if (w[t] == 0) continue;
+      f32x16 ds;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] = pr[t][i] * (dp[t][i] - delta);
+      if (DROP) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
+      }
+      put_tile<T>(sP, pr[t], lane);
+      put_tile<T>(sS, ds, lane);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const frag sf = Cr<T>::pack(ds, f);
+#pragma unroll
+        for (int d = 0; d < Gm::DT; ++d) dq[d] = Cr<T>::mma(tr_frag<T, HDP>(sK + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, dq[d]);
+      }
+      wave_lds_order();
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const frag pf = tr_frag<T, 32>(sP, PS, f, 0, lane), sf = tr_frag<T, 32>(sS, PS, f, 0, lane);
+#pragma unroll
+        for (int d = 0; d < Gm::DT; ++d) {
+          dv[t][d] = Cr<T>::mma(tr_frag<T, HDP>(sD, Gm::ST, f, d, lane), pf, dv[t][d]);
+          dk[t][d] = Cr<T>::mma(tr_frag<T, HDP>(sQ, Gm::ST, f, d, lane), sf, dk[t][d]);
+        }
+      }
+      wave_lds_order();
+    }
+    char* dst = p.dq + (tok + q) * p.lddq + h * hdb;
+#pragma unroll
+    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, p.hd, q < p.Nq, half);
+  }
+
+  // dK, dV of the four waves, added in wave order: [dk | dv][key][channel]
+  constexpr int RS = HDP + 4;
+  float* sum = reinterpret_cast<float*>(smem);
+#pragma unroll 1
+  for (int turn = 0; turn < 4; ++turn) {
+    __syncthreads();
+    if (turn != wave) continue;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int d = 0; d < Gm::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < (HDP < 32 ? 2 : 4); ++i) {
+          float* a = sum + (t * 32 + (lane & 31)) * RS + d * 32 + 8 * i + 4 * half;
+          f32x4 x = {dk[t][d][4 * i], dk[t][d][4 * i + 1], dk[t][d][4 * i + 2], dk[t][d][4 * i + 3]};
+          f32x4 y = {dv[t][d][4 * i], dv[t][d][4 * i + 1], dv[t][d][4 * i + 2], dv[t][d][4 * i + 3]};
+          f32x4* px = reinterpret_cast<f32x4*>(a);
+          f32x4* py = reinterpret_cast<f32x4*>(a + KT * 32 * RS);
+          if (turn) { x += *px; y += *py; }
+          *px = x;
+          *py = y;
+        }
+  }
+  __syncthreads();
+  if (ctx < 0) return;
+  const int per = p.hd >> 2, n = p.Nk * per;
+  for (int i = tid; i < 2 * n; i += 256) {
+    const int which = i >= n, e = which ? i - n : i, key = e / per, col = (e - key * per) * 4;
+    const f32x4 v = *reinterpret_cast<const f32x4*>(sum + (which * KT * 32 + key) * RS + col);
+    if (p.nsplit) {
+      *reinterpret_cast<f32x4*>(p.part + ((((long)b * p.H + h) * p.nqb + qb) * 2 + which) * p.Nk * p.hd + (long)key * p.hd + col) = v;
+    } else {
+      const float f = which ? 1.f : p.scale;
+      char* dst = which ? p.dv + (krow + key) * p.lddv : p.dk + (krow + key) * p.lddk;
+      store4<T>(dst + g * hdb + col * (int)sizeof(T), v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+    }
+  }
+}
+
+// dk, dv of context c: the partials of every sample that uses it (in order), of the heads of the group and of the query
+// shares.  Eight lanes split the list of one result (4 channels) and join by a fixed tree.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) {
+  const int lane = threadIdx.x & 63, slice = lane >> 3;
+  const int per = p.hd >> 2, HG = p.H / p.G, U = HG * p.nqb;
+  const long n = (long)p.Bc * p.G * 2 * p.Nk * per;       // results, context slowest
+  const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6), i = wave * 8 + (lane & 7);
+  const long r = i < n ? i : n - 1;
+  const long gw = r / per, kw = gw / p.Nk, cg = kw >> 1;
+  const int col = (int)(r - gw * per) * 4, key = (int)(gw - kw * p.Nk), which = (int)(kw & 1);
+  const int g = (int)(cg % p.G), ctx = (int)(cg / p.G);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  int m = 0;
+  auto add = [&](int b) {
+    for (int u = (slice - m * U) & 7; u < U; u += 8) {
+      const long src = (((long)b * p.H + g * HG) * p.nqb + u) * 2 + which;      // (heads and shares are adjacent: hh * nqb + share)
+      s += *reinterpret_cast<const f32x4*>(p.part + (src * p.Nk + key) * p.hd + col);
+    }
+    ++m;
+  };
+  if (!p.index) {
+    if (p.Bc == 1) for (int b = 0; b < p.B; ++b) add(b);
+    else add(ctx);
+  } else {
+    for (int b = 0; b < p.B; ++b)
+      if (p.index[b] == ctx) add(b);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) s[j] += __shfl_xor(s[j], o, 64);
+  if (i >= n || slice) return;
+  const float f = which ? 1.f : p.scale;
+  const long krow = (long)ctx * p.Nk + key;
+  char* dst = which ? p.dv + krow * p.lddv : p.dk + krow * p.lddk;
+  store4<T>(dst + (g * p.hd + col) * (long)sizeof(T), s[0] * f, s[1] * f, s[2] * f, s[3] * f);
+}
+
+template <typename T, int HDP, int KT, bool DROP>
+int launch(const CrossParams& p, hipStream_t st) {
+  auto kern = cross_few_kernel<T, HDP, KT, DROP>;
+  constexpr int lds = few_lds<T, HDP, KT>();
+  static_assert(lds <= 160 * 1024, "LDS");
+  static unsigned long long attr_devs = 0ull;
+  if (dm_first_on_device(attr_devs) &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return DM_ERR_LAUNCH;
+  const long blocks = (long)p.B * p.nqb * p.H;
+  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  static const DmVariantName nm("cross_bwd_few<%s,%d,KT=%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, KT);
+  dm_set_variant(nm.s);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
+  DM_LAUNCH_CHECK();
+  if (p.nsplit) {
+    const long n = (long)p.Bc * p.G * 2 * p.Nk * (p.hd >> 2), gb = (n + 31) / 32;
+    if (gb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((cross_gather_kernel<T>), dim3((unsigned)gb), dim3(256), 0, st, p);
+    DM_LAUNCH_CHECK();
+  }
+  return DM_OK;
+}
+// tiles of 32 keys that a wave's registers hold beside the rest
+constexpr int most_tiles(int hdp, int esize) { return hdp <= 32 ? 3 : (esize == 2 && hdp == 64 ? 2 : 1); }
+template <typename T, int HDP> int pick(const CrossParams& p, int kt, hipStream_t st) {
+  if (kt == 1) return p.thresh ? launch<T, HDP, 1, true>(p, st) : launch<T, HDP, 1, false>(p, st);
+  constexpr int KT = most_tiles(HDP, sizeof(T));
+  if constexpr (KT > 1) return p.thresh ? launch<T, HDP, KT, true>(p, st) : launch<T, HDP, KT, false>(p, st);
+  return DM_ERR_ARG;
+}
+
+}  // namespace
+
+namespace dm_cross {
+
+bool few_plan(const dm_cross_args* a, FewPlan& f) {
+  const int hdp = cross_hdp(a->hd);
+  const int most = most_tiles(hdp, a->dtype == 0 ? 2 : 4);
+  if (a->Nk < 1 || a->Nk > 32 * most || (a->dtype != 0 && hdp > 64)) return false;
+  f.kt = a->Nk <= 32 ? 1 : most;
+  const long pairs = (long)a->B * a->heads, groups = ((long)a->Nq + 127) / 128;      // one tile per wave of a workgroup
+  long nqb = (1024 + pairs - 1) / pairs;                   // about four waves per SIMD over the device
+  if (nqb > groups) nqb = groups;
+  f.iters = (int)((groups + nqb - 1) / nqb);
+  f.nqb = (int)((groups + f.iters - 1) / f.iters);
+  f.direct = f.nqb == 1 && a->heads == a->kv_heads && !a->index && a->Bc == a->B;
+  f.ws = f.direct ? 0 : pairs * f.nqb * 2 * a->Nk * a->hd * 4;
+  return f.ws <= (1L << 29);
+}
+
+int few_launch(const CrossParams& p, const FewPlan& f, int dtype, hipStream_t st) {
+  const int hdp = cross_hdp(p.hd);
+  if (dtype == 0) {
+    switch (hdp) {
+      case 16: return pick<bf16, 16>(p, f.kt, st);
+      case 32: return pick<bf16, 32>(p, f.kt, st);
+      case 64: return pick<bf16, 64>(p, f.kt, st);
+      case 96: return pick<bf16, 96>(p, f.kt, st);
+      default: return pick<bf16, 128>(p, f.kt, st);
+    }
+  }
+  switch (hdp) {
+    case 16: return pick<float, 16>(p, f.kt, st);
+    case 32: return pick<float, 32>(p, f.kt, st);
+    default: return pick<float, 64>(p, f.kt, st);
+  }
+}
+
+}  // namespace dm_cross

@@ -7,38 +7,33 @@
 
 namespace {
 
+using namespace dm_cross;
+
 template <typename T, int HDP> struct FwdState {
   f32x16 acc[Geo<T, HDP>::DT];
   float m, l;
 };
 
-// NT tiles of 32 keys (LDS rows t0..) against the wave's 32 queries
-template <typename T, int HDP, int NT, bool DROP>
+// NT tiles of 32 keys (LDS rows t0..) against the wave's 32 queries.  FIRST: the state is not read but begun, with the
+// maximum of these tiles, so nothing is cleared or rescaled (up to 96 keys need no other step).
+template <typename T, int HDP, int NT, bool FIRST, bool DROP>
 __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>& st, const char* sK, const char* sV,
-                                         const uint32_t* bits, int t0, int key0, float c,
+                                         const uint32_t* bits, const float* bias, int t0, int key0, float c,
                                          const typename Cr<T>::frag (&qf)[Geo<T, HDP>::NC], uint32_t rs, int lane) {
   typedef Geo<T, HDP> Gm;
   const int half = lane >> 5;
-  uint32_t w[NT], any = 0;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    w[t] = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t0 + t]);
-    any |= w[t];
+  if (!FIRST) {
+    uint32_t any = bits[t0];
+    if (NT > 1) any |= bits[t0 + 1];
+    if (__builtin_amdgcn_readfirstlane((int)any) == 0) return;
   }
-  if (any == 0) return;
   f32x16 s[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+    s[t] = score_init(bias + (t0 + t) * 32, half);
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc)
       s[t] = Cr<T>::mma(row_frag<T>(sK + (t0 + t) * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s[t]);
-    if (w[t] != 0xFFFFFFFFu) {
-      const uint32_t mine = w[t] >> (4 * half);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[t][i] = (mine >> tile_row(i, 0)) & 1u ? s[t][i] : -INFINITY;
-    }
   }
   float mx = s[0][0];
 #pragma unroll
@@ -46,17 +41,22 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
   mx = half_max(mx);
-  // the reference maximum moves only when a block exceeds it by more than 2^8 in the probability: exact all the same
-  // (numerator and denominator share it), and the common block rescales nothing
-  const bool up = (mx - st.m) * c > 8.f;
-  if (__any(up)) {
-    const float alpha = up ? __builtin_amdgcn_exp2f((st.m - mx) * c) : 1.f;
-    st.m = up ? mx : st.m;
-    st.l *= alpha;
+  if (FIRST) {
+    st.m = mx;
+    st.l = 0.f;
+  } else {
+    // the reference maximum moves only when a block exceeds it by more than 2^8 in the probability: exact all the same
+    // (numerator and denominator share it), and the common block rescales nothing
+    const bool up = (mx - st.m) * c > 8.f;
+    if (__any(up)) {
+      const float alpha = up ? __builtin_amdgcn_exp2f((st.m - mx) * c) : 1.f;
+      st.m = up ? mx : st.m;
+      st.l *= alpha;
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d)
+      for (int d = 0; d < Gm::DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st.acc[d][i] *= alpha;
+        for (int i = 0; i < 16; ++i) st.acc[d][i] *= alpha;
+    }
   }
   const float mc = st.m == -INFINITY ? 0.f : st.m * c;
 #pragma unroll
@@ -79,7 +79,8 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
       const typename Cr<T>::frag pf = Cr<T>::pack(s[t], f);
 #pragma unroll
       for (int d = 0; d < Gm::DT; ++d)
-        st.acc[d] = Cr<T>::mma(tr_frag<T, HDP>(sV + (t0 + t) * 32 * Gm::ST, Gm::ST, f, d, lane), pf, st.acc[d]);
+        st.acc[d] = Cr<T>::mma(tr_frag<T, HDP>(sV + (t0 + t) * 32 * Gm::ST, Gm::ST, f, d, lane), pf,
+                               FIRST && t == 0 && f == 0 ? zero16() : st.acc[d]);
     }
   }
 }
@@ -91,36 +92,25 @@ __device__ __forceinline__ void fwd_finish(const CrossParams& p, const FwdState<
   const int half = lane >> 5;
   const float l = half_sum(st.l);
   const float mc = st.m == -INFINITY ? 0.f : st.m * c;
-  if (q >= p.Nq) return;
+  const bool ok = q < p.Nq;
   const long row = ((long)b * p.H + h) * p.Nq + q;
   if (p.nsplit > 1) {
     const long rows = (long)p.B * p.H * p.Nq;
-    float* o = p.part + (split * rows + row) * p.hd;
+    char* o = (char*)(p.part + (split * rows + row) * p.hd);
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = d * 32 + 8 * i + 4 * half;
-        if (col < p.hd) *reinterpret_cast<f32x4*>(o + col) = f32x4{st.acc[d][4 * i], st.acc[d][4 * i + 1], st.acc[d][4 * i + 2], st.acc[d][4 * i + 3]};
-      }
-    if (half == 0) {
+    for (int d = 0; d < Gm::DT; ++d) store_tile<float>(o, st.acc[d], 1.f, d * 32, p.hd, ok, half);
+    if (ok && half == 0) {
       float* ml = p.part + p.nsplit * rows * p.hd + (split * rows + row) * 2;
       ml[0] = mc;
       ml[1] = l;
     }
     return;
   }
-  const float inv = l == 0.f ? 0.f : p.inv_keep / l;
+  const float inv = l == 0.f ? 0.f : p.inv_keep * __builtin_amdgcn_rcpf(l);      // (v_rcp_f32: 1 ulp)
   char* o = p.o + ((long)b * p.Nq + q) * p.ldo + h * p.hd * (long)sizeof(T);
 #pragma unroll
-  for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int col = d * 32 + 8 * i + 4 * half;
-      if (col < p.hd)
-        store4<T>(o + col * sizeof(T), st.acc[d][4 * i] * inv, st.acc[d][4 * i + 1] * inv, st.acc[d][4 * i + 2] * inv, st.acc[d][4 * i + 3] * inv);
-    }
-  if (half == 0) p.lse[row] = l == 0.f ? -INFINITY : (mc + log2f(l)) * CR_LN2;
+  for (int d = 0; d < Gm::DT; ++d) store_tile<T>(o, st.acc[d], inv, d * 32, p.hd, ok, half);
+  if (ok && half == 0) p.lse[row] = l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * CR_LN2;
 }
 
 // A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
@@ -131,7 +121,8 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
   char* sV = sK + p.kb * Gm::SR;
-  uint32_t* bits = reinterpret_cast<uint32_t*>(sV + p.kb * Gm::ST);
+  float* bias = reinterpret_cast<float*>(sV + p.kb * Gm::ST);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(bias + p.kb);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
@@ -151,51 +142,71 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) 
   const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
 
   FwdState<T, HDP> st;
-  typename Cr<T>::frag qf[Gm::NC];
+  typename Cr<T>::frag qf[Gm::NC], nf[Gm::NC];
   uint32_t rs = 0;
+  const char* qrow = p.q + ((long)b * p.Nq + qb * p.iters * 128 + wave * 32 + (lane & 31)) * p.ldq + h * hdb;
+  constexpr bool AHEAD = Gm::NC <= 4;          // (wider rows would not fit the registers twice)
+  auto fetch = [&](int q) { load_frags<T, HDP>(qrow, q < p.Nq, hdb, lane, nf); };
   auto begin = [&](int q) {
-    load_frags<T, HDP>(p.q + ((long)b * p.Nq + q) * p.ldq + h * hdb, q < p.Nq, hdb, lane, qf);
+    if (!AHEAD) fetch(q);
+#pragma unroll
+    for (int kc = 0; kc < Gm::NC; ++kc) qf[kc] = nf[kc];
     if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q));
+  };
+  auto clear = [&]() {
     st.m = -INFINITY;
     st.l = 0.f;
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.acc[d][i] = 0.f;
+    for (int d = 0; d < Gm::DT; ++d) st.acc[d] = zero16();
   };
   auto stage = [&](int from, int n) {
     stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, k1, mask, hdb, tid);
     stage_rows<T, HDP>(sV, Gm::ST, vbase, p.ldv, from, n, k1, mask, hdb, tid);
-    stage_bits(bits, from, n, k1, mask, tid);
+    stage_valid(bits, bias, from, n, k1, mask, tid);
   };
-  auto sweep = [&](int from, int tiles) {
-    int t = 0;
-    for (; t + 2 <= tiles; t += 2) fwd_step<T, HDP, 2, DROP>(p, st, sK, sV, bits, t, from + t * 32, c, qf, rs, lane);
-    if (t < tiles) fwd_step<T, HDP, 1, DROP>(p, st, sK, sV, bits, t, from + t * 32, c, qf, rs, lane);
-  };
+#define DM_STEP(NT, FIRST, t, from) \
+  fwd_step<T, HDP, NT, FIRST, DROP>(p, st, sK, sV, bits, bias, t, (from) + (t) * 32, c, qf, rs, lane)
   const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
+  if (AHEAD) fetch(q0);
   if (RES) {
-    const int n = max(0, (k1 - k0 + 31) & ~31);
+    const int n = max(0, (k1 - k0 + 31) & ~31), tiles = n >> 5;
     stage(k0, n);
     __syncthreads();
     for (int it = 0; it < p.iters; ++it) {
       const int q = q0 + it * 128;
       if (q - (lane & 31) >= p.Nq) break;      // (wave-uniform)
       begin(q);
-      sweep(k0, n >> 5);
+      if (it + 1 < p.iters) {                  // the next tile's queries fly while this one is computed
+        qrow += 128 * p.ldq;
+        if (AHEAD) fetch(q + 128);
+      }
+      int t = 2;
+      if (tiles == 0) clear();
+      else if (tiles == 1) DM_STEP(1, true, 0, k0);
+      else if (tiles & 1) {
+        if (HDP <= 64) DM_STEP(3, true, 0, k0);
+        else { DM_STEP(2, true, 0, k0); DM_STEP(1, false, 2, k0); }
+        t = 3;
+      }
+      else DM_STEP(2, true, 0, k0);
+      for (; t < tiles; t += 2) DM_STEP(2, false, t, k0);
       fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
     }
   } else {
     begin(q0);
+    clear();
     for (int from = k0; from < k1; from += p.kb) {
-      const int n = min(p.kb, (k1 - from + 31) & ~31);
+      const int n = min(p.kb, (k1 - from + 31) & ~31), tiles = n >> 5;
       __syncthreads();
       stage(from, n);
       __syncthreads();
-      sweep(from, n >> 5);
+      int t = 0;
+      for (; t + 2 <= tiles; t += 2) DM_STEP(2, false, t, from);
+      if (t < tiles) DM_STEP(1, false, t, from);
     }
     fwd_finish<T, HDP>(p, st, b, h, q0, split, c, lane);
   }
+#undef DM_STEP
 }
 
 // joins the key splits: thread = (row, 4 channels)
@@ -253,7 +264,7 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   f.ksplit = ns > 1 ? (int)((((long)a->Nk + ns - 1) / ns + 63) & ~63L) : a->Nk;
   f.nsplit = ns > 1 ? (a->Nk + f.ksplit - 1) / f.ksplit : 1;
   const int kbytes = key_bytes(a);
-  const int image = (LDS_IMAGE - 512) / kbytes / 64 * 64;     // keys per LDS image
+  const int image = (LDS_IMAGE - 64) / (kbytes + 5) / 64 * 64;     // keys per LDS image
   const int need = (f.ksplit + 63) & ~63;
   f.res = need <= image;
   f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
@@ -266,6 +277,7 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
     f.iters = it < 1 ? 1 : (int)it;
   }
   f.nqb = (int)((groups + f.iters - 1) / f.iters);
+  f.iters = (int)((groups + f.nqb - 1) / f.nqb);              // (evenly)
   f.ws = f.nsplit > 1 ? (long)f.nsplit * a->B * a->heads * a->Nq * (a->hd + 2) * 4 : 0;
   return f;
 }
@@ -277,7 +289,7 @@ int launch_fwd(const CrossParams& p, hipStream_t st) {
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST) + (p.kb / 32 + 2) * 4;
+  const size_t lds = (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4;
   const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, RES ? "resident" : "streamed");
@@ -308,7 +320,7 @@ template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t
 
 }  // namespace
 
-extern "C" long dm_cross_fwd_workspace_bytes(const dm_cross_args* a) { return cross_sizes_ok(a) ? fwd_plan(a).ws : 0; }
+extern "C" long dm_cross_fwd_workspace_bytes(const dm_cross_args* a) { return dm_cross::cross_sizes_ok(a) ? fwd_plan(a).ws : 0; }
 
 extern "C" int dm_cross_fwd(const dm_cross_args* a, dm_stream_t stream) {
   CrossParams p{};

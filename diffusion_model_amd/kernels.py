@@ -764,54 +764,58 @@ def rope(x, heads: int, plan: RopePlan, *, grid=None, positions=None, inverse: b
     if Cc >= 65536:
         raise ValueError("rope: at most 65535 channels")
     nax = len(plan.axes)
-    if (grid is None) == (positions is None):
-        raise ValueError("rope: give either grid or positions")
+    pos_ptr, pos_f32, pos_stride, places = None, 0, 0, _NO_GRID
     if grid is not None:
-        grid = tuple(int(n) for n in grid)
-        if len(grid) != nax or any(n < 1 for n in grid) or math.prod(grid) != N:
-            raise ValueError(f"rope: grid {grid} does not place {N} tokens on {nax} axes")
+        if positions is not None:
+            raise ValueError("rope: give either grid or positions")
+        if len(grid) != nax or min(grid) < 1 or math.prod(grid) != N:
+            raise ValueError(f"rope: grid {tuple(grid)} does not place {N} tokens on {nax} axes")
+        places = _GRID3(*grid)
+    elif positions is None:
+        raise ValueError("rope: give either grid or positions")
     else:
         if positions.dtype not in (torch.int32, F32) or not positions.is_contiguous():
             raise ValueError("rope: positions must be contiguous int32 or float32")
         if tuple(positions.shape) not in ((N, nax), (B, N, nax)):
             raise ValueError(f"rope: positions must be [{N}, {nax}] or [{B}, {N}, {nax}], got {tuple(positions.shape)}")
+        pos_ptr, pos_f32 = positions.data_ptr(), int(positions.dtype == F32)
+        pos_stride = N * nax if positions.dim() == 3 else 0
     if out is None:
-        out = torch.empty((B, N, Cc), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("rope: out must have x's shape and type")
     _same_device("rope", x, out, plan.freq, plan.axis, positions)
-    if x.numel() == 0:
+    if B == 0 or N == 0:
         return out
-    a = RopeArgs()
-    a.x, a.ldx, a.y, a.ldy = _p(x), _act(x, "x"), _p(out), _act(out, "out")
-    a.dtype, a.B, a.N, a.heads, a.hd, a.rot = int(_is32(x)), B, N, heads, plan.head_dim, plan.rot
-    a.pairing, a.freq, a.axis, a.axes = int(plan.pairing == "half"), _p(plan.freq), _p(plan.axis), nax
-    if positions is not None:
-        a.pos, a.pos_f32 = _p(positions), int(positions.dtype == F32)
-        a.pos_batch_stride = N * nax if positions.dim() == 3 else 0
-    else:
-        for i, n in enumerate(grid):
-            a.grid[i] = n
-    a.inverse = int(inverse)
+    a = RopeArgs(x.data_ptr(), _act(x, "x"), out.data_ptr(), _act(out, "out"), int(x.dtype == F32), B, N, heads, plan.head_dim,
+                 plan.rot, int(plan.pairing == "half"), plan.freq.data_ptr(), plan.axis.data_ptr(), nax, pos_ptr, pos_f32,
+                 pos_stride, places, int(inverse))
     check(_lib.lib().dm_rope(C.byref(a), _stream()), "dm_rope")
     return out
 
 
+_GRID3 = C.c_int * 3
+_NO_GRID = _GRID3()
+
+
 def _same_device(what: str, *tensors) -> None:
     """Every operand on the current HIP device: kernels go to that device's current stream."""
-    if _FORCED_STREAM[0] is None:
-        for t in tensors:
-            if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
-                raise ValueError(f"{what}: every tensor must be on the current GPU, got {t.device}")
+    cur = _GET_DEVICE() if _GET_DEVICE is not None and torch.cuda.is_initialized() else None
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise ValueError(f"{what}: every tensor must be on the current GPU, got {t.device}")
 
 
 # --------------------------------------------------------------------------- attention to encoder states
-def _cross_args(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed):
-    if q.dim() != 3 or k.dim() != 3 or q.dtype not in (BF16, F32):
+def _cross_check(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p):
+    """Refuses what the kernels do not take; returns (B, Bc, kv_heads, Nq, Nk, hd, scale)."""
+    dt = q.dtype
+    if q.dim() != 3 or k.dim() != 3 or dt not in (BF16, F32):
         raise ValueError(f"{what}: q must be [B, Nq, heads * hd] and k, v [Bc, Nk, kv_heads * hd], bf16 or float32")
-    if k.dtype != q.dtype or v.dtype != q.dtype or v.shape != k.shape:
+    if k.dtype != dt or v.dtype != dt or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must have one shape, and q's type")
-    kv_heads = heads if kv_heads is None else kv_heads
+    if kv_heads is None:
+        kv_heads = heads
     B, Nq, Cq = q.shape
     Bc, Nk, Ck = k.shape
     if heads < 1 or kv_heads < 1 or heads % kv_heads or Cq % heads or Ck * heads != Cq * kv_heads:
@@ -819,42 +823,37 @@ def _cross_args(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p
     hd = Cq // heads
     if hd % 8 or not 8 <= hd <= 128:
         raise ValueError(f"{what}: head width {hd} is not a multiple of 8 up to 128")
-    if index is None and Bc not in (1, B):
+    if index is None and Bc != B and Bc != 1:
         raise ValueError(f"{what}: {Bc} contexts for {B} samples need an index")
     if Bc == 0 and B > 0:
         raise ValueError(f"{what}: no context")
-    for t, name, shape, types in ((lens, "lens", (Bc,), (torch.int32,)), (index, "index", (B,), (torch.int32,)),
-                                  (mask, "mask", (Bc, Nk), (torch.bool, torch.uint8))):
-        if t is not None and (tuple(t.shape) != shape or t.dtype not in types or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be a contiguous {types[0]} tensor of shape {shape}")
+    if lens is not None and (lens.shape != (Bc,) or lens.dtype != torch.int32 or not lens.is_contiguous()):
+        raise ValueError(f"{what}: lens must be a contiguous int32 tensor [{Bc}]")
+    if index is not None and (index.shape != (B,) or index.dtype != torch.int32 or not index.is_contiguous()):
+        raise ValueError(f"{what}: index must be a contiguous int32 tensor [{B}]")
+    if mask is not None and (mask.shape != (Bc, Nk) or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
+        raise ValueError(f"{what}: mask must be a contiguous bool tensor [{Bc}, {Nk}]")
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"{what}: scale must be positive")
     if not 0.0 <= drop_p < 1.0:
         raise ValueError(f"{what}: drop_p must be in [0, 1)")
     _same_device(what, q, k, v, lens, mask, index)
-    a = CrossArgs()
-    a.B, a.Bc, a.heads, a.kv_heads, a.Nq, a.Nk, a.hd, a.dtype = B, Bc, heads, kv_heads, Nq, Nk, hd, int(_is32(q))
-    a.scale, a.drop_p, a.drop_seed = scale, float(drop_p), int(drop_seed)
-    a.lens, a.mask, a.index = _p(lens), _p(mask), _p(index)
-    a.q, a.ldq = _rows16(what, "q", q)
-    if Nk:
-        (a.k, a.ldk), (a.v, a.ldv) = _rows16(what, "k", k), _rows16(what, "v", v)
-    return a
+    return B, Bc, kv_heads, Nq, Nk, hd, scale
 
 
-def _rows16(what, name, t):
-    if t.numel() == 0:
-        return None, t.shape[-1]
-    ld = _act(t, name)
-    if t.data_ptr() % 16 or ld * t.element_size() % 16:
+def _rows16(what, name, t, esize):
+    """(address, row stride) of [.., .., C] rows that start on 16-byte boundaries."""
+    ld = t.shape[-1] if t.is_contiguous() else _act(t, name)
+    ptr = t.data_ptr()
+    if (ptr | ld * esize) & 15:
         raise ValueError(f"{what}: the rows of {name} must be 16-byte aligned")
-    return _p(t), ld
+    return ptr, ld
 
 
 def _cross_out(what, name, t, like):
     if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if t.shape != like.shape or t.dtype != like.dtype:
         raise ValueError(f"{what}: {name} must have the shape {tuple(like.shape)} and the operands' type")
     _same_device(what, t)
@@ -869,21 +868,24 @@ def cross_fwd(q, k, v, heads: int, *, kv_heads: Optional[int] = None, lens=None,
     their intersection); what invalid states hold does not matter, and a sample without any valid state gets o = 0 and
     lse = -inf.  ``index`` int32 [B]: the context of each sample (without it: one each, or Bc == 1 for all); an index
     outside [0, Bc) means no states.  ``kv_heads``: key / value heads, each shared by heads / kv_heads query heads."""
-    a = _cross_args("cross_fwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed)
+    B, Bc, kv_heads, Nq, Nk, hd, scale = _cross_check("cross_fwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p)
     out = _cross_out("cross_fwd", "out", out, q)
-    lse = torch.empty((a.B, heads, a.Nq), dtype=F32, device=q.device)
-    if out.numel() == 0:
+    lse = torch.empty((B, heads, Nq), dtype=F32, device=q.device)
+    if B == 0 or Nq == 0:
         return out, lse
-    a.o, a.ldo = _rows16("cross_fwd", "out", out)
-    a.lse = _p(lse)
-    L = _lib.lib()
-    nb = L.dm_cross_fwd_workspace_bytes(C.byref(a))
+    f32m = q.dtype == F32
+    es = 4 if f32m else 2
+    a = CrossArgs(*_rows16("cross_fwd", "q", q, es), *_rows16("cross_fwd", "k", k, es), *_rows16("cross_fwd", "v", v, es),
+                  *_rows16("cross_fwd", "out", out, es), lse.data_ptr(), None, 0, None, 0, None, 0, None, 0,
+                  _p(lens), _p(mask), _p(index), B, Bc, heads, kv_heads, Nq, Nk, hd, int(f32m), scale, drop_p, drop_seed)
+    L, ref = _lib.lib(), C.byref(a)
+    nb = L.dm_cross_fwd_workspace_bytes(ref)
     if nb:
         # a block of its own per call, not the shared workspace(): the allocator orders it on this stream, and graphs
         # captured from two calls never share it
         ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
-        a.workspace, a.ws_bytes = _p(ws), nb
-    check(L.dm_cross_fwd(C.byref(a), _stream()), "dm_cross_fwd")
+        a.workspace, a.ws_bytes = ws.data_ptr(), nb
+    check(L.dm_cross_fwd(ref, _stream()), "dm_cross_fwd")
     return out, lse
 
 
@@ -891,28 +893,29 @@ def cross_bwd(q, k, v, o, lse, d_o, heads: int, *, kv_heads: Optional[int] = Non
               scale: Optional[float] = None, drop_p: float = 0.0, drop_seed: int = 0, dq=None, dk=None, dv=None):
     """Backward of cross_fwd with the same options: (dq, dk, dv) in q's, k's and v's shapes.  dk and dv are sums over the
     query heads of a group and over the samples that share a context, in a fixed order; rows of invalid states are zero."""
-    a = _cross_args("cross_bwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p, drop_seed)
-    for t, name in ((o, "o"), (d_o, "d_o")):
-        if t.shape != q.shape or t.dtype != q.dtype:
-            raise ValueError(f"cross_bwd: {name} must have q's shape and type")
-    if tuple(lse.shape) != (a.B, heads, a.Nq) or lse.dtype != F32 or not lse.is_contiguous():
+    B, Bc, kv_heads, Nq, Nk, hd, scale = _cross_check("cross_bwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p)
+    if o.shape != q.shape or d_o.shape != q.shape or o.dtype != q.dtype or d_o.dtype != q.dtype:
+        raise ValueError("cross_bwd: o and d_o must have q's shape and type")
+    if lse.shape != (B, heads, Nq) or lse.dtype != F32 or not lse.is_contiguous():
         raise ValueError("cross_bwd: lse must be cross_fwd's")
     _same_device("cross_bwd", o, d_o, lse)
     dq = _cross_out("cross_bwd", "dq", dq, q)
     dk, dv = _cross_out("cross_bwd", "dk", dk, k), _cross_out("cross_bwd", "dv", dv, v)
-    if q.numel() == 0:
+    if B == 0 or Nq == 0:
         return dq, dk.zero_(), dv.zero_()
-    a.o, a.ldo = _rows16("cross_bwd", "o", o)
-    a.d_o, a.lddo = _rows16("cross_bwd", "d_o", d_o)
-    a.dq, a.lddq = _rows16("cross_bwd", "dq", dq)
-    a.dk, a.lddk = _rows16("cross_bwd", "dk", dk)
-    a.dv, a.lddv = _rows16("cross_bwd", "dv", dv)
-    a.lse = _p(lse)
-    L = _lib.lib()
-    nb = L.dm_cross_bwd_workspace_bytes(C.byref(a))
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
-    a.workspace, a.ws_bytes = _p(ws), nb
-    check(L.dm_cross_bwd(C.byref(a), _stream()), "dm_cross_bwd")
+    f32m = q.dtype == F32
+    es = 4 if f32m else 2
+    w = "cross_bwd"
+    a = CrossArgs(*_rows16(w, "q", q, es), *_rows16(w, "k", k, es), *_rows16(w, "v", v, es), *_rows16(w, "o", o, es),
+                  lse.data_ptr(), *_rows16(w, "d_o", d_o, es), *_rows16(w, "dq", dq, es), *_rows16(w, "dk", dk, es),
+                  *_rows16(w, "dv", dv, es), _p(lens), _p(mask), _p(index), B, Bc, heads, kv_heads, Nq, Nk, hd, int(f32m),
+                  scale, drop_p, drop_seed)
+    L, ref = _lib.lib(), C.byref(a)
+    nb = L.dm_cross_bwd_workspace_bytes(ref)
+    if nb:
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)      # (as in cross_fwd)
+        a.workspace, a.ws_bytes = ws.data_ptr(), nb
+    check(L.dm_cross_bwd(ref, _stream()), "dm_cross_bwd")
     return dq, dk, dv
 
 

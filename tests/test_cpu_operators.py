@@ -100,14 +100,18 @@ def test_cross_entry_points_refuse(kw):
 @pytest.mark.parametrize("kw", [dict(d_o=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(lddq=60), dict(workspace=None),
                                 dict(ws_bytes=4), dict(workspace=4100)])
 def test_cross_backward_entry_point_refuses(kw):
-    assert _lib.lib().dm_cross_bwd(ctypes.byref(cross_struct(**kw)), None) == -1
+    assert _lib.lib().dm_cross_bwd(ctypes.byref(cross_struct(Nk=600, **kw)), None) == -1      # (so many keys need scratch)
 
 
 def test_cross_workspace_bytes():
     L = _lib.lib()
     assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(cross_struct())) == 0
     assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(cross_struct(Nq=1, Nk=4096))) > 0     # few rows: keys are split
-    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct())) >= 2 * 2 * 5 * 4
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct(Nk=600))) >= 2 * 2 * 5 * 4
+    shared = cross_struct(heads=4, ldq=128, ldo=128, lddo=128, lddq=128)       # few keys: one partial per query head
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(shared)) == 2 * 4 * 2 * 7 * 32 * 4
+    shared.workspace = None
+    assert L.dm_cross_bwd(ctypes.byref(shared), None) == -1
     assert L.dm_cross_fwd_workspace_bytes(None) == 0 and L.dm_cross_fwd(None, None) == -1 and L.dm_cross_bwd(None, None) == -1
     few = cross_struct(Nq=1, Nk=4096, workspace=None)
     assert L.dm_cross_fwd(ctypes.byref(few), None) == -1
