@@ -12,7 +12,7 @@ using namespace dm_cross;
 
 // ---------------------------------------------------------------- dQ (and delta)
 template <typename T, int HDP, bool RES, bool DROP>
-__global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cross_dq_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
   char* sV = sK + p.kb * Gm::SR;
   float* bias = reinterpret_cast<float*>(sV + p.kb * Gm::SR);
   uint32_t* bits = reinterpret_cast<uint32_t*>(bias + p.kb);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
   id /= p.H;
@@ -37,13 +37,14 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
   f32x16 acc[Gm::DT];
   float L2 = 0.f, delta = 0.f;
   uint32_t rs = 0;
-  auto begin = [&](int q) {
+  auto begin = [&](int q0) {                   // q0: the wave's first query
+    const int q = q0 + (lane & 31), left = p.Nq - q0;
     const bool ok = q < p.Nq;
-    const long tok = (long)b * p.Nq + q, row = ((long)b * p.H + h) * p.Nq + q;
-    load_frags<T, HDP>(p.q + tok * p.ldq + h * hdb, ok, hdb, lane, qf);
-    load_frags<T, HDP>(p.d_o + tok * p.lddo + h * hdb, ok, hdb, lane, df);
+    const long tok = (long)b * p.Nq + q0, row = ((long)b * p.H + h) * p.Nq + q;
+    load_frags<T, HDP>(rows_of(p.q + tok * p.ldq + h * hdb, p.ldq, left, hdb, lane), hdb, lane, qf);
+    load_frags<T, HDP>(rows_of(p.d_o + tok * p.lddo + h * hdb, p.lddo, left, hdb, lane), hdb, lane, df);
     frag of[Gm::NC];
-    load_frags<T, HDP>(p.o + tok * p.ldo + h * hdb, ok, hdb, lane, of);
+    load_frags<T, HDP>(rows_of(p.o + tok * p.ldo + h * hdb, p.ldo, left, hdb, lane), hdb, lane, of);
     float s = 0.f;
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc)
@@ -60,8 +61,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   };
   auto stage = [&](int from, int n) {
-    stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, kn, mask, hdb, tid);
-    stage_rows<T, HDP>(sV, Gm::SR, vbase, p.ldv, from, n, kn, mask, hdb, tid);
+    stage_rows2<T, HDP>(sK, Gm::SR, kbase, p.ldk, sV, Gm::SR, vbase, p.ldv, from, n, kn, mask, hdb, tid);
     stage_valid(bits, bias, from, n, kn, mask, tid);
   };
   auto sweep = [&](int from, int tiles) {
@@ -96,18 +96,18 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const CrossParams p) {
     }
   };
   auto finish = [&](int q) {
-    char* dst = p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb;
+    const Rows dst = rows_of(p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb, p.lddq, p.Nq - q, hdb, lane);
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, acc[d], p.scale, d * 32, p.hd, q < p.Nq, half);
+    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, acc[d], p.scale, d * 32, hdb, lane);
   };
-  const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
+  const int q0 = qb * p.iters * 128 + wave * 32;
   if (RES) {
     const int n = (kn + 31) & ~31;
     stage(0, n);
     __syncthreads();
     for (int it = 0; it < p.iters; ++it) {
       const int q = q0 + it * 128;
-      if (q - (lane & 31) >= p.Nq) break;
+      if (q >= p.Nq) break;
       begin(q);
       sweep(0, n >> 5);
       finish(q);
@@ -172,8 +172,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && HDP > 64) ? 1 : 2) void cro
     const int h = g * HG + hh, r0 = qc * QS;
     const long tok = (long)b * p.Nq, row = ((long)b * p.H + h) * p.Nq;
     __syncthreads();
-    stage_rows<T, HDP>(sQ, Gm::SR, p.q + tok * p.ldq + h * hdb, p.ldq, r0, QS, p.Nq, nullptr, hdb, tid);
-    stage_rows<T, HDP>(sD, Gm::SR, p.d_o + tok * p.lddo + h * hdb, p.lddo, r0, QS, p.Nq, nullptr, hdb, tid);
+    stage_rows2<T, HDP>(sQ, Gm::SR, p.q + tok * p.ldq + h * hdb, p.ldq, sD, Gm::SR, p.d_o + tok * p.lddo + h * hdb, p.lddo,
+                        r0, QS, p.Nq, nullptr, hdb, tid);
     if (tid < QS) {
       const int q = r0 + tid;
       const float l = q < p.Nq ? p.lse[row + q] * CR_LOG2E : INFINITY;

@@ -14,17 +14,68 @@ namespace {
 using namespace dm_cross;
 
 template <typename T> constexpr int patch_stride() { return sizeof(T) == 2 ? 72 : 144; }   // 32 keys + padding: writes without conflicts
-template <typename T, int HDP> constexpr int wave_lds() { return 2 * 32 * Geo<T, HDP>::ST + 2 * 32 * patch_stride<T>(); }
+// P / dS tile pairs that go through LDS together: all of them in bf16, one at a time in fp32 (twice the bytes, and bound by
+// its matrix instructions anyway)
+template <typename T, int KT> constexpr int pairs() { return sizeof(T) == 2 ? KT : 1; }
+template <typename T, int HDP, int KT> constexpr int wave_lds() {
+  return 2 * 32 * Geo<T, HDP>::ST + pairs<T, KT>() * 2 * 32 * patch_stride<T>();
+}
 template <typename T, int HDP, int KT> constexpr int few_lds() {
-  const int keys = KT * 32 * (2 * Geo<T, HDP>::SR + 4) + 32, loop = keys + 4 * wave_lds<T, HDP>();
+  const int keys = KT * 32 * (2 * Geo<T, HDP>::SR + 4) + 32, loop = keys + 4 * wave_lds<T, HDP, KT>();
   const int sums = 2 * KT * 32 * (HDP + 4) * 4;
   return loop > sums ? loop : sums;
 }
 
 // waves per SIMD that the registers allow (dK and dV alone take 32 KT HDP / 32)
 template <typename T, int HDP, int KT> constexpr int few_waves() {
-  return sizeof(T) == 2 ? (HDP <= 32 || (HDP == 64 && KT == 1) ? 2 : 1) : (HDP <= 32 && KT == 1 ? 2 : 1);
+  return HDP * KT <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1;
 }
+
+// dK^T or dV^T of one tile of 32 keys, and what is added to it: X^T (LDS, 32 queries) times the P or dS tile (LDS patch).
+// 16-wide heads in bf16 use the 16x16 tiles, which they fill: half the registers of a 32x32 one.
+template <typename T, int HDP> struct KvAcc {
+  static constexpr int N = Geo<T, HDP>::DT;
+  f32x16 a[N];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < N; ++d) a[d] = zero16();
+  }
+  __device__ __forceinline__ void add(const char* x, const char* patch, int f, int lane) {
+    const typename Cr<T>::frag pf = tr_frag<T, 32>(patch, patch_stride<T>(), f, 0, lane);
+#pragma unroll
+    for (int d = 0; d < N; ++d) a[d] = Cr<T>::mma(tr_frag<T, HDP>(x, Geo<T, HDP>::ST, f, d, lane), pf, a[d]);
+  }
+  // four consecutive channels at a time: f(key in the tile, channel, values)
+  template <typename F> __device__ __forceinline__ void each(int lane, const F& f) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int i = 0; i < (HDP < 32 ? 2 : 4); ++i)
+        f(lane & 31, d * 32 + 8 * i + 4 * (lane >> 5), f32x4{a[d][4 * i], a[d][4 * i + 1], a[d][4 * i + 2], a[d][4 * i + 3]});
+  }
+};
+template <> struct KvAcc<bf16, 16> {
+  f32x4 a[2];      // keys 0..15 and 16..31
+  __device__ __forceinline__ void clear() { a[0] = a[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  static __device__ __forceinline__ bf16x8 operand(const char* tile, int stride, int lane) {
+    typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
+    const char* at = tile + (8 * (lane >> 4) + ((lane & 15) >> 2)) * stride + (lane & 3) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * stride));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  __device__ __forceinline__ void add(const char* x, const char* patch, int f, int lane) {
+    if (f) return;      // (one instruction reduces over all 32 queries)
+    const bf16x8 xt = operand(x, Geo<bf16, 16>::ST, lane);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      a[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xt, operand(patch + 32 * k, patch_stride<bf16>(), lane), a[k], 0, 0, 0);
+  }
+  template <typename F> __device__ __forceinline__ void each(int lane, const F& f) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f(16 * k + (lane & 15), 4 * (lane >> 4), a[k]);
+  }
+};
 
 template <typename T> __device__ __forceinline__ void put_tile(char* patch, const f32x16& s, int lane) {
 #pragma unroll
@@ -32,21 +83,106 @@ template <typename T> __device__ __forceinline__ void put_tile(char* patch, cons
     store4<T>(patch + (lane & 31) * patch_stride<T>() + (8 * i + 4 * (lane >> 5)) * (int)sizeof(T), s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
 }
 
+// NT tiles of 32 keys against the wave's 32 queries: dk, dv += ..., dq = ... .  All tiles go through each stage together, so
+// that one tile's exponentials run beside the next one's matrix instructions.
+template <typename T, int HDP, int KT, int NT, bool DROP, typename Next>
+__device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, const char* sV, const float* bias, const char* sQ,
+                                         const char* sD, char* patch, const typename Cr<T>::frag (&qf)[Geo<T, HDP>::NC],
+                                         const typename Cr<T>::frag (&df)[Geo<T, HDP>::NC], float lse2, float c, uint32_t rs,
+                                         KvAcc<T, HDP> (&dk)[KT], KvAcc<T, HDP> (&dv)[KT],
+                                         f32x16 (&dq)[Geo<T, HDP>::DT], int lane, const Next& next) {
+  typedef Geo<T, HDP> Gm;
+  typedef typename Cr<T>::frag frag;
+  constexpr int PS = patch_stride<T>(), NF = Cr<T>::NF, PT = pairs<T, KT>();
+  const int half = lane >> 5;
+  f32x16 pr[NT], dp[NT];
+  uint32_t keep[NT];
+  float delta = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    f32x16 s = score_init(bias + t * 32, half), e = zero16();
+#pragma unroll
+    for (int kc = 0; kc < Gm::NC; ++kc) {
+      s = Cr<T>::mma(row_frag<T>(sK + t * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s);
+      e = Cr<T>::mma(row_frag<T>(sV + t * 32 * Gm::SR, Gm::SR, kc, lane), df[kc], e);
+    }
+    pr[t] = s;
+    dp[t] = e;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (DROP) {
+      keep[t] = 0;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t z = dm_drop_bits(rs, (uint32_t)(t * 32 + tile_row(i, half)) >> 1);
+        const bool k0 = dm_keep16(z, 0, p.thresh), k1 = dm_keep16(z, 1, p.thresh);
+        keep[t] |= (k0 ? 1u : 0u) << i | (k1 ? 2u : 0u) << i;
+        dp[t][i] = k0 ? dp[t][i] * p.inv_keep : 0.f;
+        dp[t][i + 1] = k1 ? dp[t][i + 1] * p.inv_keep : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      pr[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(pr[t][i], c, -lse2));
+      delta = __builtin_fmaf(pr[t][i], dp[t][i], delta);
+    }
+  }
+  delta = half_sum(delta);
+  next();                       // the next tile's rows fly during the products below
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[t][i] = pr[t][i] * (dp[t][i] - delta);
+    if (DROP) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const frag sf = Cr<T>::pack(dp[t], f);
+#pragma unroll
+      for (int d = 0; d < Gm::DT; ++d)
+        dq[d] = Cr<T>::mma(tr_frag<T, HDP>(sK + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, t == 0 && f == 0 ? zero16() : dq[d]);
+      if (KT > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+  for (int t0 = 0; t0 < NT; t0 += PT) {
+#pragma unroll
+    for (int t = t0; t < NT && t < t0 + PT; ++t) {
+      put_tile<T>(patch + 2 * (t - t0) * 32 * PS, pr[t], lane);
+      put_tile<T>(patch + (2 * (t - t0) + 1) * 32 * PS, dp[t], lane);
+    }
+    wave_lds_order();
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+#pragma unroll
+      for (int t = t0; t < NT && t < t0 + PT; ++t) {
+        dv[t].add(sD, patch + 2 * (t - t0) * 32 * PS, f, lane);
+        dk[t].add(sQ, patch + (2 * (t - t0) + 1) * 32 * PS, f, lane);
+      }
+      if (KT > 1) __builtin_amdgcn_sched_barrier(0);      // (all operand reads at once would not fit the registers)
+    }
+    wave_lds_order();
+  }
+}
+
 template <typename T, int HDP, int KT, bool DROP>
 __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
-  constexpr int PS = patch_stride<T>(), NF = Cr<T>::NF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
   char* sV = sK + KT * 32 * Gm::SR;
   float* bias = reinterpret_cast<float*>(sV + KT * 32 * Gm::SR);
   uint32_t* bits = reinterpret_cast<uint32_t*>(bias + KT * 32);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  char* sQ = reinterpret_cast<char*>(bits + 8) + wave * wave_lds<T, HDP>();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  char* sQ = reinterpret_cast<char*>(bits + 8) + wave * wave_lds<T, HDP, KT>();
   char* sD = sQ + 32 * Gm::ST;
-  char* sP = sD + 32 * Gm::ST;
-  char* sS = sP + 32 * PS;
+  char* patch = sD + 32 * Gm::ST;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
   id /= p.H;
@@ -61,108 +197,52 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
 
   frag qf[Gm::NC], df[Gm::NC];
   float L2;
-  auto fetch = [&](int q) {
-    const bool ok = q < p.Nq;
-    load_frags<T, HDP>(p.q + (tok + q) * p.ldq + h * hdb, ok, hdb, lane, qf);
-    load_frags<T, HDP>(p.d_o + (tok + q) * p.lddo + h * hdb, ok, hdb, lane, df);
-    L2 = ok ? p.lse[row + q] : INFINITY;
+  auto fetch = [&](int q) {      // q: the wave's first query
+    const int left = p.Nq - q;
+    load_frags<T, HDP>(rows_of(p.q + (tok + q) * p.ldq + h * hdb, p.ldq, left, hdb, lane), hdb, lane, qf);
+    load_frags<T, HDP>(rows_of(p.d_o + (tok + q) * p.lddo + h * hdb, p.lddo, left, hdb, lane), hdb, lane, df);
+    L2 = p.lse[row + min(q + (lane & 31), p.Nq - 1)];
   };
-  const int q0 = (qb * p.iters * 4 + wave) * 32 + (lane & 31);
+  const int q0 = (qb * p.iters * 4 + wave) * 32;
   fetch(q0);
-  stage_rows<T, HDP>(sK, Gm::SR, p.k + krow * p.ldk + g * hdb, p.ldk, 0, KT * 32, kn, mask, hdb, tid);
-  stage_rows<T, HDP>(sV, Gm::SR, p.v + krow * p.ldv + g * hdb, p.ldv, 0, KT * 32, kn, mask, hdb, tid);
+  stage_rows2<T, HDP>(sK, Gm::SR, p.k + krow * p.ldk + g * hdb, p.ldk, sV, Gm::SR, p.v + krow * p.ldv + g * hdb, p.ldv, 0,
+                      KT * 32, kn, mask, hdb, tid);
   stage_valid(bits, bias, 0, KT * 32, kn, mask, tid);
   __syncthreads();
-  uint32_t w[KT];
+  int tiles = 0;       // up to the last one with a valid key
 #pragma unroll
-  for (int t = 0; t < KT; ++t) w[t] = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
-  f32x16 dk[KT][Gm::DT], dv[KT][Gm::DT];
+  for (int t = 0; t < KT; ++t) tiles = __builtin_amdgcn_readfirstlane((int)bits[t]) ? t + 1 : tiles;
+  KvAcc<T, HDP> dk[KT], dv[KT];
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) { dk[t][d] = zero16(); dv[t][d] = zero16(); }
+  for (int t = 0; t < KT; ++t) { dk[t].clear(); dv[t].clear(); }
 
   for (int it = 0; it < p.iters; ++it) {
     const int q = q0 + it * 128;
-    if (q - (lane & 31) >= p.Nq) break;        // (wave-uniform)
+    if (q >= p.Nq) break;                      // (wave-uniform)
     // a query past the end, and one without a finite score, has no probabilities
-    const float lse2 = L2 == -INFINITY ? INFINITY : L2 * CR_LOG2E;
+    const float lse2 = L2 == -INFINITY || q + (lane & 31) >= p.Nq ? INFINITY : L2 * CR_LOG2E;
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc) {
       *reinterpret_cast<frag*>(sQ + (lane & 31) * Gm::ST + kc * 32 + half * 16) = qf[kc];
       *reinterpret_cast<frag*>(sD + (lane & 31) * Gm::ST + kc * 32 + half * 16) = df[kc];
     }
-    f32x16 pr[KT], dp[KT];
-    uint32_t keep[KT];
-    float delta = 0.f;
-    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q)) : 0u;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      if (w[t] == 0) continue;
-      f32x16 s = score_init(bias + t * 32, half), e = zero16();
-#pragma unroll
-      for (int kc = 0; kc < Gm::NC; ++kc) {
-        s = Cr<T>::mma(row_frag<T>(sK + t * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s);
-        e = Cr<T>::mma(row_frag<T>(sV + t * 32 * Gm::SR, Gm::SR, kc, lane), df[kc], e);
-      }
-      if (DROP) {
-        keep[t] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const uint32_t z = dm_drop_bits(rs, (uint32_t)(t * 32 + tile_row(i, half)) >> 1);
-          const bool k0 = dm_keep16(z, 0, p.thresh), k1 = dm_keep16(z, 1, p.thresh);
-          keep[t] |= (k0 ? 1u : 0u) << i | (k1 ? 2u : 0u) << i;
-          e[i] = k0 ? e[i] * p.inv_keep : 0.f;
-          e[i + 1] = k1 ? e[i + 1] * p.inv_keep : 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
-        delta = __builtin_fmaf(s[i], e[i], delta);
-      }
-      pr[t] = s;
-      dp[t] = e;
-    }
-    delta = half_sum(delta);
-    if (it + 1 < p.iters) fetch(q + 128);      // the next tile's rows fly during the products below
-    wave_lds_order();
+    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q + (lane & 31))) : 0u;
     f32x16 dq[Gm::DT];
+    auto next = [&]() { if (it + 1 < p.iters) fetch(q + 128); };
+    wave_lds_order();
+#define DM_FEW(NT) \
+  few_step<T, HDP, KT, NT, DROP>(p, sK, sV, bias, sQ, sD, patch, qf, df, lse2, c, rs, dk, dv, dq, lane, next)
+    if (KT > 2 && tiles > 2) DM_FEW((KT > 2 ? 3 : 1));
+    else if (KT > 1 && tiles > 1) DM_FEW((KT > 1 ? 2 : 1));
+    else if (tiles > 0) DM_FEW(1);
+    else {
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) dq[d] = zero16();
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      if (w[t] == 0) continue;
-      f32x16 ds;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ds[i] = pr[t][i] * (dp[t][i] - delta);
-      if (DROP) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
-      }
-      put_tile<T>(sP, pr[t], lane);
-      put_tile<T>(sS, ds, lane);
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const frag sf = Cr<T>::pack(ds, f);
-#pragma unroll
-        for (int d = 0; d < Gm::DT; ++d) dq[d] = Cr<T>::mma(tr_frag<T, HDP>(sK + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, dq[d]);
-      }
-      wave_lds_order();
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const frag pf = tr_frag<T, 32>(sP, PS, f, 0, lane), sf = tr_frag<T, 32>(sS, PS, f, 0, lane);
-#pragma unroll
-        for (int d = 0; d < Gm::DT; ++d) {
-          dv[t][d] = Cr<T>::mma(tr_frag<T, HDP>(sD, Gm::ST, f, d, lane), pf, dv[t][d]);
-          dk[t][d] = Cr<T>::mma(tr_frag<T, HDP>(sQ, Gm::ST, f, d, lane), sf, dk[t][d]);
-        }
-      }
-      wave_lds_order();
+      for (int d = 0; d < Gm::DT; ++d) dq[d] = zero16();
     }
-    char* dst = p.dq + (tok + q) * p.lddq + h * hdb;
+#undef DM_FEW
+    const Rows dst = rows_of(p.dq + (tok + q) * p.lddq + h * hdb, p.lddq, p.Nq - q, hdb, lane);
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, p.hd, q < p.Nq, half);
+    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, hdb, lane);
   }
 
   // dK, dV of the four waves, added in wave order: [dk | dv][key][channel]
@@ -175,18 +255,12 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-        for (int i = 0; i < (HDP < 32 ? 2 : 4); ++i) {
-          float* a = sum + (t * 32 + (lane & 31)) * RS + d * 32 + 8 * i + 4 * half;
-          f32x4 x = {dk[t][d][4 * i], dk[t][d][4 * i + 1], dk[t][d][4 * i + 2], dk[t][d][4 * i + 3]};
-          f32x4 y = {dv[t][d][4 * i], dv[t][d][4 * i + 1], dv[t][d][4 * i + 2], dv[t][d][4 * i + 3]};
-          f32x4* px = reinterpret_cast<f32x4*>(a);
-          f32x4* py = reinterpret_cast<f32x4*>(a + KT * 32 * RS);
-          if (turn) { x += *px; y += *py; }
-          *px = x;
-          *py = y;
-        }
+      for (int which = 0; which < 2; ++which)
+        (which ? dv[t] : dk[t]).each(lane, [&](int key, int col, f32x4 v) {
+          f32x4* at = reinterpret_cast<f32x4*>(sum + ((which * KT + t) * 32 + key) * RS + col);
+          if (turn) v += *at;
+          *at = v;
+        });
   }
   __syncthreads();
   if (ctx < 0) return;
@@ -205,13 +279,14 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
 }
 
 // dk, dv of context c: the partials of every sample that uses it (in order), of the heads of the group and of the query
-// shares.  Eight lanes split the list of one result (4 channels) and join by a fixed tree.
-template <typename T>
+// shares.  SL lanes split the list of one result (4 channels) and join by a fixed tree: 8 for long lists, 1 for short ones.
+template <typename T, int SL>
 __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) {
-  const int lane = threadIdx.x & 63, slice = lane >> 3;
+  constexpr int RPW = 64 / SL;                             // results per wave
+  const int lane = threadIdx.x & 63, slice = lane / RPW;
   const int per = p.hd >> 2, HG = p.H / p.G, U = HG * p.nqb;
-  const long n = (long)p.Bc * p.G * 2 * p.Nk * per;       // results, context slowest
-  const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6), i = wave * 8 + (lane & 7);
+  const long n = (long)p.Bc * p.G * 2 * p.Nk * per;        // results, context slowest
+  const long i = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + lane % RPW;
   const long r = i < n ? i : n - 1;
   const long gw = r / per, kw = gw / p.Nk, cg = kw >> 1;
   const int col = (int)(r - gw * per) * 4, key = (int)(gw - kw * p.Nk), which = (int)(kw & 1);
@@ -219,8 +294,8 @@ __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) 
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   int m = 0;
   auto add = [&](int b) {
-    for (int u = (slice - m * U) & 7; u < U; u += 8) {
-      const long src = (((long)b * p.H + g * HG) * p.nqb + u) * 2 + which;      // (heads and shares are adjacent: hh * nqb + share)
+    for (int u = (slice - m * U) & (SL - 1); u < U; u += SL) {
+      const long src = (((long)b * p.H + g * HG) * p.nqb + u) * 2 + which;      // (a head's shares are adjacent: hh * nqb + share)
       s += *reinterpret_cast<const f32x4*>(p.part + (src * p.Nk + key) * p.hd + col);
     }
     ++m;
@@ -232,10 +307,12 @@ __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) 
     for (int b = 0; b < p.B; ++b)
       if (p.index[b] == ctx) add(b);
   }
+  if (SL > 1) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1) s[j] += __shfl_xor(s[j], o, 64);
+      for (int o = RPW; o < 64; o <<= 1) s[j] += __shfl_xor(s[j], o, 64);
+  }
   if (i >= n || slice) return;
   const float f = which ? 1.f : p.scale;
   const long krow = (long)ctx * p.Nk + key;
@@ -259,9 +336,12 @@ int launch(const CrossParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   if (p.nsplit) {
-    const long n = (long)p.Bc * p.G * 2 * p.Nk * (p.hd >> 2), gb = (n + 31) / 32;
+    const long n = (long)p.Bc * p.G * 2 * p.Nk * (p.hd >> 2);
+    const bool wide = (long)((p.B + p.Bc - 1) / p.Bc) * (p.H / p.G) * p.nqb > 4;
+    const long gb = (n + (wide ? 31 : 255)) / (wide ? 32 : 256);
     if (gb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((cross_gather_kernel<T>), dim3((unsigned)gb), dim3(256), 0, st, p);
+    if (wide) hipLaunchKernelGGL((cross_gather_kernel<T, 8>), dim3((unsigned)gb), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((cross_gather_kernel<T, 1>), dim3((unsigned)gb), dim3(256), 0, st, p);
     DM_LAUNCH_CHECK();
   }
   return DM_OK;

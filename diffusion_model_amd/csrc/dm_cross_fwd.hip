@@ -86,44 +86,45 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
 }
 
 template <typename T, int HDP>
-__device__ __forceinline__ void fwd_finish(const CrossParams& p, const FwdState<T, HDP>& st, int b, int h, int q, int split,
-                                           float c, int lane) {
+__device__ __forceinline__ void fwd_finish(const CrossParams& p, const FwdState<T, HDP>& st, int b, int h, int q0, int split,
+                                           float c, int lane) {      // q0: the wave's first query (uniform)
   typedef Geo<T, HDP> Gm;
-  const int half = lane >> 5;
+  const int q = q0 + (lane & 31);
   const float l = half_sum(st.l);
   const float mc = st.m == -INFINITY ? 0.f : st.m * c;
-  const bool ok = q < p.Nq;
-  const long row = ((long)b * p.H + h) * p.Nq + q;
+  const bool mine = q < p.Nq && lane < 32;
+  const long row = ((long)b * p.H + h) * p.Nq + q0;
   if (p.nsplit > 1) {
     const long rows = (long)p.B * p.H * p.Nq;
-    char* o = (char*)(p.part + (split * rows + row) * p.hd);
+    const Rows o = rows_of((char*)(p.part + (split * rows + row) * p.hd), p.hd * 4, p.Nq - q0, p.hd * 4, lane);
 #pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) store_tile<float>(o, st.acc[d], 1.f, d * 32, p.hd, ok, half);
-    if (ok && half == 0) {
-      float* ml = p.part + p.nsplit * rows * p.hd + (split * rows + row) * 2;
+    for (int d = 0; d < Gm::DT; ++d) store_tile<float>(o, st.acc[d], 1.f, d * 32, p.hd * 4, lane);
+    if (mine) {
+      float* ml = p.part + p.nsplit * rows * p.hd + (split * rows + row + lane) * 2;
       ml[0] = mc;
       ml[1] = l;
     }
     return;
   }
   const float inv = l == 0.f ? 0.f : p.inv_keep * __builtin_amdgcn_rcpf(l);      // (v_rcp_f32: 1 ulp)
-  char* o = p.o + ((long)b * p.Nq + q) * p.ldo + h * p.hd * (long)sizeof(T);
+  const int hdb = p.hd * (int)sizeof(T);
+  const Rows o = rows_of(p.o + ((long)b * p.Nq + q0) * p.ldo + h * hdb, p.ldo, p.Nq - q0, hdb, lane);
 #pragma unroll
-  for (int d = 0; d < Gm::DT; ++d) store_tile<T>(o, st.acc[d], inv, d * 32, p.hd, ok, half);
-  if (ok && half == 0) p.lse[row] = l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * CR_LN2;
+  for (int d = 0; d < Gm::DT; ++d) store_tile<T>(o, st.acc[d], inv, d * 32, hdb, lane);
+  if (mine) p.lse[row + lane] = l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * CR_LN2;
 }
 
 // A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
 // LDS image, which is staged once for all the tiles; otherwise images of p.kb keys follow each other (iters is 1).
 template <typename T, int HDP, bool RES, bool DROP>
-__global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cross_fwd_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
   char* sV = sK + p.kb * Gm::SR;
   float* bias = reinterpret_cast<float*>(sV + p.kb * Gm::ST);
   uint32_t* bits = reinterpret_cast<uint32_t*>(bias + p.kb);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
   id /= p.H;
@@ -144,14 +145,15 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) 
   FwdState<T, HDP> st;
   typename Cr<T>::frag qf[Gm::NC], nf[Gm::NC];
   uint32_t rs = 0;
-  const char* qrow = p.q + ((long)b * p.Nq + qb * p.iters * 128 + wave * 32 + (lane & 31)) * p.ldq + h * hdb;
   constexpr bool AHEAD = Gm::NC <= 4;          // (wider rows would not fit the registers twice)
-  auto fetch = [&](int q) { load_frags<T, HDP>(qrow, q < p.Nq, hdb, lane, nf); };
+  auto fetch = [&](int q) {                    // q: the wave's first query
+    load_frags<T, HDP>(rows_of(p.q + ((long)b * p.Nq + q) * p.ldq + h * hdb, p.ldq, p.Nq - q, hdb, lane), hdb, lane, nf);
+  };
   auto begin = [&](int q) {
     if (!AHEAD) fetch(q);
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc) qf[kc] = nf[kc];
-    if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q));
+    if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q + (lane & 31)));
   };
   auto clear = [&]() {
     st.m = -INFINITY;
@@ -160,13 +162,12 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) 
     for (int d = 0; d < Gm::DT; ++d) st.acc[d] = zero16();
   };
   auto stage = [&](int from, int n) {
-    stage_rows<T, HDP>(sK, Gm::SR, kbase, p.ldk, from, n, k1, mask, hdb, tid);
-    stage_rows<T, HDP>(sV, Gm::ST, vbase, p.ldv, from, n, k1, mask, hdb, tid);
+    stage_rows2<T, HDP>(sK, Gm::SR, kbase, p.ldk, sV, Gm::ST, vbase, p.ldv, from, n, k1, mask, hdb, tid);
     stage_valid(bits, bias, from, n, k1, mask, tid);
   };
 #define DM_STEP(NT, FIRST, t, from) \
   fwd_step<T, HDP, NT, FIRST, DROP>(p, st, sK, sV, bits, bias, t, (from) + (t) * 32, c, qf, rs, lane)
-  const int q0 = qb * p.iters * 128 + wave * 32 + (lane & 31);
+  const int q0 = qb * p.iters * 128 + wave * 32;
   if (AHEAD) fetch(q0);
   if (RES) {
     const int n = max(0, (k1 - k0 + 31) & ~31), tiles = n >> 5;
@@ -174,12 +175,9 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossParams p) 
     __syncthreads();
     for (int it = 0; it < p.iters; ++it) {
       const int q = q0 + it * 128;
-      if (q - (lane & 31) >= p.Nq) break;      // (wave-uniform)
+      if (q >= p.Nq) break;                    // (wave-uniform)
       begin(q);
-      if (it + 1 < p.iters) {                  // the next tile's queries fly while this one is computed
-        qrow += 128 * p.ldq;
-        if (AHEAD) fetch(q + 128);
-      }
+      if (AHEAD && it + 1 < p.iters) fetch(q + 128);      // the next tile's queries fly while this one is computed
       int t = 2;
       if (tiles == 0) clear();
       else if (tiles == 1) DM_STEP(1, true, 0, k0);
