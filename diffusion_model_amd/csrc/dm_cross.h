@@ -144,45 +144,71 @@ __device__ __forceinline__ void load_frags(const Rows& x, int hdb, int lane, typ
     f[kc] = __builtin_bit_cast(typename Cr<T>::frag, __builtin_amdgcn_raw_buffer_load_b128(x.r, off < hdb ? (int)(x.at + off) : 0x7FFFFFFF, 0, 0));
   }
 }
-// Rows [r0, r0 + n) of two tensors of one shape -> LDS rows 0..n-1; rows from `valid` on or masked out, and the padding of
-// a head, become zero.  Every thread asks for eight pieces before it waits for the first: addresses are clamped to rows
-// that exist and the surplus is zeroed afterwards, since a branch around each load would wait for each in turn (B=16, 8 heads
-// of 128, 1024 queries on 512 keys, forward: 92 us that way).
+// Rows of two tensors of one shape (keys and values, queries and their gradients) on their way into LDS, N rows at a time:
+// load() asks for all of a thread's pieces, store() puts them down, so the next rows fly while the present ones are used.
+// Loads go through buffer descriptors, one address register per thread: rows from `valid` on and the padding of a head read
+// as zero, without a clamp, a select or a branch (a branch around each load would wait for each in turn: B=16, 8 heads of
+// 128, 1024 queries on 512 keys, forward: 92 us that way, 49 with clamped addresses).  Masked rows are zeroed on the way.
+template <typename T, int HDP, int N> struct Stager {
+  static constexpr int PPR = Geo<T, HDP>::PPR, RPS = 256 / PPR;            // pieces per row, rows per step of the workgroup
+  static constexpr int U = (N + RPS - 1) / RPS;
+  u32x4 a[U], b[U];
+  uint32_t ok;
+  __device__ __forceinline__ void load(const char* srcA, long ldA, const char* srcB, long ldB, int r0, int valid,
+                                       const unsigned char* mask, int hdb, int tid) {
+    const int r = tid / PPR, pc = tid % PPR, left = min(valid - r0, N);
+    const bool mine = r < RPS && pc * 16 < hdb;
+    // a descriptor covers one step of RPS rows and ends with the tensor; rows too far apart for its 32-bit range take the
+    // plain loads
+    if ((long)RPS * ldA < 0x7FFFFFFFL && (long)RPS * ldB < 0x7FFFFFFFL) {
+      const int va = mine ? (int)(r * ldA) + pc * 16 : 0x7FFFFFFF, vb = mine ? (int)(r * ldB) + pc * 16 : 0x7FFFFFFF;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int rows = min(left - u * RPS, RPS);
+        const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(srcA + (long)(r0 + u * RPS) * ldA), 0, rows > 0 ? (int)((rows - 1) * ldA) + hdb : 0, 0x00020000);
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(srcB + (long)(r0 + u * RPS) * ldB), 0, rows > 0 ? (int)((rows - 1) * ldB) + hdb : 0, 0x00020000);
+        a[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, va, 0, 0));
+        b[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, vb, 0, 0));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = mine && r + u * RPS < left;
+        a[u] = in ? *reinterpret_cast<const u32x4*>(srcA + (r0 + r + u * RPS) * ldA + pc * 16) : u32x4{0u, 0u, 0u, 0u};
+        b[u] = in ? *reinterpret_cast<const u32x4*>(srcB + (r0 + r + u * RPS) * ldB + pc * 16) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    ok = 0xFFFFFFFFu;
+    if (mask) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = r0 + u * RPS + r;
+        ok = row < valid && mask[row] ? ok : ok & ~(1u << u);
+      }
+    }
+  }
+  // n <= N: rows that the image has room for
+  __device__ __forceinline__ void store(char* dstA, int strideA, char* dstB, int strideB, int n, bool masked, int tid) {
+    const int r = tid / PPR, pc = tid % PPR;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (masked && !(ok >> u & 1u)) { a[u] = u32x4{0u, 0u, 0u, 0u}; b[u] = a[u]; }
+      if (r >= RPS || r + u * RPS >= n) break;
+      *reinterpret_cast<u32x4*>(dstA + (r + u * RPS) * strideA + pc * 16) = a[u];
+      *reinterpret_cast<u32x4*>(dstB + (r + u * RPS) * strideB + pc * 16) = b[u];
+    }
+  }
+};
+// rows [r0, r0 + n) of a resident image
 template <typename T, int HDP>
 __device__ __forceinline__ void stage_rows2(char* dstA, int strideA, const char* srcA, long ldA, char* dstB, int strideB,
                                             const char* srcB, long ldB, int r0, int n, int valid, const unsigned char* mask,
                                             int hdb, int tid) {
-  constexpr int PPR = Geo<T, HDP>::PPR, U = 4;
-  const int total = n * PPR, last = valid - 1, lastpc = (hdb >> 4) - 1;
-  if (r0 > last) {
-    for (int i = tid; i < total; i += 256) {
-      const int r = i / PPR, pc = i % PPR;
-      *reinterpret_cast<u32x4*>(dstA + r * strideA + pc * 16) = u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(dstB + r * strideB + pc * 16) = u32x4{0u, 0u, 0u, 0u};
-    }
-    return;
-  }
-  for (int base = tid; base < total; base += 256 * U) {
-    u32x4 a[U], b[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + 256 * u, r = i / PPR, pc = i % PPR, row = min(r0 + r, last), piece = min(pc, lastpc);
-      a[u] = *reinterpret_cast<const u32x4*>(srcA + row * ldA + piece * 16);
-      b[u] = *reinterpret_cast<const u32x4*>(srcB + row * ldB + piece * 16);
-      ok[u] = r0 + r <= last && pc <= lastpc;
-    }
-    if (mask) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) ok[u] = ok[u] && mask[min(r0 + (base + 256 * u) / PPR, last)] != 0;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + 256 * u, r = i / PPR, pc = i % PPR;
-      if (i >= total) break;
-      *reinterpret_cast<u32x4*>(dstA + r * strideA + pc * 16) = ok[u] ? a[u] : u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(dstB + r * strideB + pc * 16) = ok[u] ? b[u] : u32x4{0u, 0u, 0u, 0u};
-    }
+  constexpr int N = Geo<T, HDP>::RB >= 512 ? 64 : 128;      // (at most 16 pieces in flight per thread)
+  for (int at = 0; at < n; at += N) {
+    Stager<T, HDP, N> st;
+    st.load(srcA, ldA, srcB, ldB, r0 + at, valid, mask, hdb, tid);
+    st.store(dstA + at * strideA, strideA, dstB + at * strideB, strideB, min(N, n - at), mask != nullptr, tid);
   }
 }
 // Validity of keys [r0, r0 + n): one word per 32 keys (empty tiles are skipped) and, per key, what its score starts from:

@@ -11,8 +11,11 @@ namespace {
 using namespace dm_cross;
 
 // ---------------------------------------------------------------- dQ (and delta)
+// as the forward: resident keys, or two images of 64 keys in turn
+template <typename T, int HDP> constexpr int image_bytes() { return 64 * (2 * Geo<T, HDP>::SR + 4) + 16; }
+
 template <typename T, int HDP, bool RES, bool DROP>
-__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cross_dq_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cross_dq_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -113,13 +116,32 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cro
       finish(q);
     }
   } else {
+    Stager<T, HDP, 64> next;
+    auto load = [&](int from) { next.load(kbase, p.ldk, vbase, p.ldv, from, kn, mask, hdb, tid); };
+    auto store = [&](int from) {
+      next.store(sK, Gm::SR, sV, Gm::SR, 64, mask != nullptr, tid);
+      stage_valid(bits, bias, from, 64, kn, mask, tid);
+    };
+    char* const image = smem;
+    auto use = [&](int i) {
+      sK = image + (i & 1) * image_bytes<T, HDP>();
+      sV = sK + 64 * Gm::SR;
+      bias = reinterpret_cast<float*>(sV + 64 * Gm::SR);
+      bits = reinterpret_cast<uint32_t*>(bias + 64);
+    };
+    if (kn > 0) load(0);
     begin(q0);
-    for (int from = 0; from < kn; from += p.kb) {
-      const int n = min(p.kb, (kn - from + 31) & ~31);
+    use(0);
+    if (kn > 0) store(0);
+    __syncthreads();
+    for (int from = 0, i = 0; from < kn; from += 64, ++i) {
+      const bool more = from + 64 < kn;
+      if (more) load(from + 64);
+      use(i);
+      sweep(from, 2);
+      use(i + 1);
+      if (more) store(from + 64);
       __syncthreads();
-      stage(from, n);
-      __syncthreads();
-      sweep(from, n >> 5);
     }
     finish(q0);
   }
@@ -132,16 +154,53 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cro
 // them in order: no atomics, the same inputs give the same bits.
 constexpr int QS = 64;
 
+// one image: 64 queries, their output gradients, and per query the log-sum-exp (base 2), delta and the dropout word
+template <typename T, int HDP> constexpr int list_bytes() { return QS * (2 * Geo<T, HDP>::SR + 12); }
+
+// walks the share's blocks of 64 queries: every next() is wave- and workgroup-uniform
+struct QueryList {
+  int b0, b;                  // next sample to look at (a scan position in the index), the present one
+  unsigned long long hit;     // samples of the scanned 64 that use the context
+  uint32_t u, per;            // block of the present sample; blocks per sample
+  int ctx;
+  bool done;
+  __device__ __forceinline__ bool sample(const CrossParams& p, int lane) {
+    if (!p.index) {
+      if (p.Bc != 1) { b = ctx; done = b0 > 0; b0 = 1; }
+      else { b = b0++; done = b >= p.B; }
+      return !done;
+    }
+    while (!hit) {
+      if (b0 >= p.B) { done = true; return false; }
+      hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
+      b0 += 64;
+    }
+    b = b0 - 64 + __builtin_ctzll(hit);
+    hit &= hit - 1;
+    return true;
+  }
+  __device__ __forceinline__ void settle(const CrossParams& p, int lane) {
+    while (!done && u >= per) {
+      u -= per;
+      sample(p, lane);
+    }
+  }
+  __device__ __forceinline__ void start(const CrossParams& p, int c, uint32_t blocks, int share, int lane) {
+    ctx = c; per = blocks; u = (uint32_t)share; b0 = 0; b = 0; hit = 0; done = false;
+    sample(p, lane);
+    settle(p, lane);
+  }
+  __device__ __forceinline__ void next(const CrossParams& p, int lane) {
+    u += p.nsplit;
+    settle(p, lane);
+  }
+};
+
 template <typename T, int HDP, bool DROP>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && HDP > 64) ? 1 : 2) void cross_dkv_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, HDP * (int)sizeof(T) < 192 ? 2 : 1) void cross_dkv_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char* sQ = smem;
-  char* sD = sQ + QS * Gm::SR;
-  float* sL = reinterpret_cast<float*>(sD + QS * Gm::SR);
-  float* sDelta = sL + QS;
-  uint32_t* sRow = reinterpret_cast<uint32_t*>(sDelta + QS);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int nkb = (p.Nk + 127) / 128;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -162,32 +221,47 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && HDP > 64) ? 1 : 2) void cro
   load_frags<T, HDP>(p.v + krow * p.ldv + g * hdb, valid, hdb, lane, vf);
   f32x16 dk[Gm::DT], dv[Gm::DT];
 #pragma unroll
-  for (int d = 0; d < Gm::DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
+  for (int d = 0; d < Gm::DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
 
   const int nqc = (p.Nq + QS - 1) / QS;
-  const uint32_t per = (uint32_t)HG * nqc;       // blocks of 64 queries per sample
-  auto block_of = [&](int b, int hh, int qc) {
-    const int h = g * HG + hh, r0 = qc * QS;
-    const long tok = (long)b * p.Nq, row = ((long)b * p.H + h) * p.Nq;
-    __syncthreads();
-    stage_rows2<T, HDP>(sQ, Gm::SR, p.q + tok * p.ldq + h * hdb, p.ldq, sD, Gm::SR, p.d_o + tok * p.lddo + h * hdb, p.lddo,
-                        r0, QS, p.Nq, nullptr, hdb, tid);
+  Stager<T, HDP, QS> next;
+  float nl = 0.f, nd = 0.f;
+  uint32_t nrow = 0;
+  auto load = [&](const QueryList& at) {
+    const int h = g * HG + (int)(at.u / (uint32_t)nqc), r0 = (int)(at.u % (uint32_t)nqc) * QS;
+    const long tok = (long)at.b * p.Nq, row = ((long)at.b * p.H + h) * p.Nq;
+    next.load(p.q + tok * p.ldq + h * hdb, p.ldq, p.d_o + tok * p.lddo + h * hdb, p.lddo, r0, p.Nq, nullptr, hdb, tid);
     if (tid < QS) {
-      const int q = r0 + tid;
-      const float l = q < p.Nq ? p.lse[row + q] * CR_LOG2E : INFINITY;
-      sL[tid] = l == -INFINITY ? INFINITY : l;      // no probability for queries past the end
-      sDelta[tid] = q < p.Nq ? p.delta[row + q] : 0.f;
-      if (DROP) sRow[tid] = dm_drop_row(seed, (uint32_t)(row + q));
+      const int q = min(r0 + tid, p.Nq - 1);
+      const float l = p.lse[row + q] * CR_LOG2E;
+      nl = r0 + tid >= p.Nq || l == -INFINITY ? INFINITY : l;      // no probability for queries past the end
+      nd = r0 + tid < p.Nq ? p.delta[row + q] : 0.f;
+      nrow = (uint32_t)(row + q);
     }
-    __syncthreads();
+  };
+  char *sQ, *sD;
+  float *sL, *sDelta;
+  uint32_t* sRow;
+  auto use = [&](int i) {
+    sQ = smem + (i & 1) * list_bytes<T, HDP>();
+    sD = sQ + QS * Gm::SR;
+    sL = reinterpret_cast<float*>(sD + QS * Gm::SR);
+    sDelta = sL + QS;
+    sRow = reinterpret_cast<uint32_t*>(sDelta + QS);
+  };
+  auto store = [&]() {
+    next.store(sQ, Gm::SR, sD, Gm::SR, QS, false, tid);
+    if (tid < QS) {
+      sL[tid] = nl;
+      sDelta[tid] = nd;
+      if (DROP) sRow[tid] = dm_drop_row(seed, nrow);
+    }
+  };
+  auto block = [&](int rows) {
     if (!active) return;
     for (int t = 0; t < QS / 32; ++t) {
-      if (r0 + t * 32 >= p.Nq) break;
-      f32x16 s, dp;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+      if (t * 32 >= rows) break;
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int kc = 0; kc < Gm::NC; ++kc) {
         s = Cr<T>::mma(row_frag<T>(sQ + t * 32 * Gm::SR, Gm::SR, kc, lane), kf[kc], s);
@@ -218,26 +292,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && HDP > 64) ? 1 : 2) void cro
       }
     }
   };
-  // the samples that use this context, in order; the j-th one's blocks are numbered from j * per
-  uint32_t phase = (uint32_t)split;          // first block of the next sample that is this share's
-  auto sample = [&](int b) {
-    uint32_t u = phase;
-    for (; u < per; u += p.nsplit) block_of(b, u / nqc, u % nqc);
-    phase = u - per;
-  };
   if (kblk * 128 < kn) {
-    if (!p.index) {
-      if (p.Bc == 1) for (int b = 0; b < p.B; ++b) sample(b);
-      else sample(ctx);
-    } else {
-      for (int b0 = 0; b0 < p.B; b0 += 64) {
-        unsigned long long hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
-        while (hit) {
-          const int b = b0 + __builtin_ctzll(hit);
-          hit &= hit - 1;
-          sample(b);
-        }
-      }
+    QueryList at;
+    at.start(p, ctx, (uint32_t)HG * nqc, split, lane);
+    if (!at.done) {
+      load(at);
+      use(0);
+      store();
+    }
+    __syncthreads();
+    for (int i = 0; !at.done; ++i) {
+      const int rows = p.Nq - (int)(at.u % (uint32_t)nqc) * QS;
+      at.next(p, lane);
+      if (!at.done) load(at);          // the next block's rows fly while this one is used
+      use(i);
+      block(rows);
+      use(i + 1);
+      if (!at.done) store();
+      __syncthreads();
     }
   }
   if (key >= p.Nk) return;
@@ -303,10 +375,10 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   const int image = (LDS_IMAGE - 64) / (2 * row_bytes(a) + 5) / 64 * 64;
   const int need = (a->Nk + 63) & ~63;
   f.res = need <= image;
-  f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
+  f.kb = need > 0 ? need : 64;
   f.iters = 1;
   if (f.res) {
-    long it = blocks / 1536;
+    long it = blocks / 512;
     if (it > 8) it = 8;
     if (it > groups) it = groups;
     f.iters = it < 1 ? 1 : (int)it;
@@ -314,10 +386,10 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   f.nqb = (int)((groups + f.iters - 1) / f.iters);
   f.iters = (int)((groups + f.nqb - 1) / f.nqb);
   f.delta_bytes = (((long)a->B * a->heads * a->Nq + 3) & ~3L) * 4;
-  // shares of a context's query list: enough workgroups for four per CU, at least four blocks of queries each
+  // shares of a context's query list: two workgroups per CU, at least four blocks of queries each
   const long owners = (long)a->Bc * a->kv_heads * ((a->Nk + 127) / 128);
   const long list = (long)((a->B + a->Bc - 1) / a->Bc) * (a->heads / a->kv_heads) * ((a->Nq + QS - 1) / QS);
-  long ns = owners > 0 ? 1024 / owners : 1;
+  long ns = owners > 0 ? 512 / owners : 1;
   if (ns > list / 4) ns = list / 4;
   f.nsplit = ns < 1 ? 1 : (int)ns;
   f.ws = f.delta_bytes + (f.nsplit > 1 ? (long)f.nsplit * 2 * a->Bc * a->Nk * a->kv_heads * a->hd * 4 : 0);
@@ -329,9 +401,10 @@ int launch_dq(const CrossParams& p, hipStream_t st) {
   auto kern = cross_dq_kernel<T, HDP, RES, DROP>;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
-      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          RES ? LDS_IMAGE : 2 * image_bytes<T, HDP>()) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4;
+  const size_t lds = RES ? (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
   const long blocks = (long)p.B * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
@@ -341,7 +414,7 @@ int launch_dq(const CrossParams& p, hipStream_t st) {
 template <typename T, int HDP, bool DROP>
 int launch_dkv(const CrossParams& p, hipStream_t st) {
   auto kern = cross_dkv_kernel<T, HDP, DROP>;
-  const int lds = QS * 2 * Geo<T, HDP>::SR + QS * 12;
+  const int lds = 2 * list_bytes<T, HDP>();
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)

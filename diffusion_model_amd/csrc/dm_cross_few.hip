@@ -147,7 +147,7 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
 #pragma unroll
       for (int d = 0; d < Gm::DT; ++d)
         dq[d] = Cr<T>::mma(tr_frag<T, HDP>(sK + t * 32 * Gm::SR, Gm::SR, f, d, lane), sf, t == 0 && f == 0 ? zero16() : dq[d]);
-      if (KT > 1) __builtin_amdgcn_sched_barrier(0);
+      if (KT > 1 && HDP > 16) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
   for (int t0 = 0; t0 < NT; t0 += PT) {
@@ -164,7 +164,7 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
         dv[t].add(sD, patch + 2 * (t - t0) * 32 * PS, f, lane);
         dk[t].add(sQ, patch + (2 * (t - t0) + 1) * 32 * PS, f, lane);
       }
-      if (KT > 1) __builtin_amdgcn_sched_barrier(0);      // (all operand reads at once would not fit the registers)
+      if (KT > 1 && HDP > 16) __builtin_amdgcn_sched_barrier(0);      // (all operand reads at once would not fit the registers)
     }
     wave_lds_order();
   }
@@ -365,7 +365,11 @@ bool few_plan(const dm_cross_args* a, FewPlan& f) {
   if (a->Nk < 1 || a->Nk > 32 * most || (a->dtype != 0 && hdp > 64)) return false;
   f.kt = a->Nk <= 32 ? 1 : most;
   const long pairs = (long)a->B * a->heads, groups = ((long)a->Nq + 127) / 128;      // one tile per wave of a workgroup
-  long nqb = (1024 + pairs - 1) / pairs;                   // about four waves per SIMD over the device
+  // one round of workgroups over the device: a second one would stage the keys and add up dK / dV again (B=64, 8 heads of 16,
+  // 2304 queries, 77 tokens: 80 us at one round, 84 at two, 91 at four; fp32, 64 pairs of 576 queries: 41 at one, 49 at two)
+  const int cap = 256 * (hdp * f.kt <= (a->dtype == 0 ? 64 : 32) ? 2 : 1);
+  long nqb = cap / pairs;
+  if (nqb < 1) nqb = 1;
   if (nqb > groups) nqb = groups;
   f.iters = (int)((groups + nqb - 1) / nqb);
   f.nqb = (int)((groups + f.iters - 1) / f.iters);

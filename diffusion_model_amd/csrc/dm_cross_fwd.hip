@@ -114,10 +114,13 @@ __device__ __forceinline__ void fwd_finish(const CrossParams& p, const FwdState<
   if (mine) p.lse[row + lane] = l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * CR_LN2;
 }
 
+// one image of the streamed kernel: 64 keys, values, starts and validity words
+template <typename T, int HDP> constexpr int image_bytes() { return 64 * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + 16; }
+
 // A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
-// LDS image, which is staged once for all the tiles; otherwise images of p.kb keys follow each other (iters is 1).
+// LDS image, which is staged once for all the tiles; otherwise two images of 64 keys take turns (iters is 1).
 template <typename T, int HDP, bool RES, bool DROP>
-__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cross_fwd_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cross_fwd_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cro
     load_frags<T, HDP>(rows_of(p.q + ((long)b * p.Nq + q) * p.ldq + h * hdb, p.ldq, p.Nq - q, hdb, lane), hdb, lane, nf);
   };
   auto begin = [&](int q) {
-    if (!AHEAD) fetch(q);
+    if (!AHEAD && RES) fetch(q);
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc) qf[kc] = nf[kc];
     if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q + (lane & 31)));
@@ -191,16 +194,35 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 512 ? 2 : 1)) void cro
       fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
     }
   } else {
+    // two images of 64 keys in turn: the next one's rows fly while the present one is used
+    Stager<T, HDP, 64> next;
+    auto load = [&](int from) { next.load(kbase, p.ldk, vbase, p.ldv, from, k1, mask, hdb, tid); };
+    auto store = [&](int from) {
+      next.store(sK, Gm::SR, sV, Gm::ST, 64, mask != nullptr, tid);
+      stage_valid(bits, bias, from, 64, k1, mask, tid);
+    };
+    char* const image = smem;
+    auto use = [&](int i) {
+      sK = image + (i & 1) * image_bytes<T, HDP>();
+      sV = sK + 64 * Gm::SR;
+      bias = reinterpret_cast<float*>(sV + 64 * Gm::ST);
+      bits = reinterpret_cast<uint32_t*>(bias + 64);
+    };
+    if (k0 < k1) load(k0);
+    if (!AHEAD) fetch(q0);
     begin(q0);
     clear();
-    for (int from = k0; from < k1; from += p.kb) {
-      const int n = min(p.kb, (k1 - from + 31) & ~31), tiles = n >> 5;
+    use(0);
+    if (k0 < k1) store(k0);
+    __syncthreads();
+    for (int from = k0, i = 0; from < k1; from += 64, ++i) {
+      const bool more = from + 64 < k1;
+      if (more) load(from + 64);
+      use(i);
+      DM_STEP(2, false, 0, from);
+      use(i + 1);
+      if (more) store(from + 64);
       __syncthreads();
-      stage(from, n);
-      __syncthreads();
-      int t = 0;
-      for (; t + 2 <= tiles; t += 2) DM_STEP(2, false, t, from);
-      if (t < tiles) DM_STEP(1, false, t, from);
     }
     fwd_finish<T, HDP>(p, st, b, h, q0, split, c, lane);
   }
@@ -265,11 +287,12 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   const int image = (LDS_IMAGE - 64) / (kbytes + 5) / 64 * 64;     // keys per LDS image
   const int need = (f.ksplit + 63) & ~63;
   f.res = need <= image;
-  f.kb = f.res ? (need > 0 ? need : 64) : (image > 128 ? 128 : image);
-  // resident keys serve several query tiles per wave, as long as there are about six workgroups per CU
+  f.kb = need > 0 ? need : 64;
+  // resident keys serve several query tiles per wave, as long as there are two workgroups per CU (B=64, 8 heads of 32, 576
+  // queries, 77 tokens: 13.5 us at two, 14.6 at six and more)
   f.iters = 1;
   if (f.res) {
-    long it = blocks * f.nsplit / 1536;
+    long it = blocks * f.nsplit / 512;
     if (it > 8) it = 8;
     if (it > groups) it = groups;
     f.iters = it < 1 ? 1 : (int)it;
@@ -285,9 +308,10 @@ int launch_fwd(const CrossParams& p, hipStream_t st) {
   auto kern = cross_fwd_kernel<T, HDP, RES, DROP>;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
-      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_IMAGE) != hipSuccess)
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          RES ? LDS_IMAGE : 2 * image_bytes<T, HDP>()) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4;
+  const size_t lds = RES ? (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
   const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, RES ? "resident" : "streamed");
