@@ -352,8 +352,15 @@ inline int cross_fill(CrossParams& p, const dm_cross_args* a, bool bwd) {
 }
 
 // ---------------------------------------------------------------- the one-kernel backward of few keys (dm_cross_few.hip)
-struct FewPlan { int kt, iters, nqb; bool direct; long ws; };
+struct FewPlan { int kt, iters, nqb; bool heads, direct; long ws; };
 bool few_plan(const dm_cross_args* a, FewPlan& f);          // false: these sizes take the two kernels of dm_cross_bwd.hip
 int few_launch(const CrossParams& p, const FewPlan& f, int dtype, hipStream_t st);
+
+// ---------------------------------------------------------------- the forward of single queries (dm_cross_one.hip)
+struct OnePlan { int nsplit, ksplit; long ws; };
+bool one_plan(const dm_cross_args* a, OnePlan& f);          // false: too many rows share a key / value head
+int one_launch(const CrossParams& p, int dtype, hipStream_t st);
+int join_launch(const CrossParams& p, int dtype, hipStream_t st);      // joins the key splits of either forward
+constexpr int MAX_SPLITS = 64;
 
 }  // namespace dm_cross

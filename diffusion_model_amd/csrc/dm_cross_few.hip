@@ -170,7 +170,8 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
   }
 }
 
-template <typename T, int HDP, int KT, bool DROP>
+// HEADS: a workgroup takes every query head of its key / value head (small calls), not a share of one head's queries.
+template <typename T, int HDP, int KT, bool DROP, bool HEADS>
 __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
@@ -183,28 +184,31 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
   char* sQ = reinterpret_cast<char*>(bits + 8) + wave * wave_lds<T, HDP, KT>();
   char* sD = sQ + 32 * Gm::ST;
   char* patch = sD + 32 * Gm::ST;
+  // a workgroup's units are tiles of 32 queries
+  const int HB = HEADS ? p.H / p.G : 1;
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int h = id % p.H;
-  id /= p.H;
+  const int h0 = (int)(id % (uint32_t)(p.H / HB)) * HB;
+  id /= (uint32_t)(p.H / HB);
   const int qb = id % p.nqb, b = id / p.nqb;
   const int ctx = context_of(p, b), kn = keys_of(p, ctx);
-  const int hdb = p.hd * (int)sizeof(T), g = h / (p.H / p.G);
+  const int hdb = p.hd * (int)sizeof(T), g = h0 / (p.H / p.G);
+  const int tiles_q = (p.Nq + 31) >> 5, units = HEADS ? HB * tiles_q : min(tiles_q, (qb + 1) * p.iters * 4);
   const long krow = (long)(ctx < 0 ? 0 : ctx) * p.Nk;
   const unsigned char* mask = p.mask ? p.mask + krow : nullptr;
   const float c = p.scale * CR_LOG2E;
   const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
-  const long tok = (long)b * p.Nq, row = ((long)b * p.H + h) * p.Nq;
+  const long tok = (long)b * p.Nq;
 
   frag qf[Gm::NC], df[Gm::NC];
   float L2;
-  auto fetch = [&](int q) {      // q: the wave's first query
-    const int left = p.Nq - q;
+  auto fetch = [&](int unit) {
+    const int hh = HEADS ? unit / tiles_q : 0, h = h0 + hh, q = (unit - hh * tiles_q) * 32, left = p.Nq - q;
     load_frags<T, HDP>(rows_of(p.q + (tok + q) * p.ldq + h * hdb, p.ldq, left, hdb, lane), hdb, lane, qf);
     load_frags<T, HDP>(rows_of(p.d_o + (tok + q) * p.lddo + h * hdb, p.lddo, left, hdb, lane), hdb, lane, df);
-    L2 = p.lse[row + min(q + (lane & 31), p.Nq - 1)];
+    L2 = p.lse[((long)b * p.H + h) * p.Nq + min(q + (lane & 31), p.Nq - 1)];
   };
-  const int q0 = (qb * p.iters * 4 + wave) * 32;
-  fetch(q0);
+  const int first = qb * p.iters * 4 + wave;
+  fetch(min(first, units - 1));
   stage_rows2<T, HDP>(sK, Gm::SR, p.k + krow * p.ldk + g * hdb, p.ldk, sV, Gm::SR, p.v + krow * p.ldv + g * hdb, p.ldv, 0,
                       KT * 32, kn, mask, hdb, tid);
   stage_valid(bits, bias, 0, KT * 32, kn, mask, tid);
@@ -216,19 +220,19 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
 #pragma unroll
   for (int t = 0; t < KT; ++t) { dk[t].clear(); dv[t].clear(); }
 
-  for (int it = 0; it < p.iters; ++it) {
-    const int q = q0 + it * 128;
-    if (q >= p.Nq) break;                      // (wave-uniform)
+  for (int unit = first; unit < units; unit += 4) {
+    const int hh = HEADS ? unit / tiles_q : 0, hq = h0 + hh, q0 = (unit - hh * tiles_q) * 32;
+    const long row = ((long)b * p.H + hq) * p.Nq;
     // a query past the end, and one without a finite score, has no probabilities
-    const float lse2 = L2 == -INFINITY || q + (lane & 31) >= p.Nq ? INFINITY : L2 * CR_LOG2E;
+    const float lse2 = L2 == -INFINITY || q0 + (lane & 31) >= p.Nq ? INFINITY : L2 * CR_LOG2E;
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc) {
       *reinterpret_cast<frag*>(sQ + (lane & 31) * Gm::ST + kc * 32 + half * 16) = qf[kc];
       *reinterpret_cast<frag*>(sD + (lane & 31) * Gm::ST + kc * 32 + half * 16) = df[kc];
     }
-    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q + (lane & 31))) : 0u;
+    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q0 + (lane & 31))) : 0u;
     f32x16 dq[Gm::DT];
-    auto next = [&]() { if (it + 1 < p.iters) fetch(q + 128); };
+    auto next = [&]() { if (unit + 4 < units) fetch(unit + 4); };
     wave_lds_order();
 #define DM_FEW(NT) \
   few_step<T, HDP, KT, NT, DROP>(p, sK, sV, bias, sQ, sD, patch, qf, df, lse2, c, rs, dk, dv, dq, lane, next)
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
       for (int d = 0; d < Gm::DT; ++d) dq[d] = zero16();
     }
 #undef DM_FEW
-    const Rows dst = rows_of(p.dq + (tok + q) * p.lddq + h * hdb, p.lddq, p.Nq - q, hdb, lane);
+    const Rows dst = rows_of(p.dq + (tok + q0) * p.lddq + hq * hdb, p.lddq, p.Nq - q0, hdb, lane);
 #pragma unroll
     for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, hdb, lane);
   }
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
     const int which = i >= n, e = which ? i - n : i, key = e / per, col = (e - key * per) * 4;
     const f32x4 v = *reinterpret_cast<const f32x4*>(sum + (which * KT * 32 + key) * RS + col);
     if (p.nsplit) {
-      *reinterpret_cast<f32x4*>(p.part + ((((long)b * p.H + h) * p.nqb + qb) * 2 + which) * p.Nk * p.hd + (long)key * p.hd + col) = v;
+      *reinterpret_cast<f32x4*>(p.part + ((((long)b * p.H + h0) * p.nqb + qb) * 2 + which) * p.Nk * p.hd + (long)key * p.hd + col) = v;
     } else {
       const float f = which ? 1.f : p.scale;
       char* dst = which ? p.dv + (krow + key) * p.lddv : p.dk + (krow + key) * p.lddk;
@@ -320,16 +324,16 @@ __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) 
   store4<T>(dst + (g * p.hd + col) * (long)sizeof(T), s[0] * f, s[1] * f, s[2] * f, s[3] * f);
 }
 
-template <typename T, int HDP, int KT, bool DROP>
+template <typename T, int HDP, int KT, bool DROP, bool HEADS>
 int launch(const CrossParams& p, hipStream_t st) {
-  auto kern = cross_few_kernel<T, HDP, KT, DROP>;
+  auto kern = cross_few_kernel<T, HDP, KT, DROP, HEADS>;
   constexpr int lds = few_lds<T, HDP, KT>();
   static_assert(lds <= 160 * 1024, "LDS");
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const long blocks = (long)p.B * p.nqb * p.H;
+  const long blocks = (long)p.B * p.nqb * (HEADS ? p.G : p.H);
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_bwd_few<%s,%d,KT=%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, KT);
   dm_set_variant(nm.s);
@@ -348,10 +352,15 @@ int launch(const CrossParams& p, hipStream_t st) {
 }
 // tiles of 32 keys that a wave's registers hold beside the rest
 constexpr int most_tiles(int hdp, int esize) { return hdp <= 32 ? 3 : (esize == 2 && hdp == 64 ? 2 : 1); }
-template <typename T, int HDP> int pick(const CrossParams& p, int kt, hipStream_t st) {
-  if (kt == 1) return p.thresh ? launch<T, HDP, 1, true>(p, st) : launch<T, HDP, 1, false>(p, st);
+template <typename T, int HDP, int KT, bool HEADS> int pick_drop(const CrossParams& p, hipStream_t st) {
+  return p.thresh ? launch<T, HDP, KT, true, HEADS>(p, st) : launch<T, HDP, KT, false, HEADS>(p, st);
+}
+template <typename T, int HDP> int pick(const CrossParams& p, const FewPlan& f, hipStream_t st) {
+  if constexpr (HDP <= 32)
+    if (f.heads) return pick_drop<T, HDP, 1, true>(p, st);
+  if (f.kt == 1) return pick_drop<T, HDP, 1, false>(p, st);
   constexpr int KT = most_tiles(HDP, sizeof(T));
-  if constexpr (KT > 1) return p.thresh ? launch<T, HDP, KT, true>(p, st) : launch<T, HDP, KT, false>(p, st);
+  if constexpr (KT > 1) return pick_drop<T, HDP, KT, false>(p, st);
   return DM_ERR_ARG;
 }
 
@@ -373,7 +382,13 @@ bool few_plan(const dm_cross_args* a, FewPlan& f) {
   if (nqb > groups) nqb = groups;
   f.iters = (int)((groups + nqb - 1) / nqb);
   f.nqb = (int)((groups + f.iters - 1) / f.iters);
-  f.direct = f.nqb == 1 && a->heads == a->kv_heads && !a->index && a->Bc == a->B;
+  // a small call lets one workgroup take all the heads that share a key / value head: nothing is left to add up afterwards,
+  // which saves a launch
+  const int HG = a->heads / a->kv_heads;
+  const bool own = !a->index && a->Bc == a->B;
+  f.heads = own && hdp <= 32 && f.kt == 1 && HG > 1 && (long)HG * ((a->Nq + 31) / 32) <= 32;
+  if (f.heads) f.nqb = 1;
+  f.direct = own && f.nqb == 1 && (f.heads || HG == 1);
   f.ws = f.direct ? 0 : pairs * f.nqb * 2 * a->Nk * a->hd * 4;
   return f.ws <= (1L << 29);
 }
@@ -382,17 +397,17 @@ int few_launch(const CrossParams& p, const FewPlan& f, int dtype, hipStream_t st
   const int hdp = cross_hdp(p.hd);
   if (dtype == 0) {
     switch (hdp) {
-      case 16: return pick<bf16, 16>(p, f.kt, st);
-      case 32: return pick<bf16, 32>(p, f.kt, st);
-      case 64: return pick<bf16, 64>(p, f.kt, st);
-      case 96: return pick<bf16, 96>(p, f.kt, st);
-      default: return pick<bf16, 128>(p, f.kt, st);
+      case 16: return pick<bf16, 16>(p, f, st);
+      case 32: return pick<bf16, 32>(p, f, st);
+      case 64: return pick<bf16, 64>(p, f, st);
+      case 96: return pick<bf16, 96>(p, f, st);
+      default: return pick<bf16, 128>(p, f, st);
     }
   }
   switch (hdp) {
-    case 16: return pick<float, 16>(p, f.kt, st);
-    case 32: return pick<float, 32>(p, f.kt, st);
-    default: return pick<float, 64>(p, f.kt, st);
+    case 16: return pick<float, 16>(p, f, st);
+    case 32: return pick<float, 32>(p, f, st);
+    default: return pick<float, 64>(p, f, st);
   }
 }
 

@@ -229,37 +229,6 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
 #undef DM_STEP
 }
 
-// joins the key splits: thread = (row, 4 channels)
-template <typename T>
-__global__ __launch_bounds__(256) void cross_join_kernel(const CrossParams p) {
-  const long rows = (long)p.B * p.H * p.Nq;
-  const int per = p.hd >> 2;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * per) return;
-  const long row = i / per;
-  const int col = (int)(i - row * per) * 4;
-  const float* ml = p.part + p.nsplit * rows * p.hd + row * 2;
-  float m = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s)
-    if (ml[s * rows * 2 + 1] != 0.f) m = fmaxf(m, ml[s * rows * 2]);
-  float l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float ls = ml[s * rows * 2 + 1];
-    if (ls == 0.f) continue;
-    const float w = __builtin_amdgcn_exp2f(ml[s * rows * 2] - m);
-    l += w * ls;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * p.hd + col);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] += w * a[j];
-  }
-  const float inv = l == 0.f ? 0.f : p.inv_keep / l;
-  const long bh = row / p.Nq, q = row - bh * p.Nq, b = bh / p.H;
-  const int h = (int)(bh - b * p.H);
-  store4<T>(p.o + (b * p.Nq + q) * p.ldo + (h * p.hd + col) * (long)sizeof(T), o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (col == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * CR_LN2;
-}
-
 constexpr int LDS_IMAGE = 80 * 1024;     // two workgroups per CU
 
 int key_bytes(const dm_cross_args* a) {
@@ -280,6 +249,7 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   if (blocks < 512 && a->Nk >= 256) {
     ns = (1024 + blocks - 1) / blocks;
     if (ns > a->Nk / 128) ns = a->Nk / 128;
+    if (ns > MAX_SPLITS) ns = MAX_SPLITS;
   }
   f.ksplit = ns > 1 ? (int)((((long)a->Nk + ns - 1) / ns + 63) & ~63L) : a->Nk;
   f.nsplit = ns > 1 ? (a->Nk + f.ksplit - 1) / f.ksplit : 1;
@@ -318,13 +288,7 @@ int launch_fwd(const CrossParams& p, hipStream_t st) {
   dm_set_variant(nm.s);
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
-  if (p.nsplit > 1) {
-    const long n = (long)p.B * p.H * p.Nq * (p.hd >> 2), jb = (n + 255) / 256;
-    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((cross_join_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
-    DM_LAUNCH_CHECK();
-  }
-  return DM_OK;
+  return p.nsplit > 1 ? join_launch(p, sizeof(T) == 2 ? 0 : 1, st) : DM_OK;
 }
 template <typename T, int HDP> int pick_fwd(const CrossParams& p, bool res, hipStream_t st) {
   if (res) return p.thresh ? launch_fwd<T, HDP, true, true>(p, st) : launch_fwd<T, HDP, true, false>(p, st);
@@ -342,12 +306,24 @@ template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t
 
 }  // namespace
 
-extern "C" long dm_cross_fwd_workspace_bytes(const dm_cross_args* a) { return dm_cross::cross_sizes_ok(a) ? fwd_plan(a).ws : 0; }
+extern "C" long dm_cross_fwd_workspace_bytes(const dm_cross_args* a) {
+  if (!dm_cross::cross_sizes_ok(a)) return 0;
+  dm_cross::OnePlan one;
+  const long ws = fwd_plan(a).ws;                              // (with dropout single queries take the tiles, too)
+  return dm_cross::one_plan(a, one) && one.ws > ws ? one.ws : ws;
+}
 
 extern "C" int dm_cross_fwd(const dm_cross_args* a, dm_stream_t stream) {
   CrossParams p{};
   const int rc = cross_fill(p, a, false);
   if (rc != DM_OK) return rc;
+  OnePlan one;
+  if (p.thresh == 0 && one_plan(a, one)) {
+    DM_REQUIRE(one.ws == 0 || (a->workspace && a->ws_bytes >= one.ws && (uintptr_t)a->workspace % 16 == 0));
+    p.nsplit = one.nsplit; p.ksplit = one.ksplit;
+    p.part = (float*)a->workspace;
+    return one_launch(p, a->dtype, (hipStream_t)stream);
+  }
   const FwdPlan f = fwd_plan(a);
   DM_REQUIRE(f.ws == 0 || (a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0));
   p.nsplit = f.nsplit; p.ksplit = f.ksplit; p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb;

@@ -843,8 +843,18 @@ def _cross_check(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_
 
 
 def _rows16(what, name, t, esize):
-    """(address, row stride) of [.., .., C] rows that start on 16-byte boundaries."""
-    ld = t.shape[-1] if t.is_contiguous() else _act(t, name)
+    """(address, row stride) of [.., .., C] rows that start on 16-byte boundaries, samples densely packed."""
+    if t.is_contiguous():
+        ld = t.shape[-1]
+    else:
+        s0, ld, s2 = t.stride()
+        n0, n1, _ = t.shape
+        if n1 == 1:
+            ld = s0
+        elif n0 != 1 and s0 != ld * n1:
+            s2 = 0
+        if s2 != 1:
+            raise ValueError(f"{what}: unsupported strides {t.stride()} of {name} {tuple(t.shape)}")
     ptr = t.data_ptr()
     if (ptr | ld * esize) & 15:
         raise ValueError(f"{what}: the rows of {name} must be 16-byte aligned")

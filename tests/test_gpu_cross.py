@@ -173,6 +173,24 @@ def test_cross_forward_and_backward(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, 
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,H,G,hd,Nk,lens,mask,index", [
+    (1, 2, 2, 8, 5, None, False, False), (1, 2, 2, 24, 300, "ragged", True, False), (1, 3, 3, 40, 1, None, False, False),
+    (1, 4, 2, 64, 1500, "ragged", False, True), (2, 2, 2, 104, 600, "empty", False, False), (1, 4, 1, 128, 513, None, True, True),
+    (3, 1, 1, 16, 257, "empty", True, False), (1, 3, 1, 80, 700, "ragged", False, False), (1, 2, 2, 64, 20000, "ragged", False, False)])
+def test_cross_single_queries(Nq, H, G, hd, Nk, lens, mask, index, dtype):
+    """Up to four rows on a key / value head take the streaming kernel, with and without key splits."""
+    kn = K()
+    q, k, v, d_o, L, M, I = inputs(dtype, 3, 3, Nq, Nk, H, G, hd, lens, mask, index, seed=Nk)
+    val, tol = reference(q, k, v, H, G, L, M, I)
+    kp, vp = poison(k, v, L, M)
+    qd, kd, vd, Ld, Md, Id = cuda(q, kp, vp, L, M, I)
+    o, lse = kn.cross_fwd(qd, kd, vd, H, kv_heads=G, lens=Ld, mask=Md, index=Id)
+    assert kn.last_variant().startswith("cross_one")
+    check("o", o, val, tol)
+    check("lse", lse, val, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_cross_scale_and_large_scores(dtype):
     """A scale of the caller's, and scores far apart: the running maximum moves from block to block."""
     kn = K()
