@@ -88,12 +88,27 @@ def run_reverse_process(model, scheduler, z_init, labels, guidance_scale, eta, n
 class CFGSampler:
     """Batched 500-step CFG sampler: per step ONE UNet forward over [uncond; cond] (batch 2S) and ONE
     fused elementwise kernel (CFG combine, v->eps, DDPM mean, eta noise, final clamp).  No collective
-    in the loop: under data parallelism every rank samples its own shard of the labels."""
+    in the loop: under data parallelism every rank samples its own shard of the labels.
 
-    def __init__(self, model, scheduler, context_table: torch.Tensor, uncond_id: int):
+    ``context_table``: [ids, D], or [ids, L, D] with several tokens per id.  For the latter, ``context_lens`` [ids] and
+    ``context_mask`` [ids, L] say which tokens count; the table is then handed over whole with each sample's id as its
+    context, so keys and values are computed once per id instead of once per sample (UNET.forward)."""
+
+    def __init__(self, model, scheduler, context_table: torch.Tensor, uncond_id: int, context_lens=None, context_mask=None):
+        if (context_lens is not None or context_mask is not None) and context_table.dim() != 3:
+            raise ValueError("context_lens and context_mask need a context table [ids, L, D]")
         self.model, self.sched = model, scheduler
         self.table = context_table
         self.uncond_id = uncond_id
+        self.context_lens, self.context_mask = context_lens, context_mask
+
+    def _contexts(self, ids: torch.Tensor):
+        """The context arguments of the model for a batch of context ids: (context,) or (context, ContextMap)."""
+        table = self.table.to(ids.device)
+        if self.context_lens is None and self.context_mask is None:
+            return (table[ids].contiguous(),)
+        from .unet import ContextMap
+        return table.contiguous(), ContextMap.of(ids.device, self.context_lens, self.context_mask, ids)
 
     @torch.no_grad()
     def sample(self, z: torch.Tensor, labels: torch.Tensor, guidance_scale=6.0, eta: float = 1.0,
@@ -114,8 +129,7 @@ class CFGSampler:
         labels = labels.to(dev).long()
         g = torch.as_tensor(guidance_scale, dtype=torch.float32).expand(S).clone()
         g[labels.cpu() == self.uncond_id] = 0.0
-        table = self.table.to(dev)
-        ctx = torch.cat([table[torch.full_like(labels, self.uncond_id)], table[labels]]).contiguous()
+        ctx = self._contexts(torch.cat([torch.full_like(labels, self.uncond_id), labels]))
         z = z.contiguous().clone()
         zz = torch.empty((2 * S, *z.shape[1:]), dtype=torch.float32, device=dev)
         tt = torch.empty((2 * S,), dtype=torch.long, device=dev)
@@ -130,7 +144,7 @@ class CFGSampler:
             zz[:S].copy_(z)
             zz[S:].copy_(z)
             tt.fill_(t)
-            v, _ = model._fwd(zz, tt, ctx)
+            v, _ = model._fwd(zz, tt, *ctx)
             noise = None
             if (not final) and t > 1 and any_eta:
                 if noises is not None and t in noises:
@@ -168,13 +182,12 @@ class CFGSampler:
         g = torch.full((S,), float(guidance_scale), dtype=torch.float32)
         g[labels.cpu() == self.uncond_id] = 0.0
         beta, abar = self.sched.beta_cpu, self.sched.alpha_bar_cpu
-        table = self.table.to(dev)
-        ctx_u, ctx_c = table[torch.full_like(labels, self.uncond_id)], table[labels]
+        uncond = torch.full_like(labels, self.uncond_id)
         for t in range(starts[0], -1, -1):
             n = sum(1 for s0 in starts if s0 >= t)          # the active samples are a prefix
             zz = torch.cat([z[:n], z[:n]])
             tt = torch.full((2 * n,), t, dtype=torch.long, device=dev)
-            v, _ = model._fwd(zz, tt, torch.cat([ctx_u[:n], ctx_c[:n]]).contiguous())
+            v, _ = model._fwd(zz, tt, *self._contexts(torch.cat([uncond[:n], labels[:n]])))
             coef = step_coefficients(beta, abar, t, g[:n], eta, n, final=(t == 0)).to(dev)
             if t > 1 and eta > 0.0:
                 noise = torch.randn(z[:n].shape, dtype=torch.float32, device=dev, generator=generator)
@@ -200,9 +213,7 @@ class CFGSampler:
         g = torch.as_tensor(cfg_scale, dtype=torch.float32).expand(S).clone()
         g[g <= 1.0] = 1.0                                   # 1.0 = "conditional branch only" for the kernel
         guided = bool((g != 1.0).any())
-        table = self.table.to(dev)
-        ctx_c = table[labels]
-        ctx = torch.cat([table[torch.full_like(labels, self.uncond_id)], ctx_c]).contiguous() if guided else ctx_c.contiguous()
+        ctx = self._contexts(torch.cat([torch.full_like(labels, self.uncond_id), labels]) if guided else labels)
         dpm.set_timesteps(num_inference_steps, device=dev)
         steps = [int(t) for t in dpm.timesteps.tolist()]
         rows = []
@@ -224,7 +235,7 @@ class CFGSampler:
             if guided:
                 zz[S:].copy_(z)
             tt.fill_(t)
-            v, _ = model._fwd(zz, tt, ctx)
+            v, _ = model._fwd(zz, tt, *ctx)
             v_u, v_c = (v[:S], v[S:]) if guided else (v, v)
             z, m_prev = K.cfg_dpmpp2m_step(z, v_u, v_c, m_prev, coefs[i])
         return z

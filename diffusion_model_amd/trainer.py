@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import kernels as K
-from .unet import Grads, invalidate_packed_weights, repack_all, reseed_dropout
+from .unet import ContextMap, Grads, invalidate_packed_weights, repack_all, reseed_dropout
 
 
 def lr_lambda(step: int, total_steps: int) -> float:
@@ -330,8 +330,10 @@ class Trainer:
         self._gring = self._gopt = None
 
     def micro_step(self, x: torch.Tensor, context, t: torch.Tensor, e: torch.Tensor, *,
-                   step_now: Optional[bool] = None, check_finite: bool = False) -> torch.Tensor:
+                   step_now: Optional[bool] = None, check_finite: bool = False, context_lens=None, context_mask=None,
+                   context_index=None) -> torch.Tensor:
         """x,e: [B,C,H,W] fp32 on the device; t: [B] long (device); context: [B,D] fp32 or None.
+        context_lens / context_mask / context_index: as UNET.forward (such a micro-step runs eagerly, also beside a captured one).
         Returns the (un-synchronised) loss tensor [1].
         step_now overrides the accumulation gate (reference main_stl10.py:506: the last batch of an epoch
         steps even if the accumulation window is not full); check_finite mirrors main_stl10.py:484-486
@@ -339,7 +341,10 @@ class Trainer:
         last = ((self.micro + 1) % self.accum == 0) if step_now is None else bool(step_now)
         if self._graph is not None and getattr(self, "_gwhole", False):
             raise RuntimeError("a whole-step graph is live: use graph_step() (or disable_graph() first)")
-        if self._graph is not None and not check_finite and x.shape == self._gin[0].shape and \
+        cmap = ContextMap.of(x.device, context_lens, context_mask, context_index)
+        if cmap is not None and context is None:
+            raise ValueError("context_lens, context_mask and context_index need a context")
+        if self._graph is not None and not check_finite and x.shape == self._gin[0].shape and cmap is None and \
                 (context is None) == (self._gin[1] is None):
             gx, gc, gt, ge = self._gin
             gx.copy_(x, non_blocking=True)
@@ -360,7 +365,7 @@ class Trainer:
         abar = self.scheduler.alpha_t[t].contiguous()
         xt, v = K.qsample_vtarget(x, e, abar)
         tgt = v if self.target == "v" else e
-        y, saved = self.model._fwd(xt, t, context)
+        y, saved = self.model._fwd(xt, t, context, *(() if cmap is None else (cmap,)))
         w = self._loss_weights(B, chw, t)
         loss, dout = K.mse_loss_fwd_bwd(y, tgt, w.contiguous(), grad_scale=1.0 / self.accum)
         self.last_skipped = False

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Dict, List, Optional
+from typing import Dict, List, NamedTuple, Optional
 
 import torch
 import torch.nn as nn
@@ -197,6 +197,28 @@ class Grads:
 
     def peek(self, p):
         return self.bufs.get(id(p)) if self.views is None else self.views.get(id(p))
+
+
+class ContextMap(NamedTuple):
+    """Which context tokens a sample attends to (kernels.cross_fwd): valid length of each context, valid tokens of each
+    context, context of each sample.  None in a field: all of them / one context per sample."""
+    lens: Optional[torch.Tensor] = None
+    mask: Optional[torch.Tensor] = None
+    index: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def of(device, lens=None, mask=None, index=None) -> Optional["ContextMap"]:
+        """On ``device``, in the kernels' types; None when nothing is given."""
+        if lens is None and mask is None and index is None:
+            return None
+
+        def put(t, dtype):
+            return None if t is None else torch.as_tensor(t).to(device=device, dtype=dtype).contiguous()
+
+        return ContextMap(put(lens, torch.int32), put(mask, torch.bool), put(index, torch.int32))
+
+    def kw(self) -> dict:
+        return dict(lens=self.lens, mask=self.mask, index=self.index)
 
 
 def _b(c):
@@ -462,21 +484,37 @@ class ResBlock(HipModule):
 
 
 class Attention(HipModule):
-    """Reference unet.py:110-139 (self-attention over H*W tokens; no norm, no residual inside)."""
+    """Reference unet.py:110-139 (self-attention over H*W tokens; no norm, no residual inside).  ``rope=True`` (no
+    counterpart there: its tokens have no positions) turns queries and keys by their row and column (dm_rope, half of each
+    head per axis), in place in the fused projection; no parameter is added."""
 
-    def __init__(self, C: int, num_heads: int, dropout_prob: float, use_flash_attention: bool = True):
+    def __init__(self, C: int, num_heads: int, dropout_prob: float, use_flash_attention: bool = True, rope: bool = False):
         super().__init__()
+        if rope and (C % num_heads or C // num_heads % 4):
+            raise ValueError("rope needs head widths that are multiples of 4 (two axes, pairs of channels)")
         self.linear_qkv = nn.Linear(C, C * 3, bias=False)
         self.linear_out = nn.Linear(C, C, bias=False)
         self.dropout_prob = dropout_prob
         self.num_heads = num_heads
         self.use_flash_attention = use_flash_attention
         self.C = C
+        self.rope = rope
+
+    def _turn(self, qkv, H, W, inverse=False):
+        """Rotary positions on the query and key heads of a fused [B, H*W, 3C] buffer, in place (the inverse: on its gradient)."""
+        plan = self.__dict__.get("_dm_rope_plan")
+        if plan is None or plan.freq.device != qkv.device:
+            half = self.C // self.num_heads // 2
+            plan = self.__dict__["_dm_rope_plan"] = K.rope_plan(2 * half, (half, half), device=qkv.device)
+        qk = qkv[..., :2 * self.C]
+        K.rope(qk, 2 * self.num_heads, plan, grid=(H, W), inverse=inverse, out=qk)
 
     def _fwd(self, x, res=None, out=None, seed=None):
         B, H, W, C = x.shape
         tok = x.view(B, H * W, C)
         qkv = K.gemm(tok, PW.of(self.linear_qkv).fwd, 3 * C)
+        if self.rope:
+            self._turn(qkv, H, W)
         q, k, v = qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:]
         p = self.dropout_prob if self.training else 0.0
         if seed is None:
@@ -496,6 +534,8 @@ class Attention(HipModule):
         q, k, v = qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:]
         K.attn_bwd(q, k, v, o, lse, d_o, self.num_heads, dq=dqkv[..., :C], dk=dqkv[..., C:2 * C],
                    dv=dqkv[..., 2 * C:], drop_p=p, drop_seed=seed)
+        if self.rope:
+            self._turn(dqkv, dy.shape[1], dy.shape[2], inverse=True)
         K.wgrad_side(tok, dqkv, g.of(self.linear_qkv.weight), None, taps=1)
         dx = K.gemm(dqkv, PW.of(self.linear_qkv).bwd, C, res=None if add is None else add.view(B, N, C))
         return dx.view(dy.shape)
@@ -512,7 +552,9 @@ class Attention(HipModule):
 
 
 class CrossAttention(HipModule):
-    """Reference unet.py:141-220 (queries from pixels, keys/values from the context tokens)."""
+    """Reference unet.py:141-220 (queries from pixels, keys/values from the context tokens).  Contexts of different lengths,
+    masked tokens and contexts shared by several samples (none of which the reference has) come with a ContextMap and run
+    on dm_cross_fwd / dm_cross_bwd; a sample without a valid token gets nothing added."""
 
     def __init__(self, query_dim: int, context_dim: int, num_heads: int = 8, dropout_prob: float = 0.0,
                  use_flash_attention: bool = True):
@@ -537,8 +579,23 @@ class CrossAttention(HipModule):
         o = K.attn_onekey_fwd(vc, N, self.num_heads, drop_p=p, drop_seed=seed)
         return K.gemm(o, PW.of(self.to_out).fwd, C, res=res, out=out), o
 
-    # ctx: bf16 [B, L, Dc]
-    def _fwd(self, x, ctx, res=None, out=None, elide=False):
+    def _fwd_mapped(self, x, ctx, cmap, res, out):
+        B, H, W, C = x.shape
+        tok = x.view(B, H * W, C)
+        q = K.gemm(tok, PW.of(self.to_q).fwd, C)
+        kc = K.gemm(ctx, PW.of(self.to_k).fwd, C)
+        vc = K.gemm(ctx, PW.of(self.to_v).fwd, C)
+        p = self.dropout_prob if self.training else 0.0
+        seed = next(_SEED) if p > 0 else 0
+        o, lse = K.cross_fwd(q, kc, vc, self.num_heads, drop_p=p, drop_seed=seed, **cmap.kw())
+        y = K.gemm(o, PW.of(self.to_out).fwd, C, res=None if res is None else res.view(B, H * W, C),
+                   out=None if out is None else out.view(B, H * W, C))
+        return y.view(B, H, W, C), (tok, ctx, q, kc, vc, o, lse, p, seed, cmap)
+
+    # ctx: bf16 [B, L, Dc] (with an index in cmap: [contexts, L, Dc])
+    def _fwd(self, x, ctx, res=None, out=None, elide=False, cmap=None):
+        if cmap is not None:
+            return self._fwd_mapped(x, ctx, cmap, res, out)
         B, H, W, C = x.shape
         N = H * W
         if elide:  # one context token: the output does not depend on x (see ELIDE_DEAD_ATTENTION)
@@ -546,7 +603,7 @@ class CrossAttention(HipModule):
             p = self.dropout_prob if self.training else 0.0
             seed = next(_SEED) if p > 0 else 0
             y, o = self._onekey_out(vc, B, N, C, res, out, p, seed)
-            return y.view(B, H, W, C), (None, ctx, None, None, vc, o, None, p, seed)
+            return y.view(B, H, W, C), (None, ctx, None, None, vc, o, None, p, seed, None)
         tok = x.view(B, N, C)
         q = K.gemm(tok, PW.of(self.to_q).fwd, C)
         kc = K.gemm(ctx, PW.of(self.to_k).fwd, C)
@@ -559,13 +616,13 @@ class CrossAttention(HipModule):
             # one token: same output path as the two-stream schedule (UnetLayer._fwd_attn_overlapped), so the two
             # schedules stay bit-identical; q / k only feed the log-sum-exp
             y, o = self._onekey_out(vc, B, N, C, res, out, p, seed)
-            return y.view(B, H, W, C), (tok, ctx, q, kc, vc, o, lse, p, seed)
+            return y.view(B, H, W, C), (tok, ctx, q, kc, vc, o, lse, p, seed, None)
         y = K.gemm(o, PW.of(self.to_out).fwd, C, res=None if res is None else res.view(B, N, C),
                    out=None if out is None else out.view(B, N, C))
-        return y.view(B, H, W, C), (tok, ctx, q, kc, vc, o, lse, p, seed)
+        return y.view(B, H, W, C), (tok, ctx, q, kc, vc, o, lse, p, seed, None)
 
     def _bwd(self, dy, saved, g: Grads, add=None, need_dctx=False):
-        tok, ctx, q, kc, vc, o, lse, p, seed = saved
+        tok, ctx, q, kc, vc, o, lse, p, seed, cmap = saved
         B, H, W, C = dy.shape
         N = H * W
         dyt = dy.view(B, N, C)
@@ -587,6 +644,8 @@ class CrossAttention(HipModule):
         if fused:   # one key: dq and dk are exact zeros (dm_attn_bwd writes the same zeros); the rest runs as always
             dq = _zeros_ro((B, N, C), dy.dtype, dy.device)    # (read-only operands of the GEMMs below: one cached buffer
             dk = _zeros_ro(tuple(dv.shape), dv.dtype, dv.device)  #  per shape instead of a 75 MB memset per layer and step)
+        elif cmap is not None:
+            dq, dk, dv = K.cross_bwd(q, kc, vc, o, lse, d_o, self.num_heads, drop_p=p, drop_seed=seed, **cmap.kw())
         else:
             dq, dk, dv = K.attn_bwd(q, kc, vc, o, lse, d_o, self.num_heads, drop_p=p, drop_seed=seed)
         K.wgrad_side(tok, dq, g.of(self.to_q.weight), None, taps=1)
@@ -611,15 +670,16 @@ class CrossAttention(HipModule):
             K.gemm(d, PW.of(lin).bwd, self.context_dim, out_f32=part)
             K.batchsum(part.view(1, -1), g.dctx.view(-1))
 
-    def forward(self, x, context):
-        return self._apply_fn(x, context)
+    def forward(self, x, context, context_lens=None, context_mask=None, context_index=None):
+        """``context_lens`` [contexts], ``context_mask`` [contexts, L], ``context_index`` [B]: see ContextMap."""
+        return self._apply_fn(x, context, ContextMap.of(x.device, context_lens, context_mask, context_index))
 
-    def _run_fwd(self, x, context):
+    def _run_fwd(self, x, context, cmap=None):
         c = context.detach().float()
         self._ctx2d = c.dim() == 2
         if c.dim() == 2:
             c = c.unsqueeze(1)
-        y, saved = self._fwd(_nhwc_in(x), K.to_bf16(c.contiguous()))
+        y, saved = self._fwd(_nhwc_in(x), K.to_bf16(c.contiguous()), cmap=cmap)
         return K.nhwc_to_nchw(y), saved
 
     def _run_bwd(self, dout, saved, g, need):
@@ -715,11 +775,13 @@ class UnetLayer(HipModule):
 
     def __init__(self, upscale: bool, attention: bool, num_groups: int, dropout_prob: float, in_channels: int,
                  out_channels: int, time_emb_dim: int, num_heads: int = 4, use_film: bool = False,
-                 use_cross_attention: bool = False, context_dim: int = None, use_flash_attention: bool = True):
+                 use_cross_attention: bool = False, context_dim: int = None, use_flash_attention: bool = True,
+                 rope: bool = False):
         super().__init__()
         self.res_block = ResBlock(in_channels, out_channels, time_emb_dim, num_groups, dropout_prob, use_film)
         if attention:
-            self.attention = Attention(out_channels, num_heads, dropout_prob, use_flash_attention=use_flash_attention)
+            self.attention = Attention(out_channels, num_heads, dropout_prob, use_flash_attention=use_flash_attention,
+                                       rope=rope)
         if use_cross_attention and context_dim is not None:
             self.cross_attention = CrossAttention(query_dim=out_channels, context_dim=context_dim,
                                                   num_heads=num_heads, dropout_prob=dropout_prob,
@@ -731,7 +793,7 @@ class UnetLayer(HipModule):
             self.downsample = Downsample(out_channels)
         self.cout = out_channels
 
-    def _fwd(self, x, temb, ctx, skip_out=None, y_out=None):
+    def _fwd(self, x, temb, ctx, skip_out=None, y_out=None, cmap=None):
         """Down layers write the pre-downsample tensor (the skip) into ``skip_out``; up layers write
         their output into ``y_out`` (both are channel slices of the decoder's concat buffer)."""
         has_a = hasattr(self, "attention")
@@ -740,7 +802,8 @@ class UnetLayer(HipModule):
         r, s_res = self.res_block._fwd(x, temb)
         dst = None if up else skip_out
         s_a = s_c = None
-        bf = r.dtype == BF16   # the one-token specialisations (elision, two-stream schedule, dm_cross1) are bf16-mode kernels
+        # the one-token specialisations (elision, two-stream schedule, dm_cross1): bf16 mode, every token counts
+        bf = r.dtype == BF16 and cmap is None
         elide = has_c and bf and ELIDE_DEAD_ATTENTION[0] and ctx.shape[1] == 1
         if elide:
             if has_a and self.attention.training and self.attention.dropout_prob > 0:
@@ -750,11 +813,11 @@ class UnetLayer(HipModule):
             xo, s_a, s_c = self._fwd_attn_overlapped(r, ctx, dst)
         elif has_a and has_c:
             xa, s_a = self.attention._fwd(r)
-            xo, s_c = self.cross_attention._fwd(xa, ctx, res=r, out=dst)
+            xo, s_c = self.cross_attention._fwd(xa, ctx, res=r, out=dst, cmap=cmap)
         elif has_a:
             xo, s_a = self.attention._fwd(r, res=r, out=dst)
         elif has_c:
-            xo, s_c = self.cross_attention._fwd(r, ctx, res=r, out=dst)
+            xo, s_c = self.cross_attention._fwd(r, ctx, res=r, out=dst, cmap=cmap)
         else:
             xo = K.add(r, r, out=dst)
         if up:
@@ -793,7 +856,7 @@ class UnetLayer(HipModule):
             # (only the log-sum-exp: the attention output itself is formed on the main stream, _onekey_out)
             _, lse = K.attn_fwd(q, kc, vc, ca.num_heads, drop_p=p_c, drop_seed=seed_c, want_o=False)
         y, o = ca._onekey_out(vc, B, N, C, r, dst, p_c, seed_c)
-        return y.view(B, H, W, C), s_a, (tok, ctx, q, kc, vc, o, lse, p_c, seed_c)
+        return y.view(B, H, W, C), s_a, (tok, ctx, q, kc, vc, o, lse, p_c, seed_c, None)
 
     def _bwd(self, dy, d_skip, saved, g: Grads, dts=None, need_dx=True):
         s_res, s_a, s_c, s_ud, u = saved
@@ -811,7 +874,7 @@ class UnetLayer(HipModule):
             if hasattr(self, "attention"):  # zero gradients, exactly: leave the accumulators untouched
                 g.of(self.attention.linear_qkv.weight), g.of(self.attention.linear_out.weight)
             dr = dxo  # d(xo)/d(r) is the residual branch alone
-        elif (s_c is not None and dxo.dtype == BF16 and OVERLAP_DEAD_ATTENTION[0] and s_c[1].shape[1] == 1
+        elif (s_c is not None and dxo.dtype == BF16 and OVERLAP_DEAD_ATTENTION[0] and s_c[1].shape[1] == 1 and s_c[9] is None
               and (s_a is not None or OVERLAP_CROSS_ONLY[0]) and g.dctx is None):   # (a context gradient is accumulated across layers: keep that on one stream)
             # One context token: d(cross_attention)/d(its query input) is exactly 0 (dq = 0 out of a softmax over one
             # key), so the gradient that comes back through attention(r) is an exact zero and dr = dxo.  Everything
@@ -845,14 +908,14 @@ class UNET(HipModule):
                  Attentions: List = [False, True, True, False], num_groups: int = 8, dropout_prob: float = 0.1,
                  num_heads: int = 8, time_steps: int = 1000, input_channels: int = 1, output_channels: int = 1,
                  label_embedding: bool = True, use_film: bool = False, use_cross_attention: bool = True,
-                 context_dim: int = None, use_flash_attention: bool = True):
+                 context_dim: int = None, use_flash_attention: bool = True, rope: bool = False):
         super().__init__()
         time_emb_dim = 256
         self.num_layers = len(Channels) - 1
         for i in range(self.num_layers):
             layer = UnetLayer(Upscales[i], Attentions[i], num_groups, dropout_prob, Channels[i], Channels[i + 1],
                               time_emb_dim, num_heads, use_film, use_cross_attention=use_cross_attention,
-                              context_dim=context_dim, use_flash_attention=use_flash_attention)
+                              context_dim=context_dim, use_flash_attention=use_flash_attention, rope=rope)
             setattr(self, f"Layer{i + 1}", layer)
         out_channels = (Channels[-1] // 2) + Channels[1]
         self.input_conv = nn.Conv2d(input_channels, Channels[0], kernel_size=3, padding=1)
@@ -879,7 +942,7 @@ class UNET(HipModule):
         return [getattr(self, f"Layer{i + 1}") for i in range(self.num_layers)]
 
     # ------------------------------------------------------------------ hand-scheduled forward
-    def _fwd(self, x, t, context):
+    def _fwd(self, x, t, context, cmap=None):
         B, Cin, H, W = x.shape
         dev_ = x.device
         e16 = K.to_bf16(self.time_embeddings(t).contiguous())
@@ -905,11 +968,11 @@ class UNET(HipModule):
             j = L - 1 - i
             c_dec, c_skip = self.Channels[j + 1] // 2, self.Channels[i + 1]
             cats[j] = torch.empty((B, a.shape[1], a.shape[2], c_dec + c_skip), dtype=a.dtype, device=dev_)
-            a, _, s = self.layers()[i]._fwd(a, temb, ctx, skip_out=cats[j][..., c_dec:])
+            a, _, s = self.layers()[i]._fwd(a, temb, ctx, skip_out=cats[j][..., c_dec:], cmap=cmap)
             saved_layers.append(s)
         for i in range(half, L):
             c_dec = self.Channels[i + 1] // 2
-            _, _, s = self.layers()[i]._fwd(a, temb, ctx, y_out=cats[i][..., :c_dec])
+            _, _, s = self.layers()[i]._fwd(a, temb, ctx, y_out=cats[i][..., :c_dec], cmap=cmap)
             a = cats[i]
             saved_layers.append(s)
         cat = a
@@ -996,9 +1059,15 @@ class UNET(HipModule):
         return dx
 
     # ------------------------------------------------------------------ public API
-    def forward(self, x, t, context=None):
+    def forward(self, x, t, context=None, context_lens=None, context_mask=None, context_index=None):
+        """``context`` [B, D] or [B, L, D] as in the reference.  Beyond it: ``context_lens`` (valid tokens of each context, 0
+        allowed), ``context_mask`` [B, L] (True where valid) and ``context_index`` [B] (then ``context`` holds each distinct
+        context once, [contexts, L, D], and its keys and values are computed once)."""
         if not x.is_cuda:
             raise RuntimeError("diffusion_model_amd.UNET runs only on an AMD GPU (HIP kernels); no CPU fallback")
+        cmap = ContextMap.of(x.device, context_lens, context_mask, context_index)
+        if cmap is not None and (context is None or not torch.is_floating_point(context)):
+            raise ValueError("context_lens, context_mask and context_index need a context")
         if context is not None and not torch.is_floating_point(context):
             if any(hasattr(l, "cross_attention") for l in self.layers()):
                 raise TypeError("integer labels as context are only accepted when no cross-attention exists "
@@ -1008,8 +1077,8 @@ class UNET(HipModule):
             t = torch.as_tensor(t, dtype=torch.long)
         if torch.is_grad_enabled() and (x.requires_grad or (torch.is_tensor(context) and context.requires_grad)
                                         or any(p.requires_grad for p in self.parameters())):
-            return _UNetFn.apply(self, x, t, context, *list(self.parameters()))
-        y, _ = self._fwd(x, t, context)
+            return _UNetFn.apply(self, x, t, context, cmap, *list(self.parameters()))
+        y, _ = self._fwd(x, t, context, cmap)
         return y
 
 
@@ -1023,8 +1092,8 @@ def _pad_bias(c: nn.Module, npad: int):
 
 class _UNetFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, mod, x, t, context, *params):
-        y, saved = mod._fwd(x, t, context)
+    def forward(ctx, mod, x, t, context, cmap, *params):
+        y, saved = mod._fwd(x, t, context, cmap)
         ctx.mod, ctx.saved, ctx.params = mod, saved, params
         ctx.need_dx = x.requires_grad
         ctx.need_dctx = torch.is_tensor(context) and torch.is_floating_point(context) and context.requires_grad
@@ -1042,4 +1111,4 @@ class _UNetFn(torch.autograd.Function):
         dctx = None
         if ctx.need_dctx:   # zeros when the network has no cross-attention (the context is then unused)
             dctx = (g.dctx if g.dctx is not None else torch.zeros(ctx.ctx_shape, device=dout.device)).view(ctx.ctx_shape)
-        return (None, dx, None, dctx, *pg)
+        return (None, dx, None, dctx, None, *pg)

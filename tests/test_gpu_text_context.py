@@ -1,0 +1,254 @@
+"""GPU: rotary positions and contexts of different lengths where a user has them -- Attention, CrossAttention, UNET, Trainer
+and CFGSampler -- against plain restatements in the oracle's network, and against the network's own runs without them."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from conftest import assert_close
+from oracle import unet_ref as oref
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.bfloat16: 2e-2, torch.float32: 1e-4}      # the package's parity bars for its two compute modes
+KW = dict(input_channels=3, output_channels=3, context_dim=48, dropout_prob=0.0)
+HEADS = 8
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def turned(x, H, W):
+    """[B, heads, H*W, d]: first half of the channels by row, second half by column, neighbouring pairs, theta 10000."""
+    d = x.shape[-1] // 2
+    f = 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    row, col = torch.meshgrid(torch.arange(H), torch.arange(W), indexing="ij")
+    ang = torch.cat([row.reshape(-1, 1) * f, col.reshape(-1, 1) * f], -1)
+    z = torch.view_as_complex(x.double().reshape(*x.shape[:-1], d, 2)) * torch.polar(torch.ones_like(ang), ang)
+    return torch.view_as_real(z).flatten(-2).to(x.dtype)
+
+
+def plain_self_attention(sd, p, x, heads, drop_p=0.0, train=False):
+    B, C, H, W = x.shape
+    tok = x.permute(0, 2, 3, 1).reshape(B, H * W, C)
+    q, k, v = F.linear(tok, sd[p + "linear_qkv.weight"]).reshape(B, H * W, 3, heads, C // heads).permute(2, 0, 3, 1, 4)
+    o = oref.softmax_attention(turned(q, H, W), turned(k, H, W), v).permute(0, 2, 1, 3).reshape(B, H * W, C)
+    return F.linear(o, sd[p + "linear_out.weight"]).reshape(B, H, W, C).permute(0, 3, 1, 2).contiguous()
+
+
+class PlainCross:
+    """cross_attention of the oracle with lengths, a mask and an index: sample by sample over the valid tokens alone."""
+
+    def __init__(self, lens=None, mask=None, index=None):
+        self.lens, self.mask, self.index = lens, mask, index
+
+    def __call__(self, sd, p, x, ctx, heads, drop_p=0.0, train=False):
+        B, C, H, W = x.shape
+        d = C // heads
+        outs = []
+        for b in range(B):
+            c = b if self.index is None else int(self.index[b])
+            rows = torch.arange(ctx.shape[1] if self.lens is None else int(self.lens[c]))
+            if self.mask is not None:
+                rows = rows[self.mask[c, :len(rows)]]
+            tok = x[b].permute(1, 2, 0).reshape(H * W, C)
+            if len(rows) == 0:
+                outs.append(torch.zeros_like(x[b]))
+                continue
+            q = F.linear(tok, sd[p + "to_q.weight"]).reshape(-1, heads, d).transpose(0, 1)
+            k = F.linear(ctx[c, rows], sd[p + "to_k.weight"]).reshape(-1, heads, d).transpose(0, 1)
+            v = F.linear(ctx[c, rows], sd[p + "to_v.weight"]).reshape(-1, heads, d).transpose(0, 1)
+            o = (torch.softmax(q @ k.transpose(-1, -2) / math.sqrt(d), -1) @ v).transpose(0, 1).reshape(H * W, C)
+            outs.append(F.linear(o, sd[p + "to_out.weight"]).reshape(H, W, C).permute(2, 0, 1))
+        return torch.stack(outs)
+
+
+def network(rope, seed=3):
+    from diffusion_model_amd.unet import UNET
+    torch.manual_seed(seed)
+    m = UNET(**KW, rope=rope)
+    with torch.no_grad():
+        m.output_conv.weight.normal_(0, 0.05)
+    sd = {k: v.detach().clone() for k, v in m.state_dict().items()}
+    return m.to(dev()).eval(), sd
+
+
+def case(B, Bc, L, seed=5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, 3, 24, 16, generator=g)
+    ctx = torch.randn(Bc, L, KW["context_dim"], generator=g)
+    t = torch.randint(0, 500, (B,), generator=g)
+    return x, t, ctx
+
+
+def test_rope_keeps_the_state_dict():
+    a, sa = network(False)
+    b, sb = network(True)
+    assert list(sa) == list(sb) and all(torch.equal(sa[k], sb[k]) for k in sa)
+
+
+def test_rope_refuses_odd_head_widths():
+    from diffusion_model_amd.unet import Attention
+    with pytest.raises(ValueError):
+        Attention(48, 8, 0.0, rope=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rope_self_attention_module(dtype):
+    from diffusion_model_amd import kernels as K
+    from diffusion_model_amd.unet import Attention
+    torch.manual_seed(1)
+    m = Attention(128, HEADS, 0.0, rope=True)
+    sd = {k: v.detach().clone().requires_grad_() for k, v in m.state_dict().items()}
+    m = m.to(dev()).eval()
+    x, w = torch.randn(2, 128, 7, 9), torch.randn(2, 128, 7, 9)
+    xr = x.clone().requires_grad_()
+    ref = plain_self_attention(sd, "", xr, HEADS)
+    (ref * w).sum().backward()
+    with K.compute_dtype(dtype):
+        xd = x.to(dev()).requires_grad_()
+        y = m(xd)
+        (y * w.to(dev())).sum().backward()
+    assert_close(y, ref, TOL[dtype], "y")
+    assert_close(xd.grad, xr.grad, TOL[dtype], "gx")
+    for n, p in m.named_parameters():
+        assert_close(p.grad, sd[n].grad, TOL[dtype], n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["lens", "mask", "index"])
+def test_cross_attention_module(kind, dtype):
+    from diffusion_model_amd import kernels as K
+    from diffusion_model_amd.unet import CrossAttention
+    torch.manual_seed(2)
+    B, Bc, L = 4, (2 if kind == "index" else 4), 21
+    m = CrossAttention(64, 48, HEADS, 0.0)
+    sd = {k: v.detach().clone().requires_grad_() for k, v in m.state_dict().items()}
+    m = m.to(dev()).eval()
+    x, ctx, w = torch.randn(B, 64, 6, 5), torch.randn(Bc, L, 48), torch.randn(B, 64, 6, 5)
+    lens = torch.tensor([7, 0, 21, 1][:Bc])
+    mask = torch.rand(Bc, L) < 0.6
+    index = torch.tensor([1, 0, 0, 1])
+    opt = dict(lens=dict(lens=lens), mask=dict(mask=mask), index=dict(lens=torch.tensor([9, 14]), index=index))[kind]
+    xr, cr = x.clone().requires_grad_(), ctx.clone().requires_grad_()
+    ref = PlainCross(**opt)(sd, "", xr, cr, HEADS)
+    (ref * w).sum().backward()
+    with K.compute_dtype(dtype):
+        xd, cd = x.to(dev()).requires_grad_(), ctx.to(dev()).requires_grad_()
+        y = m(xd, cd, **{"context_" + k: v for k, v in opt.items()})
+        (y * w.to(dev())).sum().backward()
+    assert_close(y, ref, TOL[dtype], "y")
+    assert_close(xd.grad, xr.grad, TOL[dtype], "gx")
+    assert_close(cd.grad, cr.grad, TOL[dtype], "gctx")
+    for n, p in m.named_parameters():
+        assert_close(p.grad, sd[n].grad, TOL[dtype], n)
+
+
+@pytest.mark.parametrize("rope,opt,Bc", [
+    (True, {}, 3), (False, dict(lens=[5, 0, 11]), 3), (True, dict(lens=[5, 11, 3]), 3), (True, dict(lens=[4, 11], index=[1, 0, 1]), 2),
+    (True, dict(mask="random"), 3)])
+def test_network_against_the_oracle(monkeypatch, rope, opt, Bc):
+    """The whole network with both operators, forward and gradients, in the fp32 mode (1e-4) and forward in bf16."""
+    from diffusion_model_amd import kernels as K
+    B, L = 3, 11
+    x, t, ctx = case(B, Bc, L)
+    opt = {k: (torch.rand(Bc, L, generator=torch.Generator().manual_seed(6)) < 0.7 if k == "mask" else torch.tensor(v)) for k, v in opt.items()}
+    m, sd = network(rope)
+    if rope:
+        monkeypatch.setattr(oref, "self_attention", plain_self_attention)
+    if opt:
+        monkeypatch.setattr(oref, "cross_attention", PlainCross(**opt))
+    sdr = {k: v.clone().requires_grad_() for k, v in sd.items()}
+    cr = ctx.clone().requires_grad_()
+    ref = oref.unet_forward(sdr, oref.UNetSpec(**KW), x, t, cr)
+    w = torch.randn(ref.shape, generator=torch.Generator().manual_seed(7))
+    (ref * w).sum().backward()
+    kw = {"context_" + k: v for k, v in opt.items()}
+    with K.compute_dtype(torch.float32):
+        cd = ctx.to(dev()).requires_grad_()
+        y = m(x.to(dev()), t, cd, **kw)
+        (y * w.to(dev())).sum().backward()
+    assert_close(y, ref, 1e-4, "y")
+    assert_close(cd.grad, cr.grad, 1e-4, "gctx")
+    for n, p in m.named_parameters():
+        assert_close(p.grad, sdr[n].grad, 1e-4, n)
+    with torch.no_grad():
+        assert_close(m(x.to(dev()), t, ctx.to(dev()), **kw), ref, 2e-2, "y bf16")
+
+
+def test_network_refuses_a_map_without_a_context():
+    m, _ = network(False)
+    with pytest.raises(ValueError):
+        m(torch.zeros(1, 3, 16, 16, device=dev()), torch.tensor([1]), None, context_lens=[1])
+
+
+def test_padding_and_sharing_change_nothing():
+    """bf16: what padding tokens hold is not read, and a shared context gives each sample what its own copy gives."""
+    m, _ = network(True)
+    x, t, ctx = case(4, 2, 13)
+    lens, index = torch.tensor([13, 6]), torch.tensor([0, 1, 1, 0])
+    with torch.no_grad():
+        a = m(x.to(dev()), t, ctx.to(dev()), context_lens=lens, context_index=index)
+        b = m(x.to(dev()), t, ctx[index].to(dev()), context_lens=lens[index])
+        noisy = ctx.clone()
+        noisy[1, 6:] = 1e4
+        c = m(x.to(dev()), t, noisy.to(dev()), context_lens=lens, context_index=index)
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_training_steps_with_lengths():
+    """Trainer with ragged contexts and dropout: the loss is finite, gradients reach every cross-attention weight, the step
+    moves the weights; the same seed gives the same bits again."""
+    from diffusion_model_amd.trainer import Trainer
+    from diffusion_model_amd.unet import UNET, reseed_dropout
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    runs = []
+    for _ in range(2):
+        torch.manual_seed(11)
+        m = UNET(**{**KW, "dropout_prob": 0.1}, rope=True)
+        with torch.no_grad():
+            m.output_conv.weight.normal_(0, 0.05)
+        m = m.to(dev()).train()
+        tr = Trainer(m, DDPM_beta_t_cosine_scheduler(500), accum=1)
+        reseed_dropout(5)
+        x, t, ctx = case(4, 4, 9)
+        before = m.Layer1.cross_attention.to_k.weight.detach().clone()
+        losses = [float(tr.micro_step(x.to(dev()), ctx.to(dev()), t.to(dev()), torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).to(dev()),
+                                      context_lens=torch.tensor([9, 4, 0, 1]))) for i in range(2)]
+        assert all(math.isfinite(v) for v in losses) and not torch.equal(before, m.Layer1.cross_attention.to_k.weight)
+        runs.append((losses, {n: p.detach().clone() for n, p in m.named_parameters()}))
+    assert runs[0][0] == runs[1][0] and all(torch.equal(runs[0][1][n], runs[1][1][n]) for n in runs[0][1])
+    with pytest.raises(ValueError):
+        tr.micro_step(x.to(dev()), None, t.to(dev()), x.to(dev()), context_lens=[1, 1, 1, 1])
+
+
+def test_sampling_from_a_table_of_token_contexts():
+    """CFGSampler: a table [ids, L, D] with lengths, handed over whole, against each sample's own copy of its context."""
+    from diffusion_model_amd.sampler import CFGSampler
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    m, _ = network(True)
+    sched = DDPM_beta_t_cosine_scheduler(500)
+    g = torch.Generator().manual_seed(8)
+    table, lens = torch.randn(4, 7, KW["context_dim"], generator=g).to(dev()), torch.tensor([7, 3, 5, 1])
+    z, labels = torch.randn(5, 3, 16, 16, generator=g).to(dev()), torch.tensor([0, 1, 2, 1, 3])
+
+    class Copies:
+        """The same model, given every sample's own context."""
+        eval = staticmethod(m.eval)
+
+        @staticmethod
+        def _fwd(zz, tt, ctx, cmap):
+            from diffusion_model_amd.unet import ContextMap
+            ids = cmap.index.long()
+            return m._fwd(zz, tt, ctx[ids].contiguous(), ContextMap(cmap.lens[ids].contiguous(), None, None))
+
+    kw = dict(guidance_scale=3.0, eta=0.0, t_stop=496)
+    a = CFGSampler(m, sched, table, 3, context_lens=lens).sample(z, labels, **kw)
+    b = CFGSampler(Copies, sched, table, 3, context_lens=lens).sample(z, labels, **kw)
+    assert torch.equal(a, b)
+    full = CFGSampler(m, sched, table, 3, context_lens=torch.full((4,), 7)).sample(z, labels, **kw)
+    plain = CFGSampler(m, sched, table, 3).sample(z, labels, **kw)      # every token counts: the kernels without a map
+    assert_close(full, plain, 2e-2, "all tokens")
+    with pytest.raises(ValueError):
+        CFGSampler(m, sched, table[:, 0], 3, context_lens=lens)
