@@ -32,8 +32,11 @@ struct CrossParams {
   int kb;                      // keys staged per LDS image (a multiple of 64)
   int iters;                   // query tiles per wave and workgroup
   int nqb;                     // workgroups along the queries
+  int wk;                      // waves of a workgroup that share a query tile, each with its own keys (1, 2 or 4)
   int nsplit, ksplit;          // forward: key splits and keys per split; dk / dv: splits of the query list
   float* part;                 // split results
+  int qsplit, qksplit;         // dq: key splits and keys per split
+  float* qpart;                // [qsplit][B, heads, Nq][hd]
 };
 
 // context of a sample, or -1 (no keys)
@@ -311,8 +314,23 @@ __device__ __forceinline__ uint32_t xcd_contiguous(uint32_t id, uint32_t n) {
   return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
 }
 
+// A query tile's result (head-dim-major, queries on the lanes) into LDS rows of HDP + 4 floats, one row per query
+template <int HDP, int DT>
+__device__ __forceinline__ void put_rows(float* rows, const f32x16 (&acc)[DT], int lane) {
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < (HDP < 32 ? 2 : 4); ++i)
+      *reinterpret_cast<f32x4*>(rows + (lane & 31) * (HDP + 4) + d * 32 + 8 * i + 4 * (lane >> 5)) =
+          f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+}
+
 // ---------------------------------------------------------------- host side
 inline int cross_hdp(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 96 ? 96 : 128))); }
+
+// waves that share a query tile: with one or two tiles of 32 queries the others would have none
+inline int cross_wk(const dm_cross_args* a) { return a->Nq <= 32 ? 4 : (a->Nq <= 64 ? 2 : 1); }
+inline long cross_groups(const dm_cross_args* a) { const long per = 32 * (4 / cross_wk(a)); return (a->Nq + per - 1) / per; }
 
 inline bool cross_sizes_ok(const dm_cross_args* a) {
   return a && a->B > 0 && a->Bc > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->Nq > 0 &&

@@ -14,7 +14,7 @@ using namespace dm_cross;
 // as the forward: resident keys, or two images of 64 keys in turn
 template <typename T, int HDP> constexpr int image_bytes() { return 64 * (2 * Geo<T, HDP>::SR + 4) + 16; }
 
-template <typename T, int HDP, bool RES, bool DROP>
+template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cross_dq_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   typedef typename Cr<T>::frag frag;
@@ -27,8 +27,11 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
   uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int h = id % p.H;
   id /= p.H;
-  const int qb = id % p.nqb, b = id / p.nqb;
-  const int ctx = context_of(p, b), kn = keys_of(p, ctx);
+  const int qb = id % p.nqb;
+  id /= p.nqb;
+  const int split = id % p.qsplit, b = id / p.qsplit;
+  const int ctx = context_of(p, b);
+  const int k0 = split * p.qksplit, kn = min(keys_of(p, ctx), k0 + p.qksplit);
   const int hdb = p.hd * (int)sizeof(T), g = h / (p.H / p.G);
   const long krow = (long)(ctx < 0 ? 0 : ctx) * p.Nk;
   const char* kbase = p.k + krow * p.ldk + g * hdb;
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     delta = half_sum(s);
     L2 = ok ? p.lse[row] * CR_LOG2E : INFINITY;
     if (L2 == -INFINITY) L2 = INFINITY;        // no probability without a finite score, nor past the last query
-    if (ok && half == 0) p.delta[row] = delta;
+    if (ok && half == 0 && split == 0) p.delta[row] = delta;
     if (DROP) rs = dm_drop_row(seed, (uint32_t)row);
 #pragma unroll
     for (int d = 0; d < Gm::DT; ++d)
@@ -67,8 +70,8 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     stage_rows2<T, HDP>(sK, Gm::SR, kbase, p.ldk, sV, Gm::SR, vbase, p.ldv, from, n, kn, mask, hdb, tid);
     stage_valid(bits, bias, from, n, kn, mask, tid);
   };
-  auto sweep = [&](int from, int tiles) {
-    for (int t = 0; t < tiles; ++t) {
+  auto sweep = [&](int from, int tiles, int first, int step) {
+    for (int t = first; t < tiles; t += step) {
       const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
       if (w == 0) continue;
       f32x16 s = score_init(bias + t * 32, half), dp = zero16();      // (masked keys: exp2(-inf) = 0)
@@ -99,20 +102,51 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     }
   };
   auto finish = [&](int q) {
+    if (p.qsplit > 1) {
+      const long row = (((long)split * p.B + b) * p.H + h) * p.Nq + q;
+      const Rows dst = rows_of((char*)(p.qpart + row * p.hd), p.hd * 4, p.Nq - q, p.hd * 4, lane);
+#pragma unroll
+      for (int d = 0; d < Gm::DT; ++d) store_tile<float>(dst, acc[d], 1.f, d * 32, p.hd * 4, lane);
+      return;
+    }
     const Rows dst = rows_of(p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb, p.lddq, p.Nq - q, hdb, lane);
 #pragma unroll
     for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, acc[d], p.scale, d * 32, hdb, lane);
   };
+  if (SPLIT) {
+    // one or two query tiles: the waves that share a tile take its keys' tiles in turn, and their sums are added in order
+    const int WK = p.wk, n = max(0, (kn - k0 + 31) & ~31);
+    begin(wave / WK * 32);
+    stage(k0, n);
+    __syncthreads();
+    sweep(k0, n >> 5, wave % WK, WK);
+    __syncthreads();
+    constexpr int RS = HDP + 4;
+    float* sum = reinterpret_cast<float*>(smem);
+    put_rows<HDP>(sum + wave * 32 * RS, acc, lane);
+    __syncthreads();
+    const int per = p.hd >> 2;
+    for (int i = tid; i < min(p.Nq, 128 / WK) * per; i += 256) {
+      const int q = i / per, col = (i - q * per) * 4;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < WK; ++k) x += *reinterpret_cast<const f32x4*>(sum + (((q >> 5) * WK + k) * 32 + (q & 31)) * RS + col);
+      if (p.qsplit > 1)
+        *reinterpret_cast<f32x4*>(p.qpart + ((((long)split * p.B + b) * p.H + h) * p.Nq + q) * p.hd + col) = x;
+      else
+        store4<T>(p.dq + ((long)b * p.Nq + q) * p.lddq + h * hdb + col * (int)sizeof(T), x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
+    }
+    return;
+  }
   const int q0 = qb * p.iters * 128 + wave * 32;
   if (RES) {
-    const int n = (kn + 31) & ~31;
-    stage(0, n);
+    const int n = max(0, (kn - k0 + 31) & ~31);
+    stage(k0, n);
     __syncthreads();
     for (int it = 0; it < p.iters; ++it) {
       const int q = q0 + it * 128;
       if (q >= p.Nq) break;
       begin(q);
-      sweep(0, n >> 5);
+      sweep(k0, n >> 5, 0, 1);
       finish(q);
     }
   } else {
@@ -129,16 +163,16 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
       bias = reinterpret_cast<float*>(sV + 64 * Gm::SR);
       bits = reinterpret_cast<uint32_t*>(bias + 64);
     };
-    if (kn > 0) load(0);
+    if (k0 < kn) load(k0);
     begin(q0);
     use(0);
-    if (kn > 0) store(0);
+    if (k0 < kn) store(k0);
     __syncthreads();
-    for (int from = 0, i = 0; from < kn; from += 64, ++i) {
+    for (int from = k0, i = 0; from < kn; from += 64, ++i) {
       const bool more = from + 64 < kn;
       if (more) load(from + 64);
       use(i);
-      sweep(from, 2);
+      sweep(from, 2, 0, 1);
       use(i + 1);
       if (more) store(from + 64);
       __syncthreads();
@@ -347,6 +381,20 @@ __global__ __launch_bounds__(256, HDP * (int)sizeof(T) < 192 ? 2 : 1) void cross
     }
 }
 
+// adds the key splits of dQ in order: thread = 4 channels of one (sample, head, query)
+template <typename T>
+__global__ __launch_bounds__(256) void cross_dqsum_kernel(const CrossParams p) {
+  const long rows = (long)p.B * p.H * p.Nq, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= rows * p.hd) return;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < p.qsplit; ++k) s += *reinterpret_cast<const f32x4*>(p.qpart + k * rows * p.hd + i);
+  const long row = i / p.hd, bh = row / p.Nq, b = bh / p.H;
+  const int col = (int)(i - row * p.hd), h = (int)(bh - b * p.H);
+  store4<T>(p.dq + (b * p.Nq + (row - bh * p.Nq)) * p.lddq + (h * p.hd + col) * (long)sizeof(T), s[0] * p.scale, s[1] * p.scale,
+            s[2] * p.scale, s[3] * p.scale);
+}
+
 // adds the shares of dK / dV in order: thread = 4 channels of one key
 template <typename T>
 __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p) {
@@ -354,6 +402,7 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p) {
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= 2 * n) return;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int k = 0; k < p.nsplit; ++k) {
     const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + (long)k * 2 * n + i);
 #pragma unroll
@@ -367,48 +416,69 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p) {
 
 constexpr int LDS_IMAGE = 80 * 1024;
 
-struct BwdPlan { int kb, iters, nqb, nsplit; bool res; long delta_bytes, ws; };
+struct BwdPlan { int kb, iters, nqb, wk, qsplit, qksplit, nsplit; bool res; long delta_bytes, part_bytes, ws; };
 int row_bytes(const dm_cross_args* a) { return cross_hdp(a->hd) * (a->dtype == 0 ? 2 : 4) + 16; }
 BwdPlan bwd_plan(const dm_cross_args* a) {
   BwdPlan f{};
-  const long groups = ((long)a->Nq + 127) / 128, blocks = groups * a->B * a->heads;
   const int image = (LDS_IMAGE - 64) / (2 * row_bytes(a) + 5) / 64 * 64;
-  const int need = (a->Nk + 63) & ~63;
+  f.wk = cross_wk(a);
+  const long groups = ((long)a->Nq + 127) / 128, blocks = cross_groups(a) * a->B * a->heads;
+  // dQ with few rows: the keys are split as in the forward (B=1, 3 heads of 40, 10 queries on 1031 states, fp32, forward and
+  // backward: 155 us without)
+  long qs = 1;
+  if (blocks < 512 && a->Nk >= 256) {
+    qs = (1024 + blocks - 1) / blocks;
+    if (qs > a->Nk / 128) qs = a->Nk / 128;
+  }
+  if (f.wk > 1 && (long)a->Nk > qs * image) qs = ((long)a->Nk + image - 1) / image;
+  if (qs > MAX_SPLITS) qs = MAX_SPLITS;
+  f.qksplit = qs > 1 ? (int)((((long)a->Nk + qs - 1) / qs + 63) & ~63L) : a->Nk;
+  f.qsplit = qs > 1 ? (a->Nk + f.qksplit - 1) / f.qksplit : 1;
+  const int need = (f.qksplit + 63) & ~63;
   f.res = need <= image;
+  if (!f.res) f.wk = 1;
   f.kb = need > 0 ? need : 64;
   f.iters = 1;
-  if (f.res) {
-    long it = blocks / 512;
+  if (f.res && f.wk == 1) {
+    long it = blocks * f.qsplit / 512;
     if (it > 8) it = 8;
     if (it > groups) it = groups;
     f.iters = it < 1 ? 1 : (int)it;
   }
-  f.nqb = (int)((groups + f.iters - 1) / f.iters);
-  f.iters = (int)((groups + f.nqb - 1) / f.nqb);
+  f.nqb = f.wk > 1 ? 1 : (int)((groups + f.iters - 1) / f.iters);
+  f.iters = f.wk > 1 ? 1 : (int)((groups + f.nqb - 1) / f.nqb);
   f.delta_bytes = (((long)a->B * a->heads * a->Nq + 3) & ~3L) * 4;
-  // shares of a context's query list: two workgroups per CU, at least four blocks of queries each
+  // shares of a context's query list: two workgroups per CU, at least two blocks of queries each
   const long owners = (long)a->Bc * a->kv_heads * ((a->Nk + 127) / 128);
   const long list = (long)((a->B + a->Bc - 1) / a->Bc) * (a->heads / a->kv_heads) * ((a->Nq + QS - 1) / QS);
   long ns = owners > 0 ? 512 / owners : 1;
-  if (ns > list / 4) ns = list / 4;
+  if (ns > list / 2) ns = list / 2;
   f.nsplit = ns < 1 ? 1 : (int)ns;
-  f.ws = f.delta_bytes + (f.nsplit > 1 ? (long)f.nsplit * 2 * a->Bc * a->Nk * a->kv_heads * a->hd * 4 : 0);
+  f.part_bytes = f.nsplit > 1 ? (long)f.nsplit * 2 * a->Bc * a->Nk * a->kv_heads * a->hd * 4 : 0;
+  f.ws = f.delta_bytes + f.part_bytes + (f.qsplit > 1 ? (long)f.qsplit * a->B * a->heads * a->Nq * a->hd * 4 : 0);
   return f;
 }
 
-template <typename T, int HDP, bool RES, bool DROP>
+template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 int launch_dq(const CrossParams& p, hipStream_t st) {
-  auto kern = cross_dq_kernel<T, HDP, RES, DROP>;
+  auto kern = cross_dq_kernel<T, HDP, RES, SPLIT, DROP>;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
                           RES ? LDS_IMAGE : 2 * image_bytes<T, HDP>()) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = RES ? (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
-  const long blocks = (long)p.B * p.nqb * p.H;
+  size_t lds = RES ? (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
+  if (SPLIT && lds < 4 * 32 * (HDP + 4) * 4) lds = 4 * 32 * (HDP + 4) * 4;
+  const long blocks = (long)p.B * p.qsplit * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
+  if (p.qsplit > 1) {
+    const long n = (long)p.B * p.H * p.Nq * (p.hd >> 2), jb = (n + 255) / 256;
+    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((cross_dqsum_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
+    DM_LAUNCH_CHECK();
+  }
   return DM_OK;
 }
 template <typename T, int HDP, bool DROP>
@@ -433,7 +503,8 @@ int launch_dkv(const CrossParams& p, hipStream_t st) {
   return DM_OK;
 }
 template <typename T, int HDP, bool DROP> int run_bwd(const CrossParams& p, bool res, hipStream_t st) {
-  const int rc = res ? launch_dq<T, HDP, true, DROP>(p, st) : launch_dq<T, HDP, false, DROP>(p, st);
+  const int rc = !res ? launch_dq<T, HDP, false, false, DROP>(p, st)
+                      : (p.wk > 1 ? launch_dq<T, HDP, true, true, DROP>(p, st) : launch_dq<T, HDP, true, false, DROP>(p, st));
   if (rc != DM_OK) return rc;
   static const DmVariantName nm("cross_bwd<%s,%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP);
   dm_set_variant(nm.s);
@@ -473,8 +544,9 @@ extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
   }
   const BwdPlan f = bwd_plan(a);
   DM_REQUIRE(a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0);
-  p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb; p.nsplit = f.nsplit;
+  p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb; p.nsplit = f.nsplit; p.wk = f.wk; p.qsplit = f.qsplit; p.qksplit = f.qksplit;
   p.delta = (float*)a->workspace;
   p.part = (float*)((char*)a->workspace + f.delta_bytes);
+  p.qpart = (float*)((char*)a->workspace + f.delta_bytes + f.part_bytes);
   return a->dtype == 0 ? pick_width<bf16>(p, f.res, (hipStream_t)stream) : pick_width<float>(p, f.res, (hipStream_t)stream);
 }

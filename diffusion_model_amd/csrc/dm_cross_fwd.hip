@@ -119,7 +119,7 @@ template <typename T, int HDP> constexpr int image_bytes() { return 64 * (Geo<T,
 
 // A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
 // LDS image, which is staged once for all the tiles; otherwise two images of 64 keys take turns (iters is 1).
-template <typename T, int HDP, bool RES, bool DROP>
+template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cross_fwd_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     load_frags<T, HDP>(rows_of(p.q + ((long)b * p.Nq + q) * p.ldq + h * hdb, p.ldq, p.Nq - q, hdb, lane), hdb, lane, nf);
   };
   auto begin = [&](int q) {
-    if (!AHEAD && RES) fetch(q);
+    if (!AHEAD && RES && !SPLIT) fetch(q);
 #pragma unroll
     for (int kc = 0; kc < Gm::NC; ++kc) qf[kc] = nf[kc];
     if (DROP) rs = dm_drop_row(seed, (uint32_t)(((long)b * p.H + h) * p.Nq + q + (lane & 31)));
@@ -170,6 +170,57 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
   };
 #define DM_STEP(NT, FIRST, t, from) \
   fwd_step<T, HDP, NT, FIRST, DROP>(p, st, sK, sV, bits, bias, t, (from) + (t) * 32, c, qf, rs, lane)
+  if (SPLIT) {
+    // one or two query tiles: the waves that share a tile take its keys' tiles in turn and join through LDS
+    const int WK = p.wk, wq = wave / WK, w = wave % WK, n = max(0, (k1 - k0 + 31) & ~31), tiles = n >> 5, q = wq * 32;
+    fetch(q);
+    stage(k0, n);
+    __syncthreads();
+    begin(q);
+    clear();
+    for (int t = w; t < tiles; t += WK) DM_STEP(1, false, t, k0);
+    const float l = half_sum(st.l);
+    __syncthreads();
+    constexpr int RS = HDP + 4;
+    float* o = reinterpret_cast<float*>(smem);
+    float* ml = o + 4 * 32 * RS;             // [wave][query] {maximum (base 2), sum}
+    put_rows<HDP>(o + wave * 32 * RS, st.acc, lane);
+    if (lane < 32) {
+      ml[(wave * 32 + lane) * 2] = st.m == -INFINITY ? -INFINITY : st.m * c;
+      ml[(wave * 32 + lane) * 2 + 1] = l;
+    }
+    __syncthreads();
+    const int per = p.hd >> 2;
+    const long rows = (long)p.B * p.H * p.Nq;
+    for (int i = tid; i < min(p.Nq, 128 / WK) * per; i += 256) {
+      const int qq = i / per, col = (i - qq * per) * 4, base = (qq >> 5) * WK, r = qq & 31;
+      float m = -INFINITY;
+      for (int k = 0; k < WK; ++k) m = fmaxf(m, ml[((base + k) * 32 + r) * 2]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < WK; ++k) {
+        const float f = __builtin_amdgcn_exp2f(ml[((base + k) * 32 + r) * 2] - ref);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(o + ((base + k) * 32 + r) * RS + col);
+        sum += f * ml[((base + k) * 32 + r) * 2 + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += f * a[j];
+      }
+      const long row = ((long)b * p.H + h) * p.Nq + qq;
+      if (p.nsplit > 1) {
+        *reinterpret_cast<f32x4*>(p.part + (split * rows + row) * p.hd + col) = f32x4{x[0], x[1], x[2], x[3]};
+        if (col == 0) {
+          float* at = p.part + p.nsplit * rows * p.hd + (split * rows + row) * 2;
+          at[0] = ref;
+          at[1] = sum;
+        }
+      } else {
+        const float inv = sum == 0.f ? 0.f : p.inv_keep * __builtin_amdgcn_rcpf(sum);
+        store4<T>(p.o + ((long)b * p.Nq + qq) * p.ldo + h * hdb + col * (int)sizeof(T), x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (col == 0) p.lse[row] = sum == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * CR_LN2;
+      }
+    }
+    return;
+  }
   const int q0 = qb * p.iters * 128 + wave * 32;
   if (AHEAD) fetch(q0);
   if (RES) {
@@ -239,60 +290,69 @@ int key_bytes(const dm_cross_args* a) {
   return 0;
 }
 
-struct FwdPlan { int nsplit, ksplit, kb, iters, nqb; bool res; long ws; };
+struct FwdPlan { int nsplit, ksplit, kb, iters, nqb, wk; bool res; long ws; };
 FwdPlan fwd_plan(const dm_cross_args* a) {
   FwdPlan f{};
-  const long groups = ((long)a->Nq + 127) / 128;              // workgroups along the queries at one tile per wave
+  const int kbytes = key_bytes(a);
+  const int image = (LDS_IMAGE - 64) / (kbytes + 5) / 64 * 64;     // keys per LDS image
+  f.wk = cross_wk(a);
+  const long groups = cross_groups(a);                        // workgroups along the queries at one tile per wave
   const long blocks = groups * a->B * a->heads;
-  // few rows: the keys are split (at least 128 each) until there are about four workgroups per CU
+  // few rows: the keys are split (at least 128 each) until there are about four workgroups per CU; with one or two query
+  // tiles also so that a split's keys fit one image
   long ns = 1;
   if (blocks < 512 && a->Nk >= 256) {
     ns = (1024 + blocks - 1) / blocks;
     if (ns > a->Nk / 128) ns = a->Nk / 128;
-    if (ns > MAX_SPLITS) ns = MAX_SPLITS;
   }
+  if (f.wk > 1 && (long)a->Nk > ns * image) ns = ((long)a->Nk + image - 1) / image;
+  if (ns > MAX_SPLITS) ns = MAX_SPLITS;
   f.ksplit = ns > 1 ? (int)((((long)a->Nk + ns - 1) / ns + 63) & ~63L) : a->Nk;
   f.nsplit = ns > 1 ? (a->Nk + f.ksplit - 1) / f.ksplit : 1;
-  const int kbytes = key_bytes(a);
-  const int image = (LDS_IMAGE - 64) / (kbytes + 5) / 64 * 64;     // keys per LDS image
   const int need = (f.ksplit + 63) & ~63;
   f.res = need <= image;
+  if (!f.res) f.wk = 1;                                       // (states beyond 64 images: streamed)
   f.kb = need > 0 ? need : 64;
   // resident keys serve several query tiles per wave, as long as there are two workgroups per CU (B=64, 8 heads of 32, 576
   // queries, 77 tokens: 13.5 us at two, 14.6 at six and more)
+  const long g1 = ((long)a->Nq + 127) / 128;
   f.iters = 1;
-  if (f.res) {
+  if (f.res && f.wk == 1) {
     long it = blocks * f.nsplit / 512;
     if (it > 8) it = 8;
-    if (it > groups) it = groups;
+    if (it > g1) it = g1;
     f.iters = it < 1 ? 1 : (int)it;
   }
-  f.nqb = (int)((groups + f.iters - 1) / f.iters);
-  f.iters = (int)((groups + f.nqb - 1) / f.nqb);              // (evenly)
+  f.nqb = f.wk > 1 ? 1 : (int)((g1 + f.iters - 1) / f.iters);
+  f.iters = f.wk > 1 ? 1 : (int)((g1 + f.nqb - 1) / f.nqb);   // (evenly)
   f.ws = f.nsplit > 1 ? (long)f.nsplit * a->B * a->heads * a->Nq * (a->hd + 2) * 4 : 0;
   return f;
 }
 
-template <typename T, int HDP, bool RES, bool DROP>
+template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 int launch_fwd(const CrossParams& p, hipStream_t st) {
-  auto kern = cross_fwd_kernel<T, HDP, RES, DROP>;
+  auto kern = cross_fwd_kernel<T, HDP, RES, SPLIT, DROP>;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
                           RES ? LDS_IMAGE : 2 * image_bytes<T, HDP>()) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const size_t lds = RES ? (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
+  size_t lds = RES ? (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
+  if (SPLIT && lds < 4 * 32 * ((HDP + 4) * 4 + 8)) lds = 4 * 32 * ((HDP + 4) * 4 + 8);
   const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-  static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, RES ? "resident" : "streamed");
+  static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, SPLIT ? "split" : (RES ? "resident" : "streamed"));
   dm_set_variant(nm.s);
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   return p.nsplit > 1 ? join_launch(p, sizeof(T) == 2 ? 0 : 1, st) : DM_OK;
 }
+template <typename T, int HDP, bool RES, bool SPLIT> int pick_drop(const CrossParams& p, hipStream_t st) {
+  return p.thresh ? launch_fwd<T, HDP, RES, SPLIT, true>(p, st) : launch_fwd<T, HDP, RES, SPLIT, false>(p, st);
+}
 template <typename T, int HDP> int pick_fwd(const CrossParams& p, bool res, hipStream_t st) {
-  if (res) return p.thresh ? launch_fwd<T, HDP, true, true>(p, st) : launch_fwd<T, HDP, true, false>(p, st);
-  return p.thresh ? launch_fwd<T, HDP, false, true>(p, st) : launch_fwd<T, HDP, false, false>(p, st);
+  if (!res) return pick_drop<T, HDP, false, false>(p, st);
+  return p.wk > 1 ? pick_drop<T, HDP, true, true>(p, st) : pick_drop<T, HDP, true, false>(p, st);
 }
 template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t st) {
   switch (cross_hdp(p.hd)) {
@@ -326,7 +386,7 @@ extern "C" int dm_cross_fwd(const dm_cross_args* a, dm_stream_t stream) {
   }
   const FwdPlan f = fwd_plan(a);
   DM_REQUIRE(f.ws == 0 || (a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0));
-  p.nsplit = f.nsplit; p.ksplit = f.ksplit; p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb;
+  p.nsplit = f.nsplit; p.ksplit = f.ksplit; p.kb = f.kb; p.iters = f.iters; p.nqb = f.nqb; p.wk = f.wk;
   p.part = (float*)a->workspace;
   return a->dtype == 0 ? pick_width<bf16>(p, f.res, (hipStream_t)stream) : pick_width<float>(p, f.res, (hipStream_t)stream);
 }

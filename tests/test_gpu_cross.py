@@ -150,6 +150,9 @@ CASES = [
     (66, 2, 9, 20, 2, 1, 16, "ragged", True, True),          # more samples than one wave scans at a time
     (5, 1, 40, 33, 2, 2, 8, None, False, False),             # one context for all
     (2, 2, 17, 600, 2, 2, 128, "ragged", True, False),       # more keys than one image holds
+    (2, 2, 64, 1500, 2, 1, 128, "ragged", True, False),      # two query tiles, two waves each
+    (1, 1, 200, 900, 1, 1, 128, "ragged", False, False),     # streamed keys, split
+    (1, 1, 20, 9000, 1, 1, 128, None, False, False),         # more keys than 64 images hold
 ]
 
 
@@ -267,12 +270,12 @@ def test_cross_nan_in_a_valid_state_reaches_only_its_sample():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("hd,Nk", [(128, 100), (64, 50)])
-def test_cross_dropout(hd, Nk, dtype):
+@pytest.mark.parametrize("hd,Nk,Nq", [(128, 100, 150), (64, 50, 150), (128, 100, 20), (64, 30, 40), (32, 20, 1)])
+def test_cross_dropout(hd, Nk, Nq, dtype):
     """The keep mask is read off with unit values (o = P Z / keep), is a fair draw, and the same seed then gives the
     forward and the backward of exactly that mask."""
     kn = K()
-    B, Nq, H, p = 2, 150, 2, 0.25
+    B, H, p = 2, 2, 0.25
     q, k, v, d_o, L, _, _ = inputs(dtype, B, B, Nq, Nk, H, H, hd, "ragged", False, False, seed=9)
     L[:] = Nk
     eye = torch.zeros(B, Nk, H, hd)
