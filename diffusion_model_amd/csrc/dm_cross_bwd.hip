@@ -395,19 +395,24 @@ __global__ __launch_bounds__(256) void cross_dqsum_kernel(const CrossParams p) {
             s[2] * p.scale, s[3] * p.scale);
 }
 
-// adds the shares of dK / dV in order: thread = 4 channels of one key
-template <typename T>
+// Adds the shares of dK / dV: SL lanes split the list of one result (4 channels of one key) and join by a fixed tree, 8 for
+// long lists, 1 for short ones.
+template <typename T, int SL>
 __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p) {
+  constexpr int RPW = 64 / SL;
+  const int lane = threadIdx.x & 63, slice = lane / RPW;
   const long n = (long)p.Bc * p.Nk * p.G * p.hd;
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= 2 * n) return;
+  const long r = (((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + lane % RPW) * 4, i = r < 2 * n ? r : 0;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int k = 0; k < p.nsplit; ++k) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + (long)k * 2 * n + i);
+  for (int k = slice; k < p.nsplit; k += SL) s += *reinterpret_cast<const f32x4*>(p.part + (long)k * 2 * n + i);
+  if (SL > 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] += a[j];
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int o = RPW; o < 64; o <<= 1) s[j] += __shfl_xor(s[j], o, 64);
   }
+  if (r >= 2 * n || slice) return;
   const bool is_v = i >= n;
   const long e = is_v ? i - n : i, w = (long)p.G * p.hd, row = e / w, col = e - row * w;
   const float f = is_v ? 1.f : p.scale;
@@ -426,8 +431,8 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   // dQ with few rows: the keys are split as in the forward (B=1, 3 heads of 40, 10 queries on 1031 states, fp32, forward and
   // backward: 155 us without)
   long qs = 1;
-  if (blocks < 512 && a->Nk >= 256) {
-    qs = (1024 + blocks - 1) / blocks;
+  if (blocks < 256 && a->Nk >= 256) {
+    qs = (512 + blocks - 1) / blocks;
     if (qs > a->Nk / 128) qs = a->Nk / 128;
   }
   if (f.wk > 1 && (long)a->Nk > qs * image) qs = ((long)a->Nk + image - 1) / image;
@@ -495,9 +500,12 @@ int launch_dkv(const CrossParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    const long n = (long)2 * p.Bc * p.Nk * p.G * (p.hd >> 2), jb = (n + 255) / 256;
+    const long n = (long)2 * p.Bc * p.Nk * p.G * (p.hd >> 2);
+    const bool wide = p.nsplit > 8;
+    const long jb = (n + (wide ? 31 : 255)) / (wide ? 32 : 256);
     if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((cross_sum_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
+    if (wide) hipLaunchKernelGGL((cross_sum_kernel<T, 8>), dim3((unsigned)jb), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((cross_sum_kernel<T, 1>), dim3((unsigned)jb), dim3(256), 0, st, p);
     DM_LAUNCH_CHECK();
   }
   return DM_OK;

@@ -289,12 +289,12 @@ __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) 
   constexpr int RPW = 64 / SL;                             // results per wave
   const int lane = threadIdx.x & 63, slice = lane / RPW;
   const int per = p.hd >> 2, HG = p.H / p.G, U = HG * p.nqb;
-  const long n = (long)p.Bc * p.G * 2 * p.Nk * per;        // results, context slowest
-  const long i = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + lane % RPW;
+  const long n = (long)p.G * 2 * p.Nk * per;               // results of a context; p.iters workgroups share one
+  const int ctx = blockIdx.x / p.iters;
+  const long i = ((long)(blockIdx.x % p.iters) * 4 + (threadIdx.x >> 6)) * RPW + lane % RPW;
   const long r = i < n ? i : n - 1;
-  const long gw = r / per, kw = gw / p.Nk, cg = kw >> 1;
-  const int col = (int)(r - gw * per) * 4, key = (int)(gw - kw * p.Nk), which = (int)(kw & 1);
-  const int g = (int)(cg % p.G), ctx = (int)(cg / p.G);
+  const long gw = r / per, kw = gw / p.Nk;
+  const int col = (int)(r - gw * per) * 4, key = (int)(gw - kw * p.Nk), which = (int)(kw & 1), g = (int)(kw >> 1);
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   int m = 0;
   auto add = [&](int b) {
@@ -308,8 +308,10 @@ __global__ __launch_bounds__(256) void cross_gather_kernel(const CrossParams p) 
     if (p.Bc == 1) for (int b = 0; b < p.B; ++b) add(b);
     else add(ctx);
   } else {
-    for (int b = 0; b < p.B; ++b)
-      if (p.index[b] == ctx) add(b);
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      unsigned long long hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
+      for (; hit; hit &= hit - 1) add(b0 + __builtin_ctzll(hit));
+    }
   }
   if (SL > 1) {
 #pragma unroll
@@ -340,12 +342,14 @@ int launch(const CrossParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   if (p.nsplit) {
-    const long n = (long)p.Bc * p.G * 2 * p.Nk * (p.hd >> 2);
+    const long n = (long)p.G * 2 * p.Nk * (p.hd >> 2);
     const bool wide = (long)((p.B + p.Bc - 1) / p.Bc) * (p.H / p.G) * p.nqb > 4;
-    const long gb = (n + (wide ? 31 : 255)) / (wide ? 32 : 256);
+    CrossParams g = p;
+    g.iters = (int)((n + (wide ? 31 : 255)) / (wide ? 32 : 256));
+    const long gb = (long)p.Bc * g.iters;
     if (gb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-    if (wide) hipLaunchKernelGGL((cross_gather_kernel<T, 8>), dim3((unsigned)gb), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((cross_gather_kernel<T, 1>), dim3((unsigned)gb), dim3(256), 0, st, p);
+    if (wide) hipLaunchKernelGGL((cross_gather_kernel<T, 8>), dim3((unsigned)gb), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((cross_gather_kernel<T, 1>), dim3((unsigned)gb), dim3(256), 0, st, g);
     DM_LAUNCH_CHECK();
   }
   return DM_OK;

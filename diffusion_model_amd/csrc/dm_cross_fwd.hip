@@ -298,11 +298,11 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   f.wk = cross_wk(a);
   const long groups = cross_groups(a);                        // workgroups along the queries at one tile per wave
   const long blocks = groups * a->B * a->heads;
-  // few rows: the keys are split (at least 128 each) until there are about four workgroups per CU; with one or two query
-  // tiles also so that a split's keys fit one image
+  // fewer workgroups than CUs: the keys are split (at least 128 each) until there are two per CU (at 336 workgroups the join
+  // cost more than the split gave); with one or two query tiles also so that a split's keys fit one image
   long ns = 1;
-  if (blocks < 512 && a->Nk >= 256) {
-    ns = (1024 + blocks - 1) / blocks;
+  if (blocks < 256 && a->Nk >= 256) {
+    ns = (512 + blocks - 1) / blocks;
     if (ns > a->Nk / 128) ns = a->Nk / 128;
   }
   if (f.wk > 1 && (long)a->Nk > ns * image) ns = ((long)a->Nk + image - 1) / image;
