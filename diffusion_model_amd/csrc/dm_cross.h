@@ -156,7 +156,7 @@ template <typename T, int HDP, int N> struct Stager {
   static constexpr int PPR = Geo<T, HDP>::PPR, RPS = 256 / PPR;            // pieces per row, rows per step of the workgroup
   static constexpr int U = (N + RPS - 1) / RPS;
   u32x4 a[U], b[U];
-  uint32_t ok;
+  unsigned char keep[U];      // mask bytes, looked at only when the rows are put down
   __device__ __forceinline__ void load(const char* srcA, long ldA, const char* srcB, long ldB, int r0, int valid,
                                        const unsigned char* mask, int hdb, int tid) {
     const int r = tid / PPR, pc = tid % PPR, left = min(valid - r0, N);
@@ -181,13 +181,9 @@ template <typename T, int HDP, int N> struct Stager {
         b[u] = in ? *reinterpret_cast<const u32x4*>(srcB + (r0 + r + u * RPS) * ldB + pc * 16) : u32x4{0u, 0u, 0u, 0u};
       }
     }
-    ok = 0xFFFFFFFFu;
     if (mask) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int row = r0 + u * RPS + r;
-        ok = row < valid && mask[row] ? ok : ok & ~(1u << u);
-      }
+      for (int u = 0; u < U; ++u) keep[u] = mask[min(r0 + u * RPS + r, valid - 1)];
     }
   }
   // n <= N: rows that the image has room for
@@ -195,13 +191,26 @@ template <typename T, int HDP, int N> struct Stager {
     const int r = tid / PPR, pc = tid % PPR;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (masked && !(ok >> u & 1u)) { a[u] = u32x4{0u, 0u, 0u, 0u}; b[u] = a[u]; }
+      if (masked && keep[u] == 0) { a[u] = u32x4{0u, 0u, 0u, 0u}; b[u] = a[u]; }
       if (r >= RPS || r + u * RPS >= n) break;
       *reinterpret_cast<u32x4*>(dstA + (r + u * RPS) * strideA + pc * 16) = a[u];
       *reinterpret_cast<u32x4*>(dstB + (r + u * RPS) * strideB + pc * 16) = b[u];
     }
   }
 };
+// Orders a run of MFMAs that read one operand fragment each from LDS: AHEAD fragments (after `lead` other LDS reads) are on
+// their way before the first MFMA, then one is asked for per MFMA.  Left alone the compiler reads two and waits for both,
+// which shows the LDS latency once per two MFMAs.
+template <typename T, int N, int LEAD, int AHEAD = 4> __device__ __forceinline__ void feed_mfma() {
+  constexpr int M = sizeof(T) == 2 ? 1 : 4;               // MFMAs per fragment
+  __builtin_amdgcn_sched_group_barrier(0x100, LEAD + (N < AHEAD ? N : AHEAD), 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, M * (N < AHEAD ? N : AHEAD), 0);
+}
 // rows [r0, r0 + n) of a resident image
 template <typename T, int HDP>
 __device__ __forceinline__ void stage_rows2(char* dstA, int strideA, const char* srcA, long ldA, char* dstB, int strideB,
@@ -209,9 +218,10 @@ __device__ __forceinline__ void stage_rows2(char* dstA, int strideA, const char*
                                             int hdb, int tid) {
   constexpr int N = Geo<T, HDP>::RB >= 512 ? 64 : 128;      // (at most 16 pieces in flight per thread)
   for (int at = 0; at < n; at += N) {
+    const unsigned char* m = r0 + at < valid ? mask : nullptr;      // (rows past the end are zero anyway)
     Stager<T, HDP, N> st;
-    st.load(srcA, ldA, srcB, ldB, r0 + at, valid, mask, hdb, tid);
-    st.store(dstA + at * strideA, strideA, dstB + at * strideB, strideB, min(N, n - at), mask != nullptr, tid);
+    st.load(srcA, ldA, srcB, ldB, r0 + at, valid, m, hdb, tid);
+    st.store(dstA + at * strideA, strideA, dstB + at * strideB, strideB, min(N, n - at), m != nullptr, tid);
   }
 }
 // Validity of keys [r0, r0 + n): one word per 32 keys (empty tiles are skipped) and, per key, what its score starts from:
@@ -224,6 +234,20 @@ __device__ __forceinline__ void stage_valid(uint32_t* bits, float* bias, int r0,
     if ((tid & 63) == 0) { bits[i >> 5] = (uint32_t)w; bits[(i >> 5) + 1] = (uint32_t)(w >> 32); }
     if (i < n) bias[i] = ok ? 0.f : -INFINITY;
   }
+}
+// the same for an image of 64 keys that is asked for early and put down late (one wave's work)
+__device__ __forceinline__ bool load_valid(int r0, int valid, const unsigned char* mask, int tid, unsigned char& byte) {
+  const int key = r0 + (tid & 63);
+  byte = 1;
+  if (mask && tid < 64) byte = mask[min(key, valid - 1)];
+  return key < valid;
+}
+__device__ __forceinline__ void store_valid(uint32_t* bits, float* bias, bool in, unsigned char byte, int tid) {
+  if (tid >= 64) return;
+  const bool ok = in && byte != 0;
+  const unsigned long long w = __ballot(ok);
+  bias[tid] = ok ? 0.f : -INFINITY;
+  if (tid == 0) { bits[0] = (uint32_t)w; bits[1] = (uint32_t)(w >> 32); }
 }
 // start of a score tile whose rows are the 32 keys of `bias`
 __device__ __forceinline__ f32x16 score_init(const float* bias, int half) {

@@ -151,10 +151,15 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     }
   } else {
     Stager<T, HDP, 64> next;
-    auto load = [&](int from) { next.load(kbase, p.ldk, vbase, p.ldv, from, kn, mask, hdb, tid); };
-    auto store = [&](int from) {
+    bool in = false;
+    unsigned char byte = 1;
+    auto load = [&](int from) {
+      next.load(kbase, p.ldk, vbase, p.ldv, from, kn, mask, hdb, tid);
+      in = load_valid(from, kn, mask, tid, byte);
+    };
+    auto store = [&]() {
       next.store(sK, Gm::SR, sV, Gm::SR, 64, mask != nullptr, tid);
-      stage_valid(bits, bias, from, 64, kn, mask, tid);
+      store_valid(bits, bias, in, byte, tid);
     };
     char* const image = smem;
     auto use = [&](int i) {
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     if (k0 < kn) load(k0);
     begin(q0);
     use(0);
-    if (k0 < kn) store(k0);
+    if (k0 < kn) store();
     __syncthreads();
     for (int from = k0, i = 0; from < kn; from += 64, ++i) {
       const bool more = from + 64 < kn;
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
       use(i);
       sweep(from, 2, 0, 1);
       use(i + 1);
-      if (more) store(from + 64);
+      if (more) store();
       __syncthreads();
     }
     finish(q0);

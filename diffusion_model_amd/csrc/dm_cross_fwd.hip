@@ -35,6 +35,7 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
     for (int kc = 0; kc < Gm::NC; ++kc)
       s[t] = Cr<T>::mma(row_frag<T>(sK + (t0 + t) * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s[t]);
   }
+  feed_mfma<T, NT * Gm::NC, NT * 4>();
   float mx = s[0][0];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -247,10 +248,15 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
   } else {
     // two images of 64 keys in turn: the next one's rows fly while the present one is used
     Stager<T, HDP, 64> next;
-    auto load = [&](int from) { next.load(kbase, p.ldk, vbase, p.ldv, from, k1, mask, hdb, tid); };
-    auto store = [&](int from) {
+    bool in = false;
+    unsigned char byte = 1;
+    auto load = [&](int from) {
+      next.load(kbase, p.ldk, vbase, p.ldv, from, k1, mask, hdb, tid);
+      in = load_valid(from, k1, mask, tid, byte);
+    };
+    auto store = [&]() {
       next.store(sK, Gm::SR, sV, Gm::ST, 64, mask != nullptr, tid);
-      stage_valid(bits, bias, from, 64, k1, mask, tid);
+      store_valid(bits, bias, in, byte, tid);
     };
     char* const image = smem;
     auto use = [&](int i) {
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     begin(q0);
     clear();
     use(0);
-    if (k0 < k1) store(k0);
+    if (k0 < k1) store();
     __syncthreads();
     for (int from = k0, i = 0; from < k1; from += 64, ++i) {
       const bool more = from + 64 < k1;
@@ -272,7 +278,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
       use(i);
       DM_STEP(2, false, 0, from);
       use(i + 1);
-      if (more) store(from + 64);
+      if (more) store();
       __syncthreads();
     }
     fwd_finish<T, HDP>(p, st, b, h, q0, split, c, lane);
