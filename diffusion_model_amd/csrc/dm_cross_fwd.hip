@@ -16,7 +16,8 @@ template <typename T, int HDP> struct FwdState {
 
 // NT tiles of 32 keys (LDS rows t0..) against the wave's 32 queries.  FIRST: the state is not read but begun, with the
 // maximum of these tiles, so nothing is cleared or rescaled (up to 96 keys need no other step).
-template <typename T, int HDP, int NT, bool FIRST, bool DROP>
+// HALF: the last tile has at most 16 keys, which are the lower halves of the registers; the upper ones are left out.
+template <typename T, int HDP, int NT, bool FIRST, bool HALF, bool DROP>
 __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>& st, const char* sK, const char* sV,
                                          const uint32_t* bits, const float* bias, int t0, int key0, float c,
                                          const typename Cr<T>::frag (&qf)[Geo<T, HDP>::NC], uint32_t rs, int lane) {
@@ -40,7 +41,7 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+    for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) mx = fmaxf(mx, s[t][i]);
   mx = half_max(mx);
   if (FIRST) {
     st.m = mx;
@@ -63,20 +64,20 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) {
       s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -mc));
       st.l += s[t][i];
     }
     if (DROP) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
+      for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); i += 2) {
         const uint32_t key = key0 + t * 32 + tile_row(i, half), z = dm_drop_bits(rs, key >> 1);
         if (!dm_keep16(z, 0, p.thresh)) s[t][i] = 0.f;
         if (!dm_keep16(z, 1, p.thresh)) s[t][i + 1] = 0.f;
       }
     }
 #pragma unroll
-    for (int f = 0; f < Cr<T>::NF; ++f) {
+    for (int f = 0; f < (HALF && t == NT - 1 ? Cr<T>::NF / 2 : Cr<T>::NF); ++f) {
       const typename Cr<T>::frag pf = Cr<T>::pack(s[t], f);
 #pragma unroll
       for (int d = 0; d < Gm::DT; ++d)
@@ -121,7 +122,7 @@ template <typename T, int HDP> constexpr int image_bytes() { return 64 * (Geo<T,
 // A workgroup: 4 waves x p.iters tiles of 32 queries of one (sample, head, key split).  RES: the keys of the split fit one
 // LDS image, which is staged once for all the tiles; otherwise two images of 64 keys take turns (iters is 1).
 template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
-__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cross_fwd_kernel(const CrossParams p) {
+__global__ __launch_bounds__(256, (HDP * (int)sizeof(T) <= 64 ? 4 : (HDP * (int)sizeof(T) < 384 ? 2 : 1))) void cross_fwd_kernel(const CrossParams p) {
   typedef Geo<T, HDP> Gm;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* sK = smem;
@@ -169,8 +170,9 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     stage_rows2<T, HDP>(sK, Gm::SR, kbase, p.ldk, sV, Gm::ST, vbase, p.ldv, from, n, k1, mask, hdb, tid);
     stage_valid(bits, bias, from, n, k1, mask, tid);
   };
-#define DM_STEP(NT, FIRST, t, from) \
-  fwd_step<T, HDP, NT, FIRST, DROP>(p, st, sK, sV, bits, bias, t, (from) + (t) * 32, c, qf, rs, lane)
+#define DM_STEP(NT, FIRST, t, from) DM_STEP_H(NT, FIRST, false, t, from)
+#define DM_STEP_H(NT, FIRST, HALF, t, from) \
+  fwd_step<T, HDP, NT, FIRST, HALF, DROP>(p, st, sK, sV, bits, bias, t, (from) + (t) * 32, c, qf, rs, lane)
   if (SPLIT) {
     // one or two query tiles: the waves that share a tile take its keys' tiles in turn and join through LDS
     const int WK = p.wk, wq = wave / WK, w = wave % WK, n = max(0, (k1 - k0 + 31) & ~31), tiles = n >> 5, q = wq * 32;
@@ -226,25 +228,32 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
   if (AHEAD) fetch(q0);
   if (RES) {
     const int n = max(0, (k1 - k0 + 31) & ~31), tiles = n >> 5;
+    const bool half = n - (k1 - k0) >= 16;
     stage(k0, n);
     __syncthreads();
-    for (int it = 0; it < p.iters; ++it) {
-      const int q = q0 + it * 128;
-      if (q >= p.Nq) break;                    // (wave-uniform)
-      begin(q);
-      if (AHEAD && it + 1 < p.iters) fetch(q + 128);      // the next tile's queries fly while this one is computed
-      int t = 2;
-      if (tiles == 0) clear();
-      else if (tiles == 1) DM_STEP(1, true, 0, k0);
-      else if (tiles & 1) {
-        if (HDP <= 64) DM_STEP(3, true, 0, k0);
-        else { DM_STEP(2, true, 0, k0); DM_STEP(1, false, 2, k0); }
-        t = 3;
+    // one loop for each number of tiles, so that each keeps only its own LDS addresses in registers
+    auto each = [&](auto step) {
+      for (int it = 0; it < p.iters; ++it) {
+        const int q = q0 + it * 128;
+        if (q >= p.Nq) break;                    // (wave-uniform)
+        begin(q);
+        if (AHEAD && it + 1 < p.iters) fetch(q + 128);      // the next tile's queries fly while this one is computed
+        step();
+        fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
       }
-      else DM_STEP(2, true, 0, k0);
-      for (; t < tiles; t += 2) DM_STEP(2, false, t, k0);
-      fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
-    }
+    };
+    if (tiles == 0) each([&]() { clear(); });
+    else if (tiles == 1 && half) each([&]() { DM_STEP_H(1, true, true, 0, k0); });
+    else if (tiles == 1) each([&]() { DM_STEP(1, true, 0, k0); });
+    else if (tiles == 2 && half) each([&]() { DM_STEP_H(2, true, true, 0, k0); });
+    else if (tiles == 3 && half && HDP <= 64) each([&]() { DM_STEP_H(3, true, true, 0, k0); });
+    else if (tiles == 3 && HDP <= 64) each([&]() { DM_STEP(3, true, 0, k0); });
+    else each([&]() {
+      int t = 2;
+      DM_STEP(2, true, 0, k0);
+      for (; t + 2 <= tiles; t += 2) DM_STEP(2, false, t, k0);
+      if (t < tiles) DM_STEP(1, false, t, k0);
+    });
   } else {
     // two images of 64 keys in turn: the next one's rows fly while the present one is used
     Stager<T, HDP, 64> next;
@@ -284,6 +293,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) < 384 ? 2 : 1)) void cro
     fwd_finish<T, HDP>(p, st, b, h, q0, split, c, lane);
   }
 #undef DM_STEP
+#undef DM_STEP_H
 }
 
 constexpr int LDS_IMAGE = 80 * 1024;     // two workgroups per CU
