@@ -77,15 +77,17 @@ template <> struct KvAcc<bf16, 16> {
   }
 };
 
-template <typename T> __device__ __forceinline__ void put_tile(char* patch, const f32x16& s, int lane) {
+// N of the tile's 32 rows (keys)
+template <typename T, int N> __device__ __forceinline__ void put_tile(char* patch, const f32x16& s, int lane) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < N / 8; ++i)
     store4<T>(patch + (lane & 31) * patch_stride<T>() + (8 * i + 4 * (lane >> 5)) * (int)sizeof(T), s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
 }
 
 // NT tiles of 32 keys against the wave's 32 queries: dk, dv += ..., dq = ... .  All tiles go through each stage together, so
-// that one tile's exponentials run beside the next one's matrix instructions.
-template <typename T, int HDP, int KT, int NT, bool DROP, typename Next>
+// that one tile's exponentials run beside the next one's matrix instructions.  HALF: the last tile has at most 16 keys; what
+// its other columns of dk and dv become is nothing that is kept.
+template <typename T, int HDP, int KT, int NT, bool HALF, bool DROP, typename Next>
 __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, const char* sV, const float* bias, const char* sQ,
                                          const char* sD, char* patch, const typename Cr<T>::frag (&qf)[Geo<T, HDP>::NC],
                                          const typename Cr<T>::frag (&df)[Geo<T, HDP>::NC], float lse2, float c, uint32_t rs,
@@ -114,7 +116,7 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
     if (DROP) {
       keep[t] = 0;
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
+      for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); i += 2) {
         const uint32_t z = dm_drop_bits(rs, (uint32_t)(t * 32 + tile_row(i, half)) >> 1);
         const bool k0 = dm_keep16(z, 0, p.thresh), k1 = dm_keep16(z, 1, p.thresh);
         keep[t] |= (k0 ? 1u : 0u) << i | (k1 ? 2u : 0u) << i;
@@ -123,7 +125,7 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
       }
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) {
       pr[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(pr[t][i], c, -lse2));
       delta = __builtin_fmaf(pr[t][i], dp[t][i], delta);
     }
@@ -133,16 +135,16 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dp[t][i] = pr[t][i] * (dp[t][i] - delta);
+    for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) dp[t][i] = pr[t][i] * (dp[t][i] - delta);
     if (DROP) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
+      for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
     }
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
+    for (int f = 0; f < (HALF && t == NT - 1 ? NF / 2 : NF); ++f) {
       const frag sf = Cr<T>::pack(dp[t], f);
 #pragma unroll
       for (int d = 0; d < Gm::DT; ++d)
@@ -153,8 +155,14 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
   for (int t0 = 0; t0 < NT; t0 += PT) {
 #pragma unroll
     for (int t = t0; t < NT && t < t0 + PT; ++t) {
-      put_tile<T>(patch + 2 * (t - t0) * 32 * PS, pr[t], lane);
-      put_tile<T>(patch + (2 * (t - t0) + 1) * 32 * PS, dp[t], lane);
+      constexpr int ALL = 32, SOME = 16;
+      if (HALF && t == NT - 1) {
+        put_tile<T, SOME>(patch + 2 * (t - t0) * 32 * PS, pr[t], lane);
+        put_tile<T, SOME>(patch + (2 * (t - t0) + 1) * 32 * PS, dp[t], lane);
+      } else {
+        put_tile<T, ALL>(patch + 2 * (t - t0) * 32 * PS, pr[t], lane);
+        put_tile<T, ALL>(patch + (2 * (t - t0) + 1) * 32 * PS, dp[t], lane);
+      }
     }
     wave_lds_order();
 #pragma unroll
@@ -214,40 +222,54 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
   stage_valid(bits, bias, 0, KT * 32, kn, mask, tid);
   __syncthreads();
   int tiles = 0;       // up to the last one with a valid key
+  bool some = false;   // which has none past its first 16
 #pragma unroll
-  for (int t = 0; t < KT; ++t) tiles = __builtin_amdgcn_readfirstlane((int)bits[t]) ? t + 1 : tiles;
+  for (int t = 0; t < KT; ++t) {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)bits[t]);
+    if (w) { tiles = t + 1; some = (w >> 16) == 0; }
+  }
   KvAcc<T, HDP> dk[KT], dv[KT];
 #pragma unroll
   for (int t = 0; t < KT; ++t) { dk[t].clear(); dv[t].clear(); }
 
-  for (int unit = first; unit < units; unit += 4) {
-    const int hh = HEADS ? unit / tiles_q : 0, hq = h0 + hh, q0 = (unit - hh * tiles_q) * 32;
-    const long row = ((long)b * p.H + hq) * p.Nq;
-    // a query past the end, and one without a finite score, has no probabilities
-    const float lse2 = L2 == -INFINITY || q0 + (lane & 31) >= p.Nq ? INFINITY : L2 * CR_LOG2E;
+  // one loop for each number of tiles, so that each keeps only its own LDS addresses in registers
+  auto each = [&](auto step) {
+    for (int unit = first; unit < units; unit += 4) {
+      const int hh = HEADS ? unit / tiles_q : 0, hq = h0 + hh, q0 = (unit - hh * tiles_q) * 32;
+      const long row = ((long)b * p.H + hq) * p.Nq;
+      // a query past the end, and one without a finite score, has no probabilities
+      const float lse2 = L2 == -INFINITY || q0 + (lane & 31) >= p.Nq ? INFINITY : L2 * CR_LOG2E;
 #pragma unroll
-    for (int kc = 0; kc < Gm::NC; ++kc) {
-      *reinterpret_cast<frag*>(sQ + (lane & 31) * Gm::ST + kc * 32 + half * 16) = qf[kc];
-      *reinterpret_cast<frag*>(sD + (lane & 31) * Gm::ST + kc * 32 + half * 16) = df[kc];
+      for (int kc = 0; kc < Gm::NC; ++kc) {
+        *reinterpret_cast<frag*>(sQ + (lane & 31) * Gm::ST + kc * 32 + half * 16) = qf[kc];
+        *reinterpret_cast<frag*>(sD + (lane & 31) * Gm::ST + kc * 32 + half * 16) = df[kc];
+      }
+      const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q0 + (lane & 31))) : 0u;
+      f32x16 dq[Gm::DT];
+      wave_lds_order();
+      step(lse2, rs, dq, [&]() { if (unit + 4 < units) fetch(unit + 4); });
+      const Rows dst = rows_of(p.dq + (tok + q0) * p.lddq + hq * hdb, p.lddq, p.Nq - q0, hdb, lane);
+#pragma unroll
+      for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, hdb, lane);
     }
-    const uint32_t rs = DROP ? dm_drop_row(seed, (uint32_t)(row + q0 + (lane & 31))) : 0u;
-    f32x16 dq[Gm::DT];
-    auto next = [&]() { if (unit + 4 < units) fetch(unit + 4); };
-    wave_lds_order();
-#define DM_FEW(NT) \
-  few_step<T, HDP, KT, NT, DROP>(p, sK, sV, bias, sQ, sD, patch, qf, df, lse2, c, rs, dk, dv, dq, lane, next)
-    if (KT > 2 && tiles > 2) DM_FEW((KT > 2 ? 3 : 1));
-    else if (KT > 1 && tiles > 1) DM_FEW((KT > 1 ? 2 : 1));
-    else if (tiles > 0) DM_FEW(1);
-    else {
+  };
+#define DM_FEW(NT, HALF) each([&](float lse2, uint32_t rs, f32x16 (&dq)[Gm::DT], const auto& next) { \
+    few_step<T, HDP, KT, NT, HALF, DROP>(p, sK, sV, bias, sQ, sD, patch, qf, df, lse2, c, rs, dk, dv, dq, lane, next); })
+  if (tiles == 0) {
+    each([&](float, uint32_t, f32x16 (&dq)[Gm::DT], const auto&) {
 #pragma unroll
       for (int d = 0; d < Gm::DT; ++d) dq[d] = zero16();
-    }
-#undef DM_FEW
-    const Rows dst = rows_of(p.dq + (tok + q0) * p.lddq + hq * hdb, p.lddq, p.Nq - q0, hdb, lane);
-#pragma unroll
-    for (int d = 0; d < Gm::DT; ++d) store_tile<T>(dst, dq[d], p.scale, d * 32, hdb, lane);
+    });
+  } else if (tiles == 1) {
+    if (some) DM_FEW(1, true); else DM_FEW(1, false);
+  } else if (KT > 1 && tiles == 2) {
+    constexpr int N2 = KT > 1 ? 2 : 1;
+    if (some) DM_FEW(N2, true); else DM_FEW(N2, false);
+  } else if (KT > 2) {
+    constexpr int N3 = KT > 2 ? 3 : 1;
+    if (some) DM_FEW(N3, true); else DM_FEW(N3, false);
   }
+#undef DM_FEW
 
   // dK, dV of the four waves, added in wave order: [dk | dv][key][channel]
   constexpr int RS = HDP + 4;
@@ -271,7 +293,8 @@ __global__ __launch_bounds__(256, (few_waves<T, HDP, KT>())) void cross_few_kern
   const int per = p.hd >> 2, n = p.Nk * per;
   for (int i = tid; i < 2 * n; i += 256) {
     const int which = i >= n, e = which ? i - n : i, key = e / per, col = (e - key * per) * 4;
-    const f32x4 v = *reinterpret_cast<const f32x4*>(sum + (which * KT * 32 + key) * RS + col);
+    const bool counts = key < kn && (!mask || mask[key]);
+    const f32x4 v = counts ? *reinterpret_cast<const f32x4*>(sum + (which * KT * 32 + key) * RS + col) : f32x4{0.f, 0.f, 0.f, 0.f};
     if (p.nsplit) {
       *reinterpret_cast<f32x4*>(p.part + ((((long)b * p.H + h0) * p.nqb + qb) * 2 + which) * p.Nk * p.hd + (long)key * p.hd + col) = v;
     } else {
