@@ -198,19 +198,6 @@ template <typename T, int HDP, int N> struct Stager {
     }
   }
 };
-// Orders a run of MFMAs that read one operand fragment each from LDS: AHEAD fragments (after `lead` other LDS reads) are on
-// their way before the first MFMA, then one is asked for per MFMA.  Left alone the compiler reads two and waits for both,
-// which shows the LDS latency once per two MFMAs.
-template <typename T, int N, int LEAD, int AHEAD = 4> __device__ __forceinline__ void feed_mfma() {
-  constexpr int M = sizeof(T) == 2 ? 1 : 4;               // MFMAs per fragment
-  __builtin_amdgcn_sched_group_barrier(0x100, LEAD + (N < AHEAD ? N : AHEAD), 0);
-#pragma unroll
-  for (int i = 0; i < N - AHEAD; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, M * (N < AHEAD ? N : AHEAD), 0);
-}
 // rows [r0, r0 + n) of a resident image
 template <typename T, int HDP>
 __device__ __forceinline__ void stage_rows2(char* dstA, int strideA, const char* srcA, long ldA, char* dstB, int strideB,
@@ -356,6 +343,23 @@ inline int cross_hdp(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64
 inline int cross_wk(const dm_cross_args* a) { return a->Nq <= 32 ? 4 : (a->Nq <= 64 ? 2 : 1); }
 inline long cross_groups(const dm_cross_args* a) { const long per = 32 * (4 / cross_wk(a)); return (a->Nq + per - 1) / per; }
 
+// Key splits in units of workgroups.  With one or two query tiles the keys of a split also fit one image (`image` keys), as
+// long as the splits' partial results (`row` bytes per query and head) stay below 1 GiB; beyond, or past MAX_SPLITS images,
+// the keys are streamed by workgroups of one wave per query tile.
+constexpr int MAX_SPLITS = 64;
+inline long cross_splits(const dm_cross_args* a, long blocks, int image, long row) {
+  long ns = 1;
+  if (blocks < 256 && a->Nk >= 256) {
+    ns = (512 + blocks - 1) / blocks;
+    if (ns > a->Nk / 128) ns = a->Nk / 128;
+  }
+  if (cross_wk(a) > 1 && (long)a->Nk > ns * image) {
+    const long fit = ((long)a->Nk + image - 1) / image;
+    if (fit <= MAX_SPLITS && (double)fit * a->B * a->heads * a->Nq * row <= (double)(1L << 30)) ns = fit;
+  }
+  return ns < MAX_SPLITS ? ns : MAX_SPLITS;
+}
+
 inline bool cross_sizes_ok(const dm_cross_args* a) {
   return a && a->B > 0 && a->Bc > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->Nq > 0 &&
          a->Nk >= 0 && a->hd >= 8 && a->hd <= 128 && a->hd % 8 == 0 && (a->dtype == 0 || a->dtype == 1) &&
@@ -403,6 +407,5 @@ struct OnePlan { int nsplit, ksplit; long ws; };
 bool one_plan(const dm_cross_args* a, OnePlan& f);          // false: too many rows share a key / value head
 int one_launch(const CrossParams& p, int dtype, hipStream_t st);
 int join_launch(const CrossParams& p, int dtype, hipStream_t st);      // joins the key splits of either forward
-constexpr int MAX_SPLITS = 64;
 
 }  // namespace dm_cross

@@ -435,13 +435,7 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   const long groups = ((long)a->Nq + 127) / 128, blocks = cross_groups(a) * a->B * a->heads;
   // dQ with few rows: the keys are split as in the forward (B=1, 3 heads of 40, 10 queries on 1031 states, fp32, forward and
   // backward: 155 us without)
-  long qs = 1;
-  if (blocks < 256 && a->Nk >= 256) {
-    qs = (512 + blocks - 1) / blocks;
-    if (qs > a->Nk / 128) qs = a->Nk / 128;
-  }
-  if (f.wk > 1 && (long)a->Nk > qs * image) qs = ((long)a->Nk + image - 1) / image;
-  if (qs > MAX_SPLITS) qs = MAX_SPLITS;
+  const long qs = cross_splits(a, blocks, image, a->hd * 4L);
   f.qksplit = qs > 1 ? (int)((((long)a->Nk + qs - 1) / qs + 63) & ~63L) : a->Nk;
   f.qsplit = qs > 1 ? (a->Nk + f.qksplit - 1) / f.qksplit : 1;
   const int need = (f.qksplit + 63) & ~63;

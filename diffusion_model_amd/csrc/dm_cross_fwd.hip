@@ -36,7 +36,6 @@ __device__ __forceinline__ void fwd_step(const CrossParams& p, FwdState<T, HDP>&
     for (int kc = 0; kc < Gm::NC; ++kc)
       s[t] = Cr<T>::mma(row_frag<T>(sK + (t0 + t) * 32 * Gm::SR, Gm::SR, kc, lane), qf[kc], s[t]);
   }
-  feed_mfma<T, NT * Gm::NC, NT * 4>();
   float mx = s[0][0];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -315,19 +314,13 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   const long groups = cross_groups(a);                        // workgroups along the queries at one tile per wave
   const long blocks = groups * a->B * a->heads;
   // fewer workgroups than CUs: the keys are split (at least 128 each) until there are two per CU (at 336 workgroups the join
-  // cost more than the split gave); with one or two query tiles also so that a split's keys fit one image
-  long ns = 1;
-  if (blocks < 256 && a->Nk >= 256) {
-    ns = (512 + blocks - 1) / blocks;
-    if (ns > a->Nk / 128) ns = a->Nk / 128;
-  }
-  if (f.wk > 1 && (long)a->Nk > ns * image) ns = ((long)a->Nk + image - 1) / image;
-  if (ns > MAX_SPLITS) ns = MAX_SPLITS;
+  // cost more than the split gave)
+  const long ns = cross_splits(a, blocks, image, (a->hd + 2) * 4L);
   f.ksplit = ns > 1 ? (int)((((long)a->Nk + ns - 1) / ns + 63) & ~63L) : a->Nk;
   f.nsplit = ns > 1 ? (a->Nk + f.ksplit - 1) / f.ksplit : 1;
   const int need = (f.ksplit + 63) & ~63;
   f.res = need <= image;
-  if (!f.res) f.wk = 1;                                       // (states beyond 64 images: streamed)
+  if (!f.res) f.wk = 1;
   f.kb = need > 0 ? need : 64;
   // resident keys serve several query tiles per wave, as long as there are two workgroups per CU (B=64, 8 heads of 32, 576
   // queries, 77 tokens: 13.5 us at two, 14.6 at six and more)

@@ -113,6 +113,8 @@ def test_cross_workspace_bytes():
     shared.workspace = None
     assert L.dm_cross_bwd(ctypes.byref(shared), None) == -1
     assert L.dm_cross_fwd_workspace_bytes(None) == 0 and L.dm_cross_fwd(None, None) == -1 and L.dm_cross_bwd(None, None) == -1
+    crowd = cross_struct(B=4096, Bc=1, Nq=64, Nk=16384)                        # the partial results of key splits stay below 1 GiB
+    assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(crowd)) < 1 << 30
     few = cross_struct(Nq=1, Nk=4096, workspace=None)
     assert L.dm_cross_fwd(ctypes.byref(few), None) == -1
 
