@@ -91,8 +91,9 @@ class CFGSampler:
     in the loop: under data parallelism every rank samples its own shard of the labels.
 
     ``context_table``: [ids, D], or [ids, L, D] with several tokens per id.  For the latter, ``context_lens`` [ids] and
-    ``context_mask`` [ids, L] say which tokens count; the table is then handed over whole with each sample's id as its
-    context, so keys and values are computed once per id instead of once per sample (UNET.forward)."""
+    ``context_mask`` [ids, L] say which tokens count; a table of no more rows than the batch is then handed over whole
+    with each sample's id as its context, so keys and values are computed once per id instead of once per sample
+    (UNET.forward), and a larger one is gathered."""
 
     def __init__(self, model, scheduler, context_table: torch.Tensor, uncond_id: int, context_lens=None, context_mask=None):
         if (context_lens is not None or context_mask is not None) and context_table.dim() != 3:
@@ -108,7 +109,13 @@ class CFGSampler:
         if self.context_lens is None and self.context_mask is None:
             return (table[ids].contiguous(),)
         from .unet import ContextMap
-        return table.contiguous(), ContextMap.of(ids.device, self.context_lens, self.context_mask, ids)
+        if bool(((ids < 0) | (ids >= table.shape[0])).any()):
+            raise IndexError(f"CFGSampler: a context id is outside the table of {table.shape[0]}")
+        cmap = ContextMap.of(ids.device, self.context_lens, self.context_mask, ids)
+        if table.shape[0] <= ids.shape[0]:
+            return table.contiguous(), cmap
+        pick = [None if x is None else x[ids].contiguous() for x in (cmap.lens, cmap.mask)]
+        return table[ids].contiguous(), ContextMap(*pick)
 
     @torch.no_grad()
     def sample(self, z: torch.Tensor, labels: torch.Tensor, guidance_scale=6.0, eta: float = 1.0,

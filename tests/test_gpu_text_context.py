@@ -252,3 +252,23 @@ def test_sampling_from_a_table_of_token_contexts():
     assert_close(full, plain, 2e-2, "all tokens")
     with pytest.raises(ValueError):
         CFGSampler(m, sched, table[:, 0], 3, context_lens=lens)
+
+
+def test_sampling_from_a_table_larger_than_the_batch():
+    """Rows of the table that no sample uses change nothing, and an id without a row is refused."""
+    from diffusion_model_amd.sampler import CFGSampler
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    m, _ = network(False)
+    sched = DDPM_beta_t_cosine_scheduler(500)
+    g = torch.Generator().manual_seed(9)
+    table, lens = torch.randn(9, 7, KW["context_dim"], generator=g).to(dev()), torch.tensor([7, 3, 5, 1, 2, 7, 6, 4, 0])
+    mask = torch.rand(9, 7, generator=g) < 0.7
+    z = torch.randn(2, 3, 16, 16, generator=g).to(dev())
+    kw = dict(guidance_scale=3.0, eta=0.0, t_stop=497)
+    a = CFGSampler(m, sched, table, 8, context_lens=lens, context_mask=mask).sample(z, torch.tensor([1, 5]), **kw)
+    used = [1, 5, 8]
+    b = CFGSampler(m, sched, table[used], 2, context_lens=lens[used], context_mask=mask[used]).sample(z, torch.tensor([0, 1]), **kw)
+    assert torch.equal(a, b)
+    for bad in (9, -1):
+        with pytest.raises(IndexError):
+            CFGSampler(m, sched, table, 8, context_lens=lens).sample(z, torch.tensor([1, bad]), **kw)
