@@ -861,9 +861,11 @@ def _rows16(what, name, t, esize):
     return ptr, ld
 
 
-def _cross_out(what, name, t, like):
+def _cross_out(what, name, t, like, *inputs):
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if t.numel() and t.data_ptr() in [x.data_ptr() for x in inputs]:
+        raise ValueError(f"{what}: {name} must not be one of the operands")
     if t.shape != like.shape or t.dtype != like.dtype:
         raise ValueError(f"{what}: {name} must have the shape {tuple(like.shape)} and the operands' type")
     _same_device(what, t)
@@ -877,9 +879,10 @@ def cross_fwd(q, k, v, heads: int, *, kv_heads: Optional[int] = None, lens=None,
     ``lens`` int32 [Bc]: the first lens[c] states of context c are valid; ``mask`` bool [Bc, Nk]: True where valid (both:
     their intersection); what invalid states hold does not matter, and a sample without any valid state gets o = 0 and
     lse = -inf.  ``index`` int32 [B]: the context of each sample (without it: one each, or Bc == 1 for all); an index
-    outside [0, Bc) means no states.  ``kv_heads``: key / value heads, each shared by heads / kv_heads query heads."""
+    outside [0, Bc) means no states.  ``kv_heads``: key / value heads, each shared by heads / kv_heads query heads.
+    ``out``, a view with rows like q's if given, shares no memory with the operands."""
     B, Bc, kv_heads, Nq, Nk, hd, scale = _cross_check("cross_fwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p)
-    out = _cross_out("cross_fwd", "out", out, q)
+    out = _cross_out("cross_fwd", "out", out, q, q, k, v)
     lse = torch.empty((B, heads, Nq), dtype=F32, device=q.device)
     if B == 0 or Nq == 0:
         return out, lse
@@ -902,15 +905,17 @@ def cross_fwd(q, k, v, heads: int, *, kv_heads: Optional[int] = None, lens=None,
 def cross_bwd(q, k, v, o, lse, d_o, heads: int, *, kv_heads: Optional[int] = None, lens=None, mask=None, index=None,
               scale: Optional[float] = None, drop_p: float = 0.0, drop_seed: int = 0, dq=None, dk=None, dv=None):
     """Backward of cross_fwd with the same options: (dq, dk, dv) in q's, k's and v's shapes.  dk and dv are sums over the
-    query heads of a group and over the samples that share a context, in a fixed order; rows of invalid states are zero."""
+    query heads of a group and over the samples that share a context, in a fixed order; rows of invalid states are zero.
+    Given ``dq``, ``dk``, ``dv`` share no memory with the operands or with one another."""
     B, Bc, kv_heads, Nq, Nk, hd, scale = _cross_check("cross_bwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p)
     if o.shape != q.shape or d_o.shape != q.shape or o.dtype != q.dtype or d_o.dtype != q.dtype:
         raise ValueError("cross_bwd: o and d_o must have q's shape and type")
     if lse.shape != (B, heads, Nq) or lse.dtype != F32 or not lse.is_contiguous():
         raise ValueError("cross_bwd: lse must be cross_fwd's")
     _same_device("cross_bwd", o, d_o, lse)
-    dq = _cross_out("cross_bwd", "dq", dq, q)
-    dk, dv = _cross_out("cross_bwd", "dk", dk, k), _cross_out("cross_bwd", "dv", dv, v)
+    read = (q, k, v, o, d_o)
+    dq = _cross_out("cross_bwd", "dq", dq, q, *read)
+    dk, dv = _cross_out("cross_bwd", "dk", dk, k, *read), _cross_out("cross_bwd", "dv", dv, v, *read)
     if B == 0 or Nq == 0:
         return dq, dk.zero_(), dv.zero_()
     f32m = q.dtype == F32

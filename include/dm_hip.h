@@ -241,8 +241,8 @@ long dm_cross1_bwd_workspace_bytes(int B, int heads, int C);
  *   - key j of context c is valid iff j < lens[c] (NULL: Nk; values are clamped to [0, Nk]) and mask[c][j] != 0 (NULL: all).
  *     What invalid rows of k and v hold does not matter (NaN and infinities included).
  *   - a query with no valid key: o = 0, lse = -infinity, and no gradient flows.
- * hd: a multiple of 8 up to 128.  Rows of every activation are 16-byte aligned and less than 64 MiB apart.  Scores, softmax statistics and accumulators
- * are fp32; with dtype 0 the probabilities (and in the backward the score gradients) are rounded to bf16 for the second
+ * hd: a multiple of 8 up to 128.  Rows of every activation are 16-byte aligned and less than 64 MiB apart, and no output
+ * shares memory with an input or another output.  Scores, softmax statistics and accumulators are fp32; with dtype 0 the probabilities (and in the backward the score gradients) are rounded to bf16 for the second
  * matrix product, like the inputs.  Dropout words as dm_attn_fwd's for 64- and 128-wide heads. */
 typedef struct dm_cross_args {
   const void* q; long ldq;        /* [B, Nq, heads*hd] */
@@ -271,7 +271,7 @@ int dm_cross_bwd(const dm_cross_args* args, dm_stream_t stream);
  * Rotary embedding with up to three position axes on every head of x [B, N, heads*hd] (an image or video's query / key
  * projection before dm_attn_fwd, reference unet.py:119-126, which has no positions): pair p turns by
  * position[axis[p]] * freq[p] TURNS (freq = theta^(-2i/d) / (2 pi), doubles); channels >= rot are copied.  Angles are reduced
- * in 64 bits.  inverse: the opposite angle, which is the backward.  y may be x itself. */
+ * in 64 bits.  inverse: the opposite angle, which is the backward.  y may be x itself, but not overlap it otherwise. */
 typedef struct dm_rope_args {
   const void* x; long ldx;        /* [B*N] rows of heads*hd */
   void* y; long ldy;

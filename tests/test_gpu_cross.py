@@ -387,3 +387,15 @@ def test_cross_states_past_32_bits():
     check("o", o, val, tol)
     for name, t in zip(("dq", "dk", "dv"), kn.cross_bwd(qd, kd, vd, o, lse, dd, 1, dk=base[..., 128:160], dv=base[..., 192:224])):
         check(name, t, val, tol)
+
+
+def test_cross_refuses_outputs_that_are_operands():
+    q, k, v = (torch.zeros(2, n, 32, dtype=BF16, device="cuda") for n in (5, 7, 7))
+    for t in (q, k, v):
+        if t.shape == q.shape:
+            with pytest.raises(ValueError):
+                K().cross_fwd(q, k, v, 2, out=t)
+    o, lse = K().cross_fwd(q, k, v, 2)
+    for kw in (dict(dq=q), dict(dq=o), dict(dk=k), dict(dk=v), dict(dv=v)):
+        with pytest.raises(ValueError):
+            K().cross_bwd(q, k, v, o, lse, torch.zeros_like(q), 2, **kw)
