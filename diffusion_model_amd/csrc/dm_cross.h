@@ -336,6 +336,64 @@ __device__ __forceinline__ void put_rows(float* rows, const f32x16 (&acc)[DT], i
           f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
 }
 
+// ---------------------------------------------------------------- single queries: 16-byte pieces of a row on LPR lanes
+template <typename T> __device__ __forceinline__ void widen(u32x4 w, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {      // bf16 -> fp32: the upper half of the word
+      const unsigned lo = w[j] << 16, hi = w[j] & 0xFFFF0000u;
+      f[2 * j] = __builtin_bit_cast(float, lo);
+      f[2 * j + 1] = __builtin_bit_cast(float, hi);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned x = w[j];
+      f[j] = __builtin_bit_cast(float, x);
+    }
+  }
+}
+
+// sum over the LPR lanes of a row, in every one of them: lane exchanges inside the adds (rows of 16 lanes), no LDS
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
+template <int LPR> __device__ __forceinline__ float row_sum(float x) {
+  if (LPR > 1) x = dpp_add<0xB1>(x);       // neighbours
+  if (LPR > 2) x = dpp_add<0x4E>(x);       // pairs
+  if (LPR > 4) x = dpp_add<0x141>(x);      // mirrored in 8
+  if (LPR > 8) x = dpp_add<0x140>(x);      // mirrored in 16
+  if (LPR > 16) x += __shfl_xor(x, 16, 64);
+  return x;
+}
+
+// The samples that use a context, in order: every step is wave- and workgroup-uniform.
+struct Samples {
+  int b0, b;                  // next sample to look at (a scan position in the index), the present one
+  unsigned long long hit;     // samples of the scanned 64 that use the context
+  int ctx;
+  bool done;
+  __device__ __forceinline__ void first(const CrossParams& p, int c, int lane) {
+    ctx = c; b0 = 0; b = 0; hit = 0; done = false;
+    sample(p, lane);
+  }
+  __device__ __forceinline__ bool sample(const CrossParams& p, int lane) {
+    if (!p.index) {
+      if (p.Bc != 1) { b = ctx; done = b0 > 0; b0 = 1; }
+      else { b = b0++; done = b >= p.B; }
+      return !done;
+    }
+    while (!hit) {
+      if (b0 >= p.B) { done = true; return false; }
+      hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
+      b0 += 64;
+    }
+    b = b0 - 64 + __builtin_ctzll(hit);
+    hit &= hit - 1;
+    return true;
+  }
+};
+
 // ---------------------------------------------------------------- host side
 inline int cross_hdp(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 96 ? 96 : 128))); }
 
@@ -407,5 +465,11 @@ struct OnePlan { int nsplit, ksplit; long ws; };
 bool one_plan(const dm_cross_args* a, OnePlan& f);          // false: too many rows share a key / value head
 int one_launch(const CrossParams& p, int dtype, hipStream_t st);
 int join_launch(const CrossParams& p, int dtype, hipStream_t st);      // joins the key splits of either forward
+
+// ---------------------------------------------------------------- the backward of single queries (dm_cross_onebwd.hip)
+struct OneBwdPlan { int tiles; long ws; };
+bool onebwd_plan(const dm_cross_args* a, OneBwdPlan& f);    // false: too many rows share a key / value head
+int onebwd_launch(const CrossParams& p, int dtype, hipStream_t st);
+int dqsum_launch(const CrossParams& p, int dtype, hipStream_t st);     // adds the p.qsplit partials of dQ
 
 }  // namespace dm_cross

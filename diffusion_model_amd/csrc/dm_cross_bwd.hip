@@ -196,28 +196,9 @@ constexpr int QS = 64;
 // one image: 64 queries, their output gradients, and per query the log-sum-exp (base 2), delta and the dropout word
 template <typename T, int HDP> constexpr int list_bytes() { return QS * (2 * Geo<T, HDP>::SR + 12); }
 
-// walks the share's blocks of 64 queries: every next() is wave- and workgroup-uniform
-struct QueryList {
-  int b0, b;                  // next sample to look at (a scan position in the index), the present one
-  unsigned long long hit;     // samples of the scanned 64 that use the context
+// walks the share's blocks of 64 queries
+struct QueryList : Samples {
   uint32_t u, per;            // block of the present sample; blocks per sample
-  int ctx;
-  bool done;
-  __device__ __forceinline__ bool sample(const CrossParams& p, int lane) {
-    if (!p.index) {
-      if (p.Bc != 1) { b = ctx; done = b0 > 0; b0 = 1; }
-      else { b = b0++; done = b >= p.B; }
-      return !done;
-    }
-    while (!hit) {
-      if (b0 >= p.B) { done = true; return false; }
-      hit = __ballot(b0 + lane < p.B && p.index[min(b0 + lane, p.B - 1)] == ctx);
-      b0 += 64;
-    }
-    b = b0 - 64 + __builtin_ctzll(hit);
-    hit &= hit - 1;
-    return true;
-  }
   __device__ __forceinline__ void settle(const CrossParams& p, int lane) {
     while (!done && u >= per) {
       u -= per;
@@ -225,8 +206,8 @@ struct QueryList {
     }
   }
   __device__ __forceinline__ void start(const CrossParams& p, int c, uint32_t blocks, int share, int lane) {
-    ctx = c; per = blocks; u = (uint32_t)share; b0 = 0; b = 0; hit = 0; done = false;
-    sample(p, lane);
+    per = blocks; u = (uint32_t)share;
+    first(p, c, lane);
     settle(p, lane);
   }
   __device__ __forceinline__ void next(const CrossParams& p, int lane) {
@@ -386,20 +367,6 @@ __global__ __launch_bounds__(256, HDP * (int)sizeof(T) < 192 ? 2 : 1) void cross
     }
 }
 
-// adds the key splits of dQ in order: thread = 4 channels of one (sample, head, query)
-template <typename T>
-__global__ __launch_bounds__(256) void cross_dqsum_kernel(const CrossParams p) {
-  const long rows = (long)p.B * p.H * p.Nq, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= rows * p.hd) return;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int k = 0; k < p.qsplit; ++k) s += *reinterpret_cast<const f32x4*>(p.qpart + k * rows * p.hd + i);
-  const long row = i / p.hd, bh = row / p.Nq, b = bh / p.H;
-  const int col = (int)(i - row * p.hd), h = (int)(bh - b * p.H);
-  store4<T>(p.dq + (b * p.Nq + (row - bh * p.Nq)) * p.lddq + (h * p.hd + col) * (long)sizeof(T), s[0] * p.scale, s[1] * p.scale,
-            s[2] * p.scale, s[3] * p.scale);
-}
-
 // Adds the shares of dK / dV: SL lanes split the list of one result (4 channels of one key) and join by a fixed tree, 8 for
 // long lists, 1 for short ones.
 template <typename T, int SL>
@@ -477,13 +444,7 @@ int launch_dq(const CrossParams& p, hipStream_t st) {
   if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
-  if (p.qsplit > 1) {
-    const long n = (long)p.B * p.H * p.Nq * (p.hd >> 2), jb = (n + 255) / 256;
-    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((cross_dqsum_kernel<T>), dim3((unsigned)jb), dim3(256), 0, st, p);
-    DM_LAUNCH_CHECK();
-  }
-  return DM_OK;
+  return p.qsplit > 1 ? dqsum_launch(p, sizeof(T) == 2 ? 0 : 1, st) : DM_OK;
 }
 template <typename T, int HDP, bool DROP>
 int launch_dkv(const CrossParams& p, hipStream_t st) {
@@ -535,6 +496,8 @@ template <typename T> int pick_width(const CrossParams& p, bool res, hipStream_t
 extern "C" long dm_cross_bwd_workspace_bytes(const dm_cross_args* a) {
   if (!dm_cross::cross_sizes_ok(a)) return 0;
   dm_cross::FewPlan few;
+  dm_cross::OneBwdPlan one;
+  if (dm_cross::onebwd_plan(a, one)) return one.ws;
   return dm_cross::few_plan(a, few) ? few.ws : bwd_plan(a).ws;
 }
 
@@ -542,6 +505,13 @@ extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
   CrossParams p{};
   const int rc = cross_fill(p, a, true);
   if (rc != DM_OK) return rc;
+  OneBwdPlan one;
+  if (onebwd_plan(a, one)) {
+    DM_REQUIRE(one.ws == 0 || (a->workspace && a->ws_bytes >= one.ws && (uintptr_t)a->workspace % 16 == 0));
+    p.qsplit = one.tiles; p.nsplit = one.ws ? 1 : 0;
+    p.qpart = (float*)a->workspace;
+    return onebwd_launch(p, a->dtype, (hipStream_t)stream);
+  }
   FewPlan few;
   if (few_plan(a, few)) {
     DM_REQUIRE(few.ws == 0 || (a->workspace && a->ws_bytes >= few.ws && (uintptr_t)a->workspace % 16 == 0));

@@ -9,36 +9,6 @@ namespace {
 
 using namespace dm_cross;
 
-template <typename T> __device__ __forceinline__ void widen(u32x4 w, float (&f)[16 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {      // bf16 -> fp32: the upper half of the word
-      const unsigned lo = w[j] << 16, hi = w[j] & 0xFFFF0000u;
-      f[2 * j] = __builtin_bit_cast(float, lo);
-      f[2 * j + 1] = __builtin_bit_cast(float, hi);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned x = w[j];
-      f[j] = __builtin_bit_cast(float, x);
-    }
-  }
-}
-
-// sum over the LPR lanes of a row, in every one of them: lane exchanges inside the adds (rows of 16 lanes), no LDS
-template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
-  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
-}
-template <int LPR> __device__ __forceinline__ float row_sum(float x) {
-  if (LPR > 1) x = dpp_add<0xB1>(x);       // neighbours
-  if (LPR > 2) x = dpp_add<0x4E>(x);       // pairs
-  if (LPR > 4) x = dpp_add<0x141>(x);      // mirrored in 8
-  if (LPR > 8) x = dpp_add<0x140>(x);      // mirrored in 16
-  if (LPR > 16) x += __shfl_xor(x, 16, 64);
-  return x;
-}
-
 template <typename T, int LPR, int R>
 __global__ __launch_bounds__(256) void cross_one_kernel(const CrossParams p) {
   constexpr int E = 16 / (int)sizeof(T), RPS = 64 / LPR, U = 4;
@@ -232,13 +202,13 @@ template <typename T, int LPR> int pick_rows(const CrossParams& p, hipStream_t s
   return rows == 2 ? launch<T, LPR, 2>(p, st) : launch<T, LPR, 4>(p, st);
 }
 template <typename T> int pick_width(const CrossParams& p, hipStream_t st) {
+  constexpr int least = 8 * (int)sizeof(T) / 16;      // pieces of the narrowest head; the widest has 16 times as many
   const int pieces = p.hd * (int)sizeof(T) / 16;
-  if (pieces <= 1) return pick_rows<T, 1>(p, st);
-  if (pieces <= 2) return pick_rows<T, 2>(p, st);
-  if (pieces <= 4) return pick_rows<T, 4>(p, st);
-  if (pieces <= 8) return pick_rows<T, 8>(p, st);
-  if (pieces <= 16) return pick_rows<T, 16>(p, st);
-  return pick_rows<T, 32>(p, st);
+  if (pieces <= least) return pick_rows<T, least>(p, st);
+  if (pieces <= 2 * least) return pick_rows<T, 2 * least>(p, st);
+  if (pieces <= 4 * least) return pick_rows<T, 4 * least>(p, st);
+  if (pieces <= 8 * least) return pick_rows<T, 8 * least>(p, st);
+  return pick_rows<T, 16 * least>(p, st);
 }
 
 }  // namespace

@@ -399,3 +399,34 @@ def test_cross_refuses_outputs_that_are_operands():
     for kw in (dict(dq=q), dict(dq=o), dict(dk=k), dict(dk=v), dict(dv=v)):
         with pytest.raises(ValueError):
             K().cross_bwd(q, k, v, o, lse, torch.zeros_like(q), 2, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Bc,Nq,Nk,H,G,hd,lens,mask,index", [
+    (2, 2, 1, 700, 2, 2, 8, "empty", False, False),          # every lane layout: 1 to 32 lanes per row
+    (3, 3, 1, 700, 4, 2, 16, "ragged", True, False),
+    (3, 3, 5, 333, 3, 1, 24, "ragged", False, False),        # 15 rows
+    (2, 2, 4, 517, 4, 1, 40, None, True, False),             # 16 rows, the whole list at once
+    (4, 4, 2, 129, 2, 1, 64, "ragged", False, False),        # one state in the last tile
+    (2, 2, 1, 1300, 2, 1, 96, "empty", True, False),
+    (2, 2, 3, 401, 3, 3, 128, None, False, False),
+    (7, 1, 1, 150, 4, 2, 32, None, True, False),             # one context for all
+    (23, 4, 1, 260, 2, 1, 80, "ragged", True, True),         # a list of more than 16 rows for some, of none for others
+    (70, 9, 1, 64, 2, 2, 64, "empty", False, True),          # an index longer than a wave
+])
+def test_cross_short_row_lists(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, dtype):
+    kn = K()
+    q, k, v, d_o, L, M, I = inputs(dtype, B, Bc, Nq, Nk, H, G, hd, lens, mask, index, seed=Nk + hd)
+    if index:
+        I[1], I[B - 1] = -3, Bc                               # no context: no gradient, zeros in dq
+    val, tol = reference(q, k, v, H, G, L, M, I, d_o=d_o)
+    kp, vp = poison(k, v, L, M)
+    dq_, dk_, dv_, do_, dL, dM, dI = cuda(q, kp, vp, d_o, L, M, I)
+    kw = dict(kv_heads=G, lens=dL, mask=dM, index=dI)
+    o, lse = kn.cross_fwd(dq_, dk_, dv_, H, **kw)
+    first = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert kn.last_variant().startswith("cross_bwd_one")
+    for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *first)):
+        check(name, t, val, tol)
+    again = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
