@@ -12,6 +12,8 @@ namespace {
 using namespace dm_cross;
 
 constexpr int ROWS = 16;       // rows in LDS at a time
+// states in a lane's registers, in 32 bits with their gradients (two instead of four for wide heads: 49 us, not 40, for 8 rows
+// on 32 x 500 states, 8 heads of 64, bf16: what each row costs a wave is spread over fewer states)
 constexpr int states_per_lane(int lpr) { return lpr >= 8 ? 4 : (lpr == 4 ? 2 : 1); }
 constexpr int states_per_wg(int lpr) { return 4 * (64 / lpr) * states_per_lane(lpr); }
 
@@ -62,17 +64,18 @@ __global__ __launch_bounds__(256) void cross_onebwd_kernel(const CrossParams p) 
   const long krow = (long)ctx * p.Nk;
   const float c = p.scale * CR_LOG2E;
   const uint32_t seed = DROP ? dm_eff_seed(p.seed, p.seed_ctr) : 0u;
-  u32x4 kw[U], vw[U];
   bool ok[U];
-  float dk[U][E], dv[U][E];
+  float kf[U][E], vf[U][E], dk[U][E], dv[U][E];
   auto key_of = [&](int u) { return k0 + (wave * U + u) * RPS + group; };
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int key = key_of(u);
     ok[u] = key < kn && (!p.mask || p.mask[krow + key]);
     const bool get = ok[u] && mine;      // (what invalid states hold is not read)
-    kw[u] = get ? *reinterpret_cast<const u32x4*>(p.k + (krow + key) * p.ldk + g * hdb + piece * 16) : u32x4{0u, 0u, 0u, 0u};
-    vw[u] = get ? *reinterpret_cast<const u32x4*>(p.v + (krow + key) * p.ldv + g * hdb + piece * 16) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 kw = get ? *reinterpret_cast<const u32x4*>(p.k + (krow + key) * p.ldk + g * hdb + piece * 16) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 vw = get ? *reinterpret_cast<const u32x4*>(p.v + (krow + key) * p.ldv + g * hdb + piece * 16) : u32x4{0u, 0u, 0u, 0u};
+    widen<T>(kw, kf[u]);
+    widen<T>(vw, vf[u]);
 #pragma unroll
     for (int e = 0; e < E; ++e) dk[u][e] = dv[u][e] = 0.f;
   }
@@ -133,13 +136,11 @@ __global__ __launch_bounds__(256) void cross_onebwd_kernel(const CrossParams p) 
         for (int e = 0; e < E; ++e) dq[e] = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          float kf[E], vf[E], s = 0.f, dp = 0.f;
-          widen<T>(kw[u], kf);
-          widen<T>(vw[u], vf);
+          float s = 0.f, dp = 0.f;
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            s = __builtin_fmaf(qf[e], kf[e], s);
-            dp = __builtin_fmaf(df[e], vf[e], dp);
+            s = __builtin_fmaf(qf[e], kf[u][e], s);
+            dp = __builtin_fmaf(df[e], vf[u][e], dp);
           }
           s = row_sum<LPR>(s);
           dp = row_sum<LPR>(dp);
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(256) void cross_onebwd_kernel(const CrossParams p) 
           for (int e = 0; e < E; ++e) {
             dk[u][e] = __builtin_fmaf(ds, qf[e], dk[u][e]);
             dv[u][e] = __builtin_fmaf(pr, df[e], dv[u][e]);
-            dq[e] = __builtin_fmaf(ds, kf[e], dq[e]);
+            dq[e] = __builtin_fmaf(ds, kf[u][e], dq[e]);
           }
         }
         const int off = group_sum<LPR, E>(dq, lane);
@@ -262,9 +263,14 @@ template <typename T> int pick_width(const CrossParams& p, hipStream_t st) {
 namespace dm_cross {
 
 bool onebwd_plan(const dm_cross_args* a, OneBwdPlan& f) {
+  // rows per context, on average, up to which this beats the matrix tiles, whose time hardly depends on them (16 samples, 8
+  // heads of 128, 1000 states, backward: bf16 34 us here and 74 with tiles at 1 row, 56 and 76 at 6, 86 and 79 at 12; fp32 49
+  // and 194 at 1, 107 and 218 at 16; 32 samples, 8 heads of 32, 77 states: bf16 4.8 and 10.3 at 1, 9.0 and 10.5 at 6, fp32
+  // 4.8 and 17.3 at 1, 13.0 and 18.3 at 16)
+  const int e = a->dtype == 0 ? 2 : 4;
   const double rows = (double)a->B * (a->heads / a->kv_heads) * a->Nq;
-  if (a->Nk < 1 || rows > (double)ROWS * a->Bc) return false;
-  const int keys = states_per_wg(lanes_per_row(a->hd, a->dtype == 0 ? 2 : 4));
+  if (a->Nk < 1 || rows > (e == 2 ? 6.0 : 16.0) * a->Bc) return false;
+  const int keys = states_per_wg(lanes_per_row(a->hd, e));
   const long tiles = ((long)a->Nk + keys - 1) / keys;
   f.tiles = (int)tiles;
   // (with an index a sample may have no context, whose dQ the sum kernel writes)

@@ -110,9 +110,9 @@ def test_cross_workspace_bytes():
     assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct(Nk=600))) >= 2 * 2 * 5 * 4
     shared = cross_struct(B=3, Bc=1, Nq=9)                                     # few keys, one context for all: a partial per sample
     assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(shared)) == 3 * 2 * 2 * 7 * 32 * 4
-    one = cross_struct(B=3, Bc=1, Nk=300)                                      # few rows: a partial of dQ per 128 states
-    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(one)) == 3 * 3 * 2 * 5 * 32 * 4
-    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct(B=3, Bc=1))) == 0
+    one = cross_struct(B=3, Bc=1, Nq=2, Nk=300)                                      # few rows: a partial of dQ per 128 states
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(one)) == 3 * 3 * 2 * 2 * 32 * 4
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(cross_struct(B=3, Bc=1, Nq=2))) == 0
     shared.workspace = None
     assert L.dm_cross_bwd(ctypes.byref(shared), None) == -1
     assert L.dm_cross_fwd_workspace_bytes(None) == 0 and L.dm_cross_fwd(None, None) == -1 and L.dm_cross_bwd(None, None) == -1
