@@ -17,12 +17,12 @@ template <typename T> constexpr int patch_stride() { return sizeof(T) == 2 ? 72 
 // P / dS tile pairs that go through LDS together: all of them in bf16, one at a time in fp32 (twice the bytes, and bound by
 // its matrix instructions anyway)
 template <typename T, int KT> constexpr int pairs() { return sizeof(T) == 2 ? KT : 1; }
-// In bf16 the operands P and dS are rounded (half a step, 2^-8 of each value).  dS is a difference that the sums over few keys
-// do not even out, so for one tile of keys it goes in as two bf16 numbers, the value and what its rounding left: one more
-// matrix instruction per product where these are few.  With more tiles it would be a tenth of the kernel's work.
+// In bf16 the operands P and dS are rounded (half a step, 2^-8 of each value).  Sums over few queries or keys do not even that
+// out, so for one tile of keys both go in as two bf16 numbers, the value and what its rounding left: one more matrix
+// instruction per product where these are few.  With more tiles it would be a fifth of the kernel's work.
 template <typename T, int KT> constexpr bool two_terms() { return sizeof(T) == 2 && KT == 1; }
 template <typename T, int HDP, int KT> constexpr int wave_lds() {
-  return 2 * 32 * Geo<T, HDP>::ST + (pairs<T, KT>() * 2 + two_terms<T, KT>()) * 32 * patch_stride<T>();
+  return 2 * 32 * Geo<T, HDP>::ST + (pairs<T, KT>() + two_terms<T, KT>()) * 2 * 32 * patch_stride<T>();
 }
 template <typename T, int HDP, int KT> constexpr int few_lds() {
   const int keys = KT * 32 * (2 * Geo<T, HDP>::SR + 4) + 32, loop = keys + 4 * wave_lds<T, HDP, KT>();
@@ -145,10 +145,13 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
       for (int i = 0; i < (HALF && t == NT - 1 ? 8 : 16); ++i) pr[t][i] = keep[t] >> i & 1u ? pr[t][i] * p.inv_keep : 0.f;
     }
   }
-  f32x16 rest;         // of dS, where it has two terms (of its rows that hold no key: nothing that is kept)
+  f32x16 rest, prest;  // of dS and P, where they have two terms (of the rows that hold no key: nothing that is kept)
   if constexpr (two_terms<T, KT>()) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) rest[i] = dp[0][i] - (float)(T)dp[0][i];
+    for (int i = 0; i < 16; ++i) {
+      rest[i] = dp[0][i] - (float)(T)dp[0][i];
+      prest[i] = pr[0][i] - (float)(T)pr[0][i];
+    }
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -180,7 +183,10 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
         put_tile<T, ALL>(patch + (2 * (t - t0) + 1) * 32 * PS, dp[t], lane);
       }
     }
-    if constexpr (two_terms<T, KT>()) put_tile<T, HALF ? 16 : 32>(patch + 2 * 32 * PS, rest, lane);
+    if constexpr (two_terms<T, KT>()) {
+      put_tile<T, HALF ? 16 : 32>(patch + 2 * 32 * PS, prest, lane);
+      put_tile<T, HALF ? 16 : 32>(patch + 3 * 32 * PS, rest, lane);
+    }
     wave_lds_order();
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
@@ -188,7 +194,10 @@ __device__ __forceinline__ void few_step(const CrossParams& p, const char* sK, c
       for (int t = t0; t < NT && t < t0 + PT; ++t) {
         dv[t].add(sD, patch + 2 * (t - t0) * 32 * PS, f, lane);
         dk[t].add(sQ, patch + (2 * (t - t0) + 1) * 32 * PS, f, lane);
-        if constexpr (two_terms<T, KT>()) dk[t].add(sQ, patch + 2 * 32 * PS, f, lane);
+        if constexpr (two_terms<T, KT>()) {
+          dv[t].add(sD, patch + 2 * 32 * PS, f, lane);
+          dk[t].add(sQ, patch + 3 * 32 * PS, f, lane);
+        }
       }
       if (KT > 1 && HDP > 16) __builtin_amdgcn_sched_barrier(0);      // (all operand reads at once would not fit the registers)
     }
