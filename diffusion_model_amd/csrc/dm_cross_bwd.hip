@@ -3,7 +3,12 @@
 //   P = exp2(c S - lse log2(e)),  dP = dO V^T,  dS = P (dP - delta),  delta = sum_d dO * O,
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
 // dQ runs with the queries on the lanes (as the forward), dK / dV with the keys on the lanes; each probability tile is then
-// already the operand of the product that reduces over its rows.
+// already the operand of the product that reduces over its rows.  S and dP are computed in
+// both kernels, seven products in all: one kernel for both sides would have to add dQ up over its key blocks in memory, 4
+// bytes per channel and block.
+// The pipes (matrix, vector, LDS) are each about a third busy at two waves per SIMD; more waves, or two tiles at a time, were
+// not faster.  bf16, 16 x 1024 queries, 8 heads of 64 on 333 states (2 key / value heads, a tenth masked): dQ 36 us, dK and dV
+// 41 us; fp32, 8 key / value heads: 477 us together (82 TFLOP/s).
 #include "dm_cross.h"
 
 namespace {
@@ -400,8 +405,8 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   const int image = (LDS_IMAGE - 64) / (2 * row_bytes(a) + 5) / 64 * 64;
   f.wk = cross_wk(a);
   const long groups = ((long)a->Nq + 127) / 128, blocks = cross_groups(a) * a->B * a->heads;
-  // dQ with few rows: the keys are split as in the forward (B=1, 3 heads of 40, 10 queries on 1031 states, fp32, forward and
-  // backward: 155 us without)
+  // dQ with few rows: the keys are split as in the forward (B=1, 3 heads of 40, 40 queries on 1031 states, fp32, backward: 28
+  // us, 128 without)
   const long qs = cross_splits(a, blocks, image, a->hd * 4L);
   f.qksplit = qs > 1 ? (int)((((long)a->Nk + qs - 1) / qs + 63) & ~63L) : a->Nk;
   f.qsplit = qs > 1 ? (a->Nk + f.qksplit - 1) / f.qksplit : 1;

