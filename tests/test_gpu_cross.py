@@ -321,11 +321,10 @@ def test_cross_gradients_against_differences():
         assert abs(num - want) < 2e-3 * size + 1e-3, (i, num, want)
 
 
-@pytest.mark.parametrize("few", [False, True])
-def test_cross_captured_replays(few):
+@pytest.mark.parametrize("shape", [(4, 2, 200, 70, 4, 2, 32), (2, 2, 3, 900, 2, 2, 64), (2, 2, 20, 900, 2, 2, 64), (5, 2, 1, 400, 2, 2, 64)])
+def test_cross_captured_replays(shape):
     """Forward and backward in one HIP graph, replayed with other inputs and other lengths, eager calls in between."""
     kn = K()
-    shape = (2, 2, 3, 900, 2, 2, 64) if few else (4, 2, 200, 70, 4, 2, 32)
     B, Bc, Nq, Nk, H, G, hd = shape
     q, k, v, d_o, L, M, I = cuda(*inputs(BF16, *shape, "ragged", True, Bc != B))
     kw = dict(kv_heads=G, lens=L, mask=M, index=I)
@@ -350,10 +349,11 @@ def test_cross_captured_replays(few):
         assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
 
 
-def test_cross_two_streams_at_once():
+@pytest.mark.parametrize("Nq", [4, 20])
+def test_cross_two_streams_at_once(Nq):
     """Two calls that need scratch, on two streams, many times: each has its own."""
     kn = K()
-    sets = [cuda(*inputs(BF16, 2, 2, 4, 1500, 2, 2, 64, None, False, False, seed=s))[:4] for s in (1, 2)]
+    sets = [cuda(*inputs(BF16, 2, 2, Nq, 1500, 2, 2, 64, None, False, False, seed=s))[:4] for s in (1, 2)]
 
     def both(q, k, v, d_o):
         o, lse = kn.cross_fwd(q, k, v, 2)
@@ -372,12 +372,13 @@ def test_cross_two_streams_at_once():
         assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
 
 
-def test_cross_states_past_32_bits():
+@pytest.mark.parametrize("Nq", [1, 20])
+def test_cross_states_past_32_bits(Nq):
     """Rows of k and v whose byte offsets pass 2^32."""
     kn = K()
     Nk, ld = 600, 1 << 22
     base = torch.empty(1, Nk, ld, dtype=BF16, device="cuda")      # 4.7 GiB
-    q, k, v, d_o, *_ = inputs(BF16, 1, 1, 20, Nk, 1, 1, 32, None, False, False, seed=13)
+    q, k, v, d_o, *_ = inputs(BF16, 1, 1, Nq, Nk, 1, 1, 32, None, False, False, seed=13)
     kd, vd = base[..., :32], base[..., 64:96]
     kd.copy_(k)
     vd.copy_(v)
