@@ -20,7 +20,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffast-math", "
          # forms have given wrong results on this hardware
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Sources whose kernels see infinities and NaN in earnest (masked keys, empty rows) or reduce angles in 64 bits: no fast math.
-PRECISE = {"dm_cross_fwd.hip", "dm_cross_bwd.hip", "dm_cross_few.hip", "dm_cross_one.hip", "dm_cross_onebwd.hip", "dm_rope.hip"}
+PRECISE = {"dm_cross_fwd.hip", "dm_cross_bwd.hip", "dm_cross_few.hip", "dm_cross_one.hip", "dm_cross_onebwd.hip", "dm_cross_rowsbwd.hip", "dm_rope.hip"}
 
 
 def hipcc():

@@ -467,9 +467,12 @@ int one_launch(const CrossParams& p, int dtype, hipStream_t st);
 int join_launch(const CrossParams& p, int dtype, hipStream_t st);      // joins the key splits of either forward
 
 // ---------------------------------------------------------------- the backward of single queries (dm_cross_onebwd.hip)
-struct OneBwdPlan { int tiles; long ws; };
+struct OneBwdPlan { int tiles; long ws; };                  // workgroups along the states, scratch
 bool onebwd_plan(const dm_cross_args* a, OneBwdPlan& f);    // false: too many rows share a key / value head
 int onebwd_launch(const CrossParams& p, int dtype, hipStream_t st);
+// ---------------------------------------------------------------- the backward of longer row lists (dm_cross_rowsbwd.hip)
+bool rowsbwd_plan(const dm_cross_args* a, OneBwdPlan& f);
+int rowsbwd_launch(const CrossParams& p, int dtype, hipStream_t st);
 int dqsum_launch(const CrossParams& p, int dtype, hipStream_t st);     // adds the p.qsplit partials of dQ
 
 }  // namespace dm_cross

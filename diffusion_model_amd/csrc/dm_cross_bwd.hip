@@ -503,7 +503,8 @@ extern "C" long dm_cross_bwd_workspace_bytes(const dm_cross_args* a) {
   dm_cross::FewPlan few;
   dm_cross::OneBwdPlan one;
   if (dm_cross::onebwd_plan(a, one)) return one.ws;
-  return dm_cross::few_plan(a, few) ? few.ws : bwd_plan(a).ws;
+  if (dm_cross::few_plan(a, few)) return few.ws;
+  return dm_cross::rowsbwd_plan(a, one) ? one.ws : bwd_plan(a).ws;
 }
 
 extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
@@ -523,6 +524,12 @@ extern "C" int dm_cross_bwd(const dm_cross_args* a, dm_stream_t stream) {
     p.iters = few.iters; p.nqb = few.nqb; p.nsplit = few.direct ? 0 : 1;
     p.part = (float*)a->workspace;
     return few_launch(p, few, a->dtype, (hipStream_t)stream);
+  }
+  if (rowsbwd_plan(a, one)) {
+    DM_REQUIRE(one.ws == 0 || (a->workspace && a->ws_bytes >= one.ws && (uintptr_t)a->workspace % 16 == 0));
+    p.qsplit = one.tiles; p.nsplit = one.ws ? 1 : 0;
+    p.qpart = (float*)a->workspace;
+    return rowsbwd_launch(p, a->dtype, (hipStream_t)stream);
   }
   const BwdPlan f = bwd_plan(a);
   DM_REQUIRE(a->workspace && a->ws_bytes >= f.ws && (uintptr_t)a->workspace % 16 == 0);

@@ -270,7 +270,7 @@ def test_cross_nan_in_a_valid_state_reaches_only_its_sample():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("hd,Nk,Nq", [(128, 100, 150), (64, 50, 150), (128, 100, 20), (64, 30, 40), (32, 20, 1)])
+@pytest.mark.parametrize("hd,Nk,Nq", [(128, 100, 150), (64, 50, 150), (128, 100, 20), (128, 100, 50), (64, 30, 40), (32, 20, 1)])
 def test_cross_dropout(hd, Nk, Nq, dtype):
     """The keep mask is read off with unit values (o = P Z / keep), is a fair draw, and the same seed then gives the
     forward and the backward of exactly that mask."""
@@ -321,7 +321,7 @@ def test_cross_gradients_against_differences():
         assert abs(num - want) < 2e-3 * size + 1e-3, (i, num, want)
 
 
-@pytest.mark.parametrize("shape", [(4, 2, 200, 70, 4, 2, 32), (2, 2, 3, 900, 2, 2, 64), (2, 2, 20, 900, 2, 2, 64), (5, 2, 1, 400, 2, 2, 64)])
+@pytest.mark.parametrize("shape", [(4, 2, 200, 70, 4, 2, 32), (2, 2, 3, 900, 2, 2, 64), (2, 2, 20, 900, 2, 2, 64), (2, 2, 80, 900, 2, 2, 64), (5, 2, 1, 400, 2, 2, 64)])
 def test_cross_captured_replays(shape):
     """Forward and backward in one HIP graph, replayed with other inputs and other lengths, eager calls in between."""
     kn = K()
@@ -349,7 +349,7 @@ def test_cross_captured_replays(shape):
         assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
 
 
-@pytest.mark.parametrize("Nq", [4, 20])
+@pytest.mark.parametrize("Nq", [4, 20, 40])
 def test_cross_two_streams_at_once(Nq):
     """Two calls that need scratch, on two streams, many times: each has its own."""
     kn = K()
@@ -372,7 +372,7 @@ def test_cross_two_streams_at_once(Nq):
         assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
 
 
-@pytest.mark.parametrize("Nq", [1, 20])
+@pytest.mark.parametrize("Nq", [1, 20, 40])
 def test_cross_states_past_32_bits(Nq):
     """Rows of k and v whose byte offsets pass 2^32."""
     kn = K()
@@ -430,6 +430,47 @@ def test_cross_short_row_lists(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, dtype
     first = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
     rows = B * Nq * H // G / Bc                               # (up to 6 rows per context on average in bf16, 16 in fp32)
     assert kn.last_variant().startswith("cross_bwd_one") == (rows <= (6 if dtype == BF16 else 16))
+    for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *first)):
+        check(name, t, val, tol)
+    again = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Bc,Nq,Nk,H,G,hd,lens,mask,index,p", [
+    (2, 2, 17, 300, 2, 2, 8, "ragged", False, False, 0.0),           # every width; 17 rows: one tile, half of it empty
+    (3, 3, 32, 129, 2, 2, 24, "empty", True, False, 0.0),            # a whole tile; one state in the last workgroup
+    (2, 2, 3, 700, 7, 1, 64, "ragged", True, False, 0.0),            # seven heads of a group
+    (2, 2, 5, 260, 8, 2, 80, "ragged", False, False, 0.0),
+    (1, 1, 30, 100, 1, 1, 128, None, True, False, 0.0),              # one workgroup: no partials
+    (9, 1, 3, 200, 2, 2, 32, None, True, False, 0.0),                # one context for all: rows of nine samples in a tile
+    (23, 4, 5, 333, 2, 2, 40, "ragged", True, True, 0.0),            # lists of several tiles, and empty ones
+    (70, 9, 3, 150, 2, 2, 64, "empty", False, True, 0.0),
+    (2, 2, 20, 140, 4, 4, 104, "ragged", False, False, 0.25),        # dropout
+])
+def test_cross_middle_row_lists(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, p, dtype):
+    kn = K()
+    q, k, v, d_o, L, M, I = inputs(dtype, B, Bc, Nq, Nk, H, G, hd, lens, mask, index, seed=Nk + hd)
+    if index:
+        I[1], I[B - 1] = -3, Bc                               # no context: no gradient, zeros in dq
+        I[2:14] = 3
+    keep = None
+    if p:                                                     # the mask, read off with unit values, a head width at a time
+        cols = []
+        for k0 in range(0, Nk, hd):
+            eye = torch.zeros(Bc, Nk, G, hd)
+            n = min(hd, Nk - k0)
+            eye[:, torch.arange(k0, k0 + n), :, torch.arange(n)] = 1.0
+            z, _ = kn.cross_fwd(q.cuda(), k.cuda(), eye.reshape(Bc, Nk, -1).to(dtype).cuda(), H, drop_p=p, drop_seed=5)
+            cols.append((z.float().cpu().reshape(B, Nq, H, hd).permute(0, 2, 1, 3)[..., :n] > 0).double())
+        keep = torch.cat(cols, -1) / (1.0 - round(p * 32768) / 32768)
+    val, tol = reference(q, k, v, H, G, L, M, I, d_o=d_o, keep=keep)
+    kp, vp = poison(k, v, L, M)
+    dq_, dk_, dv_, do_, dL, dM, dI = cuda(q, kp, vp, d_o, L, M, I)
+    kw = dict(kv_heads=G, lens=dL, mask=dM, index=dI, drop_p=p, drop_seed=5)
+    o, lse = kn.cross_fwd(dq_, dk_, dv_, H, **kw)
+    first = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert kn.last_variant().startswith("cross_bwd_rows") or (dtype == F32 and B * Nq * H // G <= 16 * Bc)
     for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *first)):
         check(name, t, val, tol)
     again = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
