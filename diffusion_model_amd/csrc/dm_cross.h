@@ -1,4 +1,4 @@
-// Shared pieces of the cross-attention kernels (dm_cross_fwd.hip, dm_cross_bwd.hip).
+// Shared pieces of the cross-attention kernels (dm_cross_*.hip).
 //
 // One source serves bf16 and fp32.  Everything runs on the 32x32 MFMA tiles (32x32x16 bf16, four 32x32x2 fp32): in both
 // types a FRAGMENT is 16 bytes per lane, the reduction chunk of one fragment is 32 bytes of a row (16 bf16 or 8 fp32), and
@@ -8,7 +8,7 @@
 // A 32x32 result tile puts column l % 32 and rows 8 i + 4 (l / 32) + r (register 4 i + r) into lane l.  Scores are computed
 // with the softmax axis on the registers (forward, dq) or the lanes (dk, dv), and the probability tile is then, register by
 // register, already the second product's operand over the reduction order "rows 8 i + 4 half + r"; the other operand takes
-// that order through the row addresses of its transposing LDS reads (tr_frag).  No probability passes through LDS.
+// that order through the row addresses of its transposing LDS reads (tr_frag).  Where one pass computes the products of both axes, a probability tile is also turned through LDS.
 #pragma once
 #include "dm_common.h"
 
@@ -396,6 +396,9 @@ struct Samples {
 
 // ---------------------------------------------------------------- host side
 inline int cross_hdp(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 96 ? 96 : 128))); }
+
+// contexts that can have a sample at all (a table may hold many more than a batch uses)
+inline long cross_used(const dm_cross_args* a) { return a->B < a->Bc ? a->B : a->Bc; }
 
 // waves that share a query tile: with one or two tiles of 32 queries the others would have none
 inline int cross_wk(const dm_cross_args* a) { return a->Nq <= 32 ? 4 : (a->Nq <= 64 ? 2 : 1); }

@@ -424,11 +424,13 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
   f.nqb = f.wk > 1 ? 1 : (int)((groups + f.iters - 1) / f.iters);
   f.iters = f.wk > 1 ? 1 : (int)((groups + f.nqb - 1) / f.nqb);
   f.delta_bytes = (((long)a->B * a->heads * a->Nq + 3) & ~3L) * 4;
-  // shares of a context's query list: two workgroups per CU, at least two blocks of queries each
-  const long owners = (long)a->Bc * a->kv_heads * ((a->Nk + 127) / 128);
-  const long list = (long)((a->B + a->Bc - 1) / a->Bc) * (a->heads / a->kv_heads) * ((a->Nq + QS - 1) / QS);
+  // shares of a context's query list: two workgroups per CU, at least two blocks of queries each, partials of at most 256 MiB
+  const long used = cross_used(a), owners = used * a->kv_heads * ((a->Nk + 127) / 128);
+  const long list = (a->B + used - 1) / used * (a->heads / a->kv_heads) * ((a->Nq + QS - 1) / QS);
   long ns = owners > 0 ? 512 / owners : 1;
   if (ns > list / 2) ns = list / 2;
+  const double part = 8.0 * a->Bc * a->Nk * a->kv_heads * a->hd;
+  if (ns * part > (double)(1L << 28)) ns = (long)((double)(1L << 28) / part);
   f.nsplit = ns < 1 ? 1 : (int)ns;
   f.part_bytes = f.nsplit > 1 ? (long)f.nsplit * 2 * a->Bc * a->Nk * a->kv_heads * a->hd * 4 : 0;
   f.ws = f.delta_bytes + f.part_bytes + (f.qsplit > 1 ? (long)f.qsplit * a->B * a->heads * a->Nq * a->hd * 4 : 0);

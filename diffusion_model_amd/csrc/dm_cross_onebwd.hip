@@ -271,7 +271,7 @@ bool onebwd_plan(const dm_cross_args* a, OneBwdPlan& f) {
   // 4.8 and 17.3 at 1, 13.0 and 18.3 at 16)
   const int e = a->dtype == 0 ? 2 : 4;
   const double rows = (double)a->B * (a->heads / a->kv_heads) * a->Nq;
-  if (a->Nk < 1 || rows > (e == 2 ? 6.0 : 16.0) * a->Bc) return false;
+  if (a->Nk < 1 || rows > (e == 2 ? 6.0 : 16.0) * cross_used(a)) return false;
   const int keys = states_per_wg(lanes_per_row(a->hd, e));
   const long tiles = ((long)a->Nk + keys - 1) / keys;
   f.tiles = (int)tiles;

@@ -223,7 +223,7 @@ bool rowsbwd_plan(const dm_cross_args* a, OneBwdPlan& f) {
   // samples, 8 heads on 2 of 96, 77 states, 32 rows: bf16 12.1 and 19.0, fp32 19.5 and 39.0; 16 samples, 8 heads of 128, 1000
   // states, fp32, 32 rows: 145 and 244)
   const double rows = (double)a->B * (a->heads / a->kv_heads) * a->Nq;
-  if (a->Nk < 1 || rows > (a->dtype == 0 ? 32.0 : 64.0) * a->Bc) return false;
+  if (a->Nk < 1 || rows > (a->dtype == 0 ? 32.0 : 64.0) * cross_used(a)) return false;
   const long tiles = ((long)a->Nk + STATES - 1) / STATES;
   f.tiles = (int)tiles;
   f.ws = tiles > 1 || a->index ? tiles * a->B * a->heads * a->Nq * a->hd * 4 : 0;      // (as in onebwd_plan)

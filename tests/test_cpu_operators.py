@@ -118,6 +118,11 @@ def test_cross_workspace_bytes():
     assert L.dm_cross_fwd_workspace_bytes(None) == 0 and L.dm_cross_fwd(None, None) == -1 and L.dm_cross_bwd(None, None) == -1
     crowd = cross_struct(B=4096, Bc=1, Nq=64, Nk=16384)                        # the partial results of key splits stay below 1 GiB
     assert L.dm_cross_fwd_workspace_bytes(ctypes.byref(crowd)) < 1 << 30
+    # contexts that no sample uses leave the way the work is done as it is: long rows keep the kernels of long rows
+    own, table = (cross_struct(B=2, Bc=n, Nq=2304, Nk=77, index=4096) for n in (2, 1000))
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(table)) == L.dm_cross_bwd_workspace_bytes(ctypes.byref(own))
+    table.Nk = 600
+    assert L.dm_cross_bwd_workspace_bytes(ctypes.byref(table)) < 1 << 29
     few = cross_struct(Nq=1, Nk=4096, workspace=None)
     assert L.dm_cross_fwd(ctypes.byref(few), None) == -1
 

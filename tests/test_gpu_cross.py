@@ -475,3 +475,22 @@ def test_cross_middle_row_lists(B, Bc, Nq, Nk, H, G, hd, lens, mask, index, p, d
         check(name, t, val, tol)
     again = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,Nk,variant", [(1, 150, "cross_bwd_one"), (25, 150, "cross_bwd_rows"), (200, 150, "cross_bwd<"), (200, 20, "cross_bwd_few")])
+def test_cross_table_of_more_contexts_than_samples(Nq, Nk, variant, dtype):
+    """The form goes by the contexts that can have samples; the others get zeros."""
+    kn = K()
+    B, Bc, H, hd = 2, 50, 2, 64
+    q, k, v, d_o, L, M, I = inputs(dtype, B, Bc, Nq, Nk, H, H, hd, "ragged", True, True, seed=Nq + Nk)
+    I[:] = torch.tensor([7, 30])
+    L[7], L[30] = Nk, Nk // 2
+    val, tol = reference(q, k, v, H, H, L, M, I, d_o=d_o)
+    dq_, dk_, dv_, do_, dL, dM, dI = cuda(q, *poison(k, v, L, M), d_o, L, M, I)
+    kw = dict(lens=dL, mask=dM, index=dI)
+    o, lse = kn.cross_fwd(dq_, dk_, dv_, H, **kw)
+    grads = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, H, **kw)
+    assert kn.last_variant().startswith(variant)
+    for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *grads)):
+        check(name, t, val, tol)
