@@ -222,8 +222,12 @@ bool rowsbwd_plan(const dm_cross_args* a, OneBwdPlan& f) {
   // 38.4 with two kernels at 32 rows, 44.6 and 41.8 at 48; fp32 78 and 90 at 32, 122 and 122 at 64, 165 and 156 at 96; 16
   // samples, 8 heads on 2 of 96, 77 states, 32 rows: bf16 12.1 and 19.0, fp32 19.5 and 39.0; 16 samples, 8 heads of 128, 1000
   // states, fp32, 32 rows: 145 and 244)
+  // Shared contexts make some lists longer than the average; the widest heads in bf16 (one wave per SIMD)
+  // lose by that (97 samples of 20 rows on 79 contexts of 917 states, 3 heads of 128, forward and backward: 205 us
+  // here, 180 with two kernels; 27 samples on 20 contexts, 8 heads on 4 of 64: 38 and 48).
   const double rows = (double)a->B * (a->heads / a->kv_heads) * a->Nq;
   if (a->Nk < 1 || rows > (a->dtype == 0 ? 32.0 : 64.0) * cross_used(a)) return false;
+  if (a->dtype == 0 && a->hd > 96 && a->index) return false;
   const long tiles = ((long)a->Nk + STATES - 1) / STATES;
   f.tiles = (int)tiles;
   f.ws = tiles > 1 || a->index ? tiles * a->B * a->heads * a->Nq * a->hd * 4 : 0;      // (as in onebwd_plan)
