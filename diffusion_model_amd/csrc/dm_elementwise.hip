@@ -79,6 +79,26 @@ __global__ void cast_bf16_f32_kernel(const bf16* __restrict__ x, float* __restri
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) y[i] = (float)x[i];
 }
 
+// Context rows as operands: the ones that some sample attends to are cast, the others become zeros by a select (their
+// gradients are exact zeros, and a product with what padding holds -- NaN, infinities -- would not be).  One wave per row;
+// whether the row's context has a sample is looked up in the index 64 entries at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void context_rows_kernel(const float* __restrict__ x, T* __restrict__ y, long rows, int L, int D,
+                                                           const int* __restrict__ lens, const unsigned char* __restrict__ mask,
+                                                           const int* __restrict__ index, int B) {
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63, c = (int)(row / L), l = (int)(row - (long)c * L);
+  bool counts = (!lens || l < lens[c]) && (!mask || mask[row]);
+  if (counts && index) {
+    counts = false;
+    for (int b0 = 0; b0 < B && !counts; b0 += 64) counts = __any(b0 + lane < B && index[min(b0 + lane, B - 1)] == c);
+  }
+  const float* src = x + row * D;
+  T* dst = y + row * D;
+  for (int i = lane; i < D; i += 64) dst[i] = counts ? (T)src[i] : (T)0.f;
+}
+
 // dx = dy * silu'(x) (+ add)
 __global__ void silu_bwd_kernel(const bf16* __restrict__ dy, long lddy, const bf16* __restrict__ x, long ldx,
                                 bf16* __restrict__ dx, long lddx, long P, int C) {
@@ -562,6 +582,21 @@ extern "C" int dm_cast_f32_to_bf16(const float* x, void* y, long n, dm_stream_t 
 extern "C" int dm_cast_bf16_to_f32(const void* x, float* y, long n, dm_stream_t stream) {
   DM_REQUIRE(x && y && n > 0);
   hipLaunchKernelGGL(cast_bf16_f32_kernel, dim3(ew_grid(n)), dim3(EW_BLOCK), 0, (hipStream_t)stream, (const bf16*)x, y, n);
+  DM_LAUNCH_CHECK();
+  return DM_OK;
+}
+
+extern "C" int dm_context_rows(const float* x, void* y, int y_is_f32, int Bc, int L, int D, const int* lens,
+                               const unsigned char* mask, const int* index, int B, dm_stream_t stream) {
+  DM_REQUIRE(x && y && Bc > 0 && L > 0 && D > 0 && (!index || B > 0));
+  const long rows = (long)Bc * L, blocks = (rows + 3) / 4;
+  if (blocks >= (1L << 24)) return DM_ERR_TOO_LARGE;      // (a grid has fewer than 2^32 threads)
+  if (y_is_f32)
+    hipLaunchKernelGGL(context_rows_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, x, (float*)y, rows, L, D,
+                       lens, mask, index, B);
+  else
+    hipLaunchKernelGGL(context_rows_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, x, (bf16*)y, rows, L, D,
+                       lens, mask, index, B);
   DM_LAUNCH_CHECK();
   return DM_OK;
 }

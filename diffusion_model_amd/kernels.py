@@ -807,6 +807,32 @@ def _same_device(what: str, *tensors) -> None:
 
 
 # --------------------------------------------------------------------------- attention to encoder states
+def _map_check(what, B, Bc, Nk, lens, mask, index):
+    """Which of Nk states count in each of Bc contexts, and the context of each of B samples: shapes and types."""
+    if lens is not None and (lens.shape != (Bc,) or lens.dtype != torch.int32 or not lens.is_contiguous()):
+        raise ValueError(f"{what}: lens must be a contiguous int32 tensor [{Bc}]")
+    if index is not None and (index.shape != (B,) or index.dtype != torch.int32 or not index.is_contiguous()):
+        raise ValueError(f"{what}: index must be a contiguous int32 tensor [{B}]")
+    if mask is not None and (mask.shape != (Bc, Nk) or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
+        raise ValueError(f"{what}: mask must be a contiguous bool tensor [{Bc}, {Nk}]")
+
+
+def context_rows(x: torch.Tensor, B: int, *, lens=None, mask=None, index=None) -> torch.Tensor:
+    """fp32 contexts [Bc, L, D] of B samples in the compute mode's activation dtype, as operands of the key and value
+    projections and their weight gradients: rows that no sample attends to (cross_fwd's options) are zero, whatever they
+    held (dm_context_rows, include/dm_hip.h)."""
+    if x.dim() != 3:
+        raise ValueError("context_rows: x must be [contexts, L, D]")
+    x = _f32(x.contiguous(), "x")
+    _map_check("context_rows", B, x.shape[0], x.shape[1], lens, mask, index)
+    _same_device("context_rows", x, lens, mask, index)
+    out = torch.empty(x.shape, dtype=ACT[0], device=x.device)
+    if x.numel():
+        check(_lib.lib().dm_context_rows(_p(x), _p(out), int(ACT[0] == F32), *x.shape, _p(lens), _p(mask), _p(index), B, _stream()),
+              "dm_context_rows")
+    return out
+
+
 def _cross_check(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p):
     """Refuses what the kernels do not take; returns (B, Bc, kv_heads, Nq, Nk, hd, scale)."""
     dt = q.dtype
@@ -827,12 +853,7 @@ def _cross_check(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_
         raise ValueError(f"{what}: {Bc} contexts for {B} samples need an index")
     if Bc == 0 and B > 0:
         raise ValueError(f"{what}: no context")
-    if lens is not None and (lens.shape != (Bc,) or lens.dtype != torch.int32 or not lens.is_contiguous()):
-        raise ValueError(f"{what}: lens must be a contiguous int32 tensor [{Bc}]")
-    if index is not None and (index.shape != (B,) or index.dtype != torch.int32 or not index.is_contiguous()):
-        raise ValueError(f"{what}: index must be a contiguous int32 tensor [{B}]")
-    if mask is not None and (mask.shape != (Bc, Nk) or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
-        raise ValueError(f"{what}: mask must be a contiguous bool tensor [{Bc}, {Nk}]")
+    _map_check(what, B, Bc, Nk, lens, mask, index)
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"{what}: scale must be positive")

@@ -221,6 +221,11 @@ class ContextMap(NamedTuple):
         return dict(lens=self.lens, mask=self.mask, index=self.index)
 
 
+def _context_in(c, B, cmap: Optional[ContextMap]):
+    """fp32 contexts [.., L, D] of B samples as an operand; with a map, tokens that no sample attends to become zeros."""
+    return K.to_bf16(c.contiguous()) if cmap is None else K.context_rows(c, B, **cmap.kw())
+
+
 def _b(c):
     return None if c.bias is None else c.bias.detach()
 
@@ -679,7 +684,7 @@ class CrossAttention(HipModule):
         self._ctx2d = c.dim() == 2
         if c.dim() == 2:
             c = c.unsqueeze(1)
-        y, saved = self._fwd(_nhwc_in(x), K.to_bf16(c.contiguous()), cmap=cmap)
+        y, saved = self._fwd(_nhwc_in(x), _context_in(c, x.shape[0], cmap), cmap=cmap)
         return K.nhwc_to_nchw(y), saved
 
     def _run_bwd(self, dout, saved, g, need):
@@ -958,7 +963,7 @@ class UNET(HipModule):
             c = context.detach().float()
             if c.dim() == 2:
                 c = c.unsqueeze(1)
-            ctx = K.to_bf16(c.contiguous())
+            ctx = _context_in(c, B, cmap)
         x0 = K.nchw_to_nhwc(x.detach().float().contiguous(), (Cin + 63) // 64 * 64)
         a = K.conv3x3(x0, PW.of(self.input_conv).fwd, self.Channels[0], bias=_b(self.input_conv))
         L, half = self.num_layers, self.num_layers // 2

@@ -34,7 +34,8 @@ typedef void* dm_stream_t;
 /* ABI version / arch string ("gfx950").  Version 2 (round 2): dm_conv_args / dm_wgrad_args grew the trailing
  * norm_scale / norm_shift fields.  Version 3: dm_attn_args grew the trailing workspace / ws_bytes fields and
  * dm_attn_bwd_workspace_bytes, dm_film_fwd / dm_film_bwd were added.  Version 4 (round 3): the fp32 compute mode (the *_f32
- * entry points at the end of this header); nothing older changed; dm_cross_* and dm_rope were added to it since.  Callers
+ * entry points at the end of this header); nothing older changed; dm_cross_*, dm_rope and
+ * dm_context_rows were added to it since.  Callers
  * built against an older version must be rebuilt. */
 int dm_abi_version(void);
 const char* dm_target_arch(void);
@@ -298,6 +299,11 @@ int dm_nhwc_to_nchw_f32(const void* x, int x_is_f32, long ldx, float* y, int B, 
 /* dtype casts of small contiguous buffers (time-embedding rows, per-(b,c) sums). */
 int dm_cast_f32_to_bf16(const float* x, void* y, long n, dm_stream_t stream);
 int dm_cast_bf16_to_f32(const void* x, float* y, long n, dm_stream_t stream);
+/* Context rows as dm_cross_*'s states are projected from: y[Bc, L, D] = x where a sample attends to the row, 0 elsewhere, whatever
+ * x holds there (weight gradients multiply every row, also one whose own gradient is zero).  Row l of context c counts iff
+ * l < lens[c] (NULL: all), mask[c][l] != 0 (NULL: all) and some index[b] == c (NULL: every context has a sample). */
+int dm_context_rows(const float* x, void* y, int y_is_f32, int Bc, int L, int D, const int* lens, const unsigned char* mask,
+                    const int* index, int B, dm_stream_t stream);
 /* out = a (+ b): residual add / strided copy into a concat slice (unet.py:274,355). */
 int dm_add_bf16(const void* a, long lda, const void* b, long ldb, void* out, long ldo, long P, int C,
                 dm_stream_t stream);

@@ -148,3 +148,24 @@ def rope_struct(**kw):
     dict(grid=(2, 4)), dict(grid=(0, 3)), dict(grid=(-2, -3)), dict(grid=(1 << 30, 1 << 30)), dict(heads=2048)])
 def test_rope_entry_point_refuses(kw):
     assert _lib.lib().dm_rope(ctypes.byref(rope_struct(**kw)), None) == -1
+
+
+C3 = torch.zeros(2, 7, 48)
+
+
+@pytest.mark.parametrize("x,kw", [
+    (C3[0], {}), (C3, dict(lens=torch.zeros(3, dtype=torch.int32))), (C3, dict(lens=torch.zeros(2, dtype=torch.int64))),
+    (C3, dict(mask=torch.zeros(2, 6, dtype=torch.bool))), (C3, dict(index=torch.zeros(5, dtype=torch.int32))),
+    (C3, {})])                                        # the last one: everything fits, but no tensor is on the GPU
+def test_context_rows_refusals(x, kw):
+    with pytest.raises(ValueError):
+        K.context_rows(x, 4, **kw)
+
+
+def test_context_rows_entry_point_refuses():
+    f = _lib.lib().dm_context_rows
+    for args in ((None, 4096, 0, 2, 7, 48, None, None, None, 2), (4096, None, 0, 2, 7, 48, None, None, None, 2),
+                 (4096, 4096, 0, 0, 7, 48, None, None, None, 2), (4096, 4096, 0, 2, 0, 48, None, None, None, 2),
+                 (4096, 4096, 0, 2, 7, 0, None, None, None, 2), (4096, 4096, 0, 2, 7, 48, None, None, 4096, 0)):
+        assert f(*args, None) == -1
+    assert f(4096, 4096, 0, 1 << 20, 1 << 10, 48, None, None, None, 2, None) == -3       # more rows than a launch holds

@@ -272,3 +272,100 @@ def test_sampling_from_a_table_larger_than_the_batch():
     for bad in (9, -1):
         with pytest.raises(IndexError):
             CFGSampler(m, sched, table, 8, context_lens=lens).sample(z, torch.tensor([1, bad]), **kw)
+
+
+def padded(kind, Bc, L):
+    """Map options for four samples, and which tokens of the Bc contexts no sample attends to."""
+    lens, mask = torch.tensor([9, 4, 0, 1, 7])[:Bc], torch.rand(Bc, L, generator=torch.Generator().manual_seed(1)) < 0.6
+    bad = torch.zeros(Bc, L, dtype=torch.bool)
+    if kind != "mask":
+        bad |= torch.arange(L) >= lens[:, None]
+    if kind != "lens":
+        bad |= ~mask
+    kw = {"lens": dict(context_lens=lens), "mask": dict(context_mask=mask), "index": dict(context_lens=lens, context_mask=mask)}[kind]
+    if kind == "index":
+        kw["context_index"] = torch.tensor([0, 1, 1, 2])
+        bad[3:] = True
+    return kw, bad
+
+
+FILLS = [0.0, float("nan"), -float("inf"), 3.4e38]            # (the last one is finite, and infinite in bf16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["lens", "mask", "index"])
+def test_padding_reaches_no_gradient(kind, dtype):
+    """A training micro-step has the same bits whatever the padding holds: tokens past a length, masked ones, and contexts
+    that no sample uses."""
+    from diffusion_model_amd import kernels as K
+    from diffusion_model_amd.trainer import Trainer
+    from diffusion_model_amd.unet import UNET, reseed_dropout
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    x, t, ctx = case(4, 5 if kind == "index" else 4, 9)
+    kw, bad = padded(kind, ctx.shape[0], 9)
+    e = torch.randn(x.shape, generator=torch.Generator().manual_seed(2)).to(dev())
+    runs = []
+    for fill in FILLS:
+        c = ctx.clone()
+        c[bad] = fill
+        torch.manual_seed(11)
+        m = UNET(**{**KW, "dropout_prob": 0.1})
+        with torch.no_grad():
+            m.output_conv.weight.normal_(0, 0.05)
+        tr = Trainer(m.to(dev()).train(), DDPM_beta_t_cosine_scheduler(500), accum=2)
+        reseed_dropout(5)
+        with K.compute_dtype(dtype):
+            loss = tr.micro_step(x.to(dev()), c.to(dev()), t.to(dev()), e, **kw)
+            K.join_side(dev())                                # (weight gradients of an open accumulation window)
+        runs.append((loss.clone(), tr.fp.grad.clone()))
+    assert bool(torch.isfinite(runs[0][1]).all()) and float(runs[0][1].abs().max()) > 0
+    for loss, grad in runs[1:]:
+        assert torch.equal(loss, runs[0][0]) and torch.equal(grad, runs[0][1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["lens", "mask", "index"])
+def test_padding_in_the_module(kind, dtype):
+    """CrossAttention by itself: output, input and weight gradients do not depend on the padding, whose own gradient is zero."""
+    from diffusion_model_amd import kernels as K
+    from diffusion_model_amd.unet import CrossAttention
+    torch.manual_seed(4)
+    m = CrossAttention(64, 48, HEADS, 0.0).to(dev()).eval()
+    Bc = 5 if kind == "index" else 4
+    x, ctx, w = torch.randn(4, 64, 6, 5), torch.randn(Bc, 9, 48), torch.randn(4, 64, 6, 5).to(dev())
+    kw, bad = padded(kind, Bc, 9)
+    runs = []
+    for fill in FILLS:
+        c = ctx.clone()
+        c[bad] = fill
+        m.zero_grad()
+        with K.compute_dtype(dtype):
+            xd, cd = x.to(dev()).requires_grad_(), c.to(dev()).requires_grad_()
+            y = m(xd, cd, **kw)
+            (y * w).sum().backward()
+        assert bool((cd.grad[bad.to(dev())] == 0).all())
+        runs.append([y.detach(), xd.grad, cd.grad, *(p.grad.clone() for p in m.parameters())])
+    assert all(bool(torch.isfinite(t).all()) for t in runs[0])
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Bc,L,D,B", [(1, 1, 1, 1), (3, 7, 48, 3), (5, 77, 130, 200), (130, 3, 65, 2)])
+def test_context_rows(Bc, L, D, B, dtype):
+    from diffusion_model_amd import kernels as K
+    g = torch.Generator().manual_seed(Bc + B)
+    x, index = torch.randn(Bc, L, D, generator=g), torch.randint(-1, Bc + 1, (B,), generator=g, dtype=torch.int32)
+    lens, mask = torch.randint(-1, L + 2, (Bc,), generator=g, dtype=torch.int32), torch.rand(Bc, L, generator=g) < 0.7
+    with K.compute_dtype(dtype):
+        for li, mi, ii in ((lens, None, None), (None, mask, None), (None, None, index), (lens, mask, index)):
+            ok = torch.ones(Bc, L, dtype=torch.bool)
+            if li is not None:
+                ok &= torch.arange(L) < lens[:, None]
+            if mi is not None:
+                ok &= mask
+            if ii is not None:
+                ok &= (index[None] == torch.arange(Bc)[:, None]).any(1)[:, None]
+            c = torch.where(ok[..., None], x, torch.full_like(x, float("nan")))
+            y = K.context_rows(c.to(dev()), B, **{n: None if v is None else v.to(dev()) for n, v in (("lens", li), ("mask", mi), ("index", ii))})
+            assert y.dtype == dtype and torch.equal(y.cpu(), torch.where(ok[..., None], x, torch.zeros_like(x)).to(dtype))
