@@ -69,8 +69,10 @@ __global__ __launch_bounds__(256) void cross_one_kernel(const CrossParams p) {
       float mx = m[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
-      const float mc = mx == -INFINITY ? 0.f : mx * c;
-      const float alpha = __builtin_amdgcn_exp2f(m[r] * c - mc);      // (m = -inf: 0)
+      // exactly 1 while the maximum stays: from m[r] * c - mc, contracted, the rounding of mc would be left, a factor on l and
+      // o in every step
+      const float ref = mx == -INFINITY ? 0.f : mx, mc = ref * c;
+      const float alpha = __builtin_amdgcn_exp2f((m[r] - ref) * c);      // (m = -inf: 0)
       m[r] = mx;
       l[r] *= alpha;
 #pragma unroll
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(256) void cross_one_kernel(const CrossParams p) {
     float mx = m[r];
 #pragma unroll
     for (int w = LPR; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w, 64));
-    const float mc = mx == -INFINITY ? 0.f : mx * c, f = __builtin_amdgcn_exp2f(m[r] * c - mc);
+    const float ref = mx == -INFINITY ? 0.f : mx, mc = ref * c, f = __builtin_amdgcn_exp2f((m[r] - ref) * c);      // (as alpha)
     float x = l[r] * f;
 #pragma unroll
     for (int w = LPR; w < 64; w <<= 1) x += __shfl_xor(x, w, 64);

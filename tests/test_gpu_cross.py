@@ -494,3 +494,27 @@ def test_cross_table_of_more_contexts_than_samples(Nq, Nk, variant, dtype):
     assert kn.last_variant().startswith(variant)
     for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *grads)):
         check(name, t, val, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_cross_single_query_long_stream_keeps_its_weights(dtype):
+    """512 workgroups, so each streams its 4096 states alone, with scores around 369, whose product with log2(e) is rounded by
+    2.9e-5: were that left in the factor of a step, it would grow with every step.  The scores 41 * 9 - j are exact in both types.
+    Errors: lse rounds log2(e) and ln(2), their products and the last sum (4 u |lse|), the logarithm of at most 2^12 by 2 ulp
+    (17 u); a weight is off by the argument of its exponential (at most 8.7 + 2.9e-5 / u, rounded: 9 u), the exponential (2 u),
+    the adds of its lane (4 states a step, 4 waves, 64 / lanes-per-state states each) and 12 more in the joins."""
+    kn = K()
+    B, Nk, hd = 512, 4096, 128
+    j = torch.randint(0, 7, (Nk,), generator=torch.Generator().manual_seed(1)).double()
+    j[:64] = 0
+    q, k, v = torch.zeros(B, 1, hd), torch.zeros(1, Nk, hd), torch.zeros(1, Nk, hd)
+    q[..., 0], q[..., 1] = 41.0, 1.0
+    k[0, :, 0], k[0, :, 1] = 9.0, -j.float()
+    v[0, Nk // 2:] = 1.0
+    o, lse = kn.cross_fwd(*(t.to(dtype).cuda() for t in (q, k, v)), 1, scale=1.0)
+    assert kn.last_variant().startswith("cross_one")
+    w = torch.exp(-j)
+    want_lse, want_o = 369 + math.log(float(w.sum())), float(w[Nk // 2:].sum() / w.sum())
+    rel = (9 + 2 + Nk // (4 * (64 // (16 if dtype == BF16 else 32))) + 12) * U
+    assert float((lse.double().cpu() - want_lse).abs().max()) <= 4 * U * want_lse + 17 * U + rel
+    assert float((o.double().cpu()[..., 0] - want_o).abs().max()) <= (2 * rel + 2 * U + (2.0 ** -8 if dtype == BF16 else U)) * want_o
