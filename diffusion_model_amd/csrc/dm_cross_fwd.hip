@@ -236,6 +236,11 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) <= 64 ? 4 : (HDP * (int)
     const bool half = n - (k1 - k0) >= 16;
     stage(k0, n);
     __syncthreads();
+    // the first step looks at no validity word, and a masked key's score is -infinity only under a finite query (its product
+    // with the zeroed key is not zero under a NaN or an infinity): without any valid key there is no step
+    bool some = !mask;
+    if (mask)
+      for (int t = 0; t < tiles; ++t) some = some || __builtin_amdgcn_readfirstlane((int)bits[t]) != 0;
     // one loop for each number of tiles, so that each keeps only its own LDS addresses in registers
     auto each = [&](auto step) {
       for (int it = 0; it < p.iters; ++it) {
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(256, (HDP * (int)sizeof(T) <= 64 ? 4 : (HDP * (int)
         fwd_finish<T, HDP>(p, st, b, h, q, split, c, lane);
       }
     };
-    if (tiles == 0) each([&]() { clear(); });
+    if (tiles == 0 || !some) each([&]() { clear(); });
     else if (tiles == 1 && half) each([&]() { DM_STEP_H(1, true, true, 0, k0); });
     else if (tiles == 1) each([&]() { DM_STEP(1, true, 0, k0); });
     else if (tiles == 2 && half) each([&]() { DM_STEP_H(2, true, true, 0, k0); });

@@ -518,3 +518,22 @@ def test_cross_single_query_long_stream_keeps_its_weights(dtype):
     rel = (9 + 2 + Nk // (4 * (64 // (16 if dtype == BF16 else 32))) + 12) * U
     assert float((lse.double().cpu() - want_lse).abs().max()) <= 4 * U * want_lse + 17 * U + rel
     assert float((o.double().cpu()[..., 0] - want_o).abs().max()) <= (2 * rel + 2 * U + (2.0 ** -8 if dtype == BF16 else U)) * want_o
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,Nk,hd", [(40, 20, 32), (40, 40, 32), (300, 13, 32), (300, 30, 32), (300, 40, 32), (300, 77, 16), (300, 90, 16), (200, 300, 64), (200, 900, 128),
+                                      (20, 300, 64), (1, 300, 64), (4, 50, 32)])
+@pytest.mark.parametrize("kind", ["lens", "mask"])
+def test_cross_no_valid_state_whatever_the_query_holds(kind, Nq, Nk, hd, dtype):
+    """Samples without a valid state get o = 0, lse = -infinity and no gradient also under NaN and infinite queries and output
+    gradients, in every form."""
+    kn = K()
+    q, k, v, d_o, *_ = inputs(dtype, 3, 3, Nq, Nk, 2, 2, hd, None, False, False, seed=Nq + Nk)
+    q[0], q[1], d_o[0] = float("nan"), float("inf"), float("nan")
+    lens = torch.tensor([0, 0, Nk], dtype=torch.int32) if kind == "lens" else None
+    mask = torch.tensor([[False], [False], [True]]).expand(3, Nk).contiguous() if kind == "mask" else None
+    q, k, v, d_o, lens, mask = cuda(q, k, v, d_o, lens, mask)
+    o, lse = kn.cross_fwd(q, k, v, 2, lens=lens, mask=mask)
+    assert bool((o[:2] == 0).all()) and bool((lse[:2] == -math.inf).all()) and bool(torch.isfinite(lse[2]).all())
+    for t in kn.cross_bwd(q, k, v, o, lse, d_o, 2, lens=lens, mask=mask):
+        assert bool((t[:2] == 0).all()) and bool(torch.isfinite(t[2]).all())
