@@ -262,7 +262,8 @@ typedef struct dm_cross_args {
   float drop_p; unsigned long long drop_seed;
   void* workspace; long ws_bytes; /* >= dm_cross_fwd_workspace_bytes / dm_cross_bwd_workspace_bytes; 16-byte aligned */
 } dm_cross_args;
-/* Scratch for these sizes (0: none needed); only B, Bc, heads, kv_heads, Nq, Nk, hd and dtype are read. */
+/* Scratch for these sizes (0: none needed).  Only B, Bc, heads, kv_heads, Nq, Nk, hd, dtype and whether index is NULL are
+ * read: with an index the backward needs other scratch than without (a sample may then have no context). */
 long dm_cross_fwd_workspace_bytes(const dm_cross_args* args);
 long dm_cross_bwd_workspace_bytes(const dm_cross_args* args);
 int dm_cross_fwd(const dm_cross_args* args, dm_stream_t stream);

@@ -169,3 +169,25 @@ def test_context_rows_entry_point_refuses():
                  (4096, 4096, 0, 2, 7, 0, None, None, None, 2), (4096, 4096, 0, 2, 7, 48, None, None, 4096, 0)):
         assert f(*args, None) == -1
     assert f(4096, 4096, 0, 1 << 20, 1 << 10, 48, None, None, None, 2, None) == -3       # more rows than a launch holds
+
+
+@pytest.mark.parametrize("kw", [dict(B=3, Bc=3, Nq=2, Nk=20), dict(B=4, Bc=4, Nq=20, Nk=150, hd=128, ldq=256, ldk=256, ldv=256),
+                                dict(B=2, Bc=2, Nq=64, Nk=20), dict(B=2, Bc=2, Nq=200, Nk=400)])
+def test_cross_workspace_bytes_read_the_fields_that_the_header_names(kw):
+    """Scratch sized from the named fields alone is the scratch that the call asks for; whether index is NULL is one of them."""
+    import os
+    L = _lib.lib()
+    names = ("B", "Bc", "heads", "kv_heads", "Nq", "Nk", "hd", "dtype", "index")
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "dm_hip.h")).read()
+    said = header[header.index("/* Scratch for these sizes"):header.index("long dm_cross_fwd_workspace_bytes")]
+    assert all(n in said for n in names)
+    sizes = []
+    for index in (None, 4096):
+        full, bare = cross_struct(**kw, index=index, lens=4096, mask=4096), _lib.CrossArgs()
+        for n in names:
+            setattr(bare, n, getattr(full, n))
+        for f in (L.dm_cross_fwd_workspace_bytes, L.dm_cross_bwd_workspace_bytes):
+            assert f(ctypes.byref(bare)) == f(ctypes.byref(full))
+        sizes.append(L.dm_cross_bwd_workspace_bytes(ctypes.byref(bare)))
+    if kw["Nk"] < 200:
+        assert sizes[0] != sizes[1]
