@@ -190,11 +190,14 @@ class CFGSampler:
         g[labels.cpu() == self.uncond_id] = 0.0
         beta, abar = self.sched.beta_cpu, self.sched.alpha_bar_cpu
         uncond = torch.full_like(labels, self.uncond_id)
+        n, ctx = 0, ()
         for t in range(starts[0], -1, -1):
-            n = sum(1 for s0 in starts if s0 >= t)          # the active samples are a prefix
+            active = sum(1 for s0 in starts if s0 >= t)     # the active samples are a prefix
+            if active != n:                                 # (contexts change only when samples join)
+                n, ctx = active, self._contexts(torch.cat([uncond[:active], labels[:active]]))
             zz = torch.cat([z[:n], z[:n]])
             tt = torch.full((2 * n,), t, dtype=torch.long, device=dev)
-            v, _ = model._fwd(zz, tt, *self._contexts(torch.cat([uncond[:n], labels[:n]])))
+            v, _ = model._fwd(zz, tt, *ctx)
             coef = step_coefficients(beta, abar, t, g[:n], eta, n, final=(t == 0)).to(dev)
             if t > 1 and eta > 0.0:
                 noise = torch.randn(z[:n].shape, dtype=torch.float32, device=dev, generator=generator)

@@ -191,3 +191,35 @@ def test_cross_workspace_bytes_read_the_fields_that_the_header_names(kw):
         sizes.append(L.dm_cross_bwd_workspace_bytes(ctypes.byref(bare)))
     if kw["Nk"] < 200:
         assert sizes[0] != sizes[1]
+
+
+def test_partial_sampling_makes_its_contexts_once_per_joining_group(monkeypatch):
+    """sample_from: the table goes to the device, is gathered and its ids are looked over when samples join the walk, not in
+    every step."""
+    from diffusion_model_amd.sampler import CFGSampler
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    seen, made = [], []
+
+    class Model:
+        def eval(self):
+            return self
+
+        def _fwd(self, zz, tt, ctx, cmap=None):
+            n = zz.shape[0]
+            index = torch.arange(ctx.shape[0]) if cmap is None or cmap.index is None else cmap.index.long()
+            seen.append((int(tt[0]), ctx[index][:, 0, 0].tolist(), None if cmap is None else cmap.lens.tolist()))
+            assert index.numel() == n
+            return torch.zeros_like(zz), None
+
+    monkeypatch.setattr(K, "cfg_ddpm_step", lambda z, v_u, v_c, noise, coef: z)
+    make = CFGSampler._contexts
+    monkeypatch.setattr(CFGSampler, "_contexts", lambda self, ids: made.append(ids.tolist()) or make(self, ids))
+    table = torch.arange(4.0)[:, None, None].expand(4, 7, 8).contiguous()
+    labels, starts = torch.tensor([0, 1, 2, 1, 3]), [0, 6, 9, 6, 9]
+    for lens in (None, torch.tensor([7, 3, 5, 1])):
+        seen.clear(), made.clear()
+        CFGSampler(Model(), DDPM_beta_t_cosine_scheduler(50), table, 3, context_lens=lens).sample_from(torch.zeros(5, 1, 2, 2), labels, starts)
+        assert made == [[3, 3, 2, 3], [3] * 4 + [2, 3, 1, 1], [3] * 5 + [2, 3, 1, 1, 0]]
+        assert [t for t, *_ in seen] == list(range(9, -1, -1))
+        for t, ids, _ in seen:
+            assert ids == made[0 if t > 6 else (1 if t > 0 else 2)]

@@ -369,3 +369,38 @@ def test_context_rows(Bc, L, D, B, dtype):
             c = torch.where(ok[..., None], x, torch.full_like(x, float("nan")))
             y = K.context_rows(c.to(dev()), B, **{n: None if v is None else v.to(dev()) for n, v in (("lens", li), ("mask", mi), ("index", ii))})
             assert y.dtype == dtype and torch.equal(y.cpu(), torch.where(ok[..., None], x, torch.zeros_like(x)).to(dtype))
+
+
+@pytest.mark.parametrize("how", ["from", "dpm", "dpm unguided"])
+def test_partial_and_dpm_sampling_with_lengths(how):
+    """sample_from and sample_dpm with lengths: a table handed over whole (or gathered, while few samples walk) against each
+    sample's own copy of its context."""
+    from diffusion_model_amd.dpm_solver import DPMSolverMultistepScheduler
+    from diffusion_model_amd.sampler import CFGSampler
+    from diffusion_model_amd.unet import ContextMap
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    m, _ = network(True)
+    g = torch.Generator().manual_seed(8)
+    table, lens = torch.randn(4, 7, KW["context_dim"], generator=g).to(dev()), torch.tensor([7, 3, 5, 1])
+    z, labels = torch.randn(5, 3, 16, 16, generator=g).to(dev()), torch.tensor([0, 1, 2, 1, 3])
+
+    class Copies:
+        """The same model, given every sample's own context."""
+        eval = staticmethod(m.eval)
+
+        @staticmethod
+        def _fwd(zz, tt, ctx, cmap):
+            if cmap.index is None:
+                return m._fwd(zz, tt, ctx, cmap)
+            ids = cmap.index.long()
+            return m._fwd(zz, tt, ctx[ids].contiguous(), ContextMap(cmap.lens[ids].contiguous(), None, None))
+
+    def run(model):
+        s = CFGSampler(model, DDPM_beta_t_cosine_scheduler(500), table, 3, context_lens=lens)
+        if how == "from":
+            return s.sample_from(z, labels, [0, 2, 3, 1, 3], guidance_scale=2.0, eta=0.0)
+        dpm = DPMSolverMultistepScheduler(num_train_timesteps=500, prediction_type="v_prediction")
+        return s.sample_dpm(z, labels, dpm, cfg_scale=2.0 if how == "dpm" else 0.0, num_inference_steps=4)
+
+    a, b = run(m), run(Copies)
+    assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
