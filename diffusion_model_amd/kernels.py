@@ -882,14 +882,42 @@ def _rows16(what, name, t, esize):
     return ptr, ld
 
 
-def _cross_out(what, name, t, like, *inputs):
+def _span(t):
+    """(address, row stride, rows, bytes of a row) of a tensor's memory: one row if contiguous."""
+    es = t.element_size()
+    if t.is_contiguous():
+        return t.data_ptr(), 0, 1, t.numel() * es
+    ld, n, w = t.stride(-2) if t.shape[-2] > 1 else t.stride(-3), t.numel() // t.shape[-1], t.shape[-1]
+    if ld <= w:                                          # (rows without a gap)
+        return t.data_ptr(), 0, 1, ((n - 1) * ld + w) * es
+    return t.data_ptr(), ld * es, n, w * es
+
+
+def _share(a, b) -> bool:
+    """Whether two tensors of densely packed rows share memory (slices of one fused buffer do not).  Interleaved rows of
+    different strides count as sharing."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (p, lp, n, w), (q, lq, m, x) = sorted((_span(a), _span(b)))
+    if q >= p + (n - 1) * lp + w:
+        return False
+    if n == 1:
+        return True                                      # (the other one starts inside)
+    if m == 1:
+        d = (q - p) % lp
+        return d < w or d + x > lp
+    return lp != lq or (q - p) % lp < w or (q - p) % lp + x > lp
+
+
+def _cross_out(what, name, t, like, *others):
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if t.numel() and t.data_ptr() in [x.data_ptr() for x in inputs]:
-        raise ValueError(f"{what}: {name} must not be one of the operands")
     if t.shape != like.shape or t.dtype != like.dtype:
         raise ValueError(f"{what}: {name} must have the shape {tuple(like.shape)} and the operands' type")
     _same_device(what, t)
+    _rows16(what, name, t, t.element_size())
+    if any(_share(t, x) for x in others if x is not None):
+        raise ValueError(f"{what}: {name} must not share memory with an operand or another result")
     return t
 
 
@@ -927,16 +955,18 @@ def cross_bwd(q, k, v, o, lse, d_o, heads: int, *, kv_heads: Optional[int] = Non
               scale: Optional[float] = None, drop_p: float = 0.0, drop_seed: int = 0, dq=None, dk=None, dv=None):
     """Backward of cross_fwd with the same options: (dq, dk, dv) in q's, k's and v's shapes.  dk and dv are sums over the
     query heads of a group and over the samples that share a context, in a fixed order; rows of invalid states are zero.
-    Given ``dq``, ``dk``, ``dv`` share no memory with the operands or with one another."""
+    Given ``dq``, ``dk``, ``dv``, views with rows like q's and k's, share no memory with the operands or with one another."""
     B, Bc, kv_heads, Nq, Nk, hd, scale = _cross_check("cross_bwd", q, k, v, heads, kv_heads, lens, mask, index, scale, drop_p)
     if o.shape != q.shape or d_o.shape != q.shape or o.dtype != q.dtype or d_o.dtype != q.dtype:
         raise ValueError("cross_bwd: o and d_o must have q's shape and type")
     if lse.shape != (B, heads, Nq) or lse.dtype != F32 or not lse.is_contiguous():
         raise ValueError("cross_bwd: lse must be cross_fwd's")
     _same_device("cross_bwd", o, d_o, lse)
-    read = (q, k, v, o, d_o)
+    read = (q, k, v, o, d_o, lse)
+    dq_, dk_ = dq, dk
     dq = _cross_out("cross_bwd", "dq", dq, q, *read)
-    dk, dv = _cross_out("cross_bwd", "dk", dk, k, *read), _cross_out("cross_bwd", "dv", dv, v, *read)
+    dk = _cross_out("cross_bwd", "dk", dk, k, *read, dq_)
+    dv = _cross_out("cross_bwd", "dv", dv, v, *read, dq_, dk_)
     if B == 0 or Nq == 0:
         return dq, dk.zero_(), dv.zero_()
     f32m = q.dtype == F32

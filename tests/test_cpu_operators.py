@@ -223,3 +223,31 @@ def test_partial_sampling_makes_its_contexts_once_per_joining_group(monkeypatch)
         assert [t for t, *_ in seen] == list(range(9, -1, -1))
         for t, ids, _ in seen:
             assert ids == made[0 if t > 6 else (1 if t > 0 else 2)]
+
+
+def test_shared_memory_of_row_views():
+    """_share against the sets of addresses, for views of one buffer with the rows that the front-ends take."""
+    import random
+    rng, buf, both = random.Random(3), torch.zeros(400), [0, 0]
+
+    def view():
+        while True:
+            n0, n1, w, at = rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 8), rng.randint(0, 200)
+            ld = rng.choice([16, 16, 16, w, 11])
+            if w <= ld and at + (n0 * n1 - 1) * ld + w <= 400:
+                return buf.as_strided((n0, n1, w), (n1 * ld, ld, 1), at)
+
+    def cells(t):
+        return {t.storage_offset() + i * t.stride(0) + j * t.stride(1) + c for i in range(t.shape[0]) for j in range(t.shape[1]) for c in range(t.shape[2])}
+
+    for _ in range(4000):
+        a, b = view(), view()
+        share = bool(cells(a) & cells(b))
+        (_, la, n, _), (_, lb, m, _) = K._span(a), K._span(b)
+        if n == 1 or m == 1 or la == lb:
+            assert K._share(a, b) == share == K._share(b, a)
+            both[share] += 1
+        elif share:
+            assert K._share(a, b) and K._share(b, a)
+    assert min(both) > 300
+    assert not K._share(buf[:0].view(1, 0, 4), buf.view(1, 100, 4)) and K._share(buf[:1].expand(2, 3, 1), buf.view(1, 100, 4))

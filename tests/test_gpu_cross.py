@@ -537,3 +537,23 @@ def test_cross_no_valid_state_whatever_the_query_holds(kind, Nq, Nk, hd, dtype):
     assert bool((o[:2] == 0).all()) and bool((lse[:2] == -math.inf).all()) and bool(torch.isfinite(lse[2]).all())
     for t in kn.cross_bwd(q, k, v, o, lse, d_o, 2, lens=lens, mask=mask):
         assert bool((t[:2] == 0).all()) and bool(torch.isfinite(t[2]).all())
+
+
+def test_cross_refuses_outputs_that_share_memory():
+    """With one another (the same tensor for two gradients, views that overlap) or with an operand, from another start; slices
+    of one fused buffer are fine."""
+    kn = K()
+    buf = torch.zeros(2, 7, 96, dtype=BF16, device="cuda")
+    q, k, v = (torch.randn(2, 7, 32, device="cuda").to(BF16) for _ in range(3))
+    o, lse = kn.cross_fwd(q, k, v, 2)
+    d_o, g = torch.randn_like(q), torch.zeros_like(q)
+    for kw in (dict(dk=g, dv=g), dict(dq=g, dk=g), dict(dq=g, dv=g), dict(dk=buf[..., :32], dv=buf[..., 16:48]),
+               dict(dq=buf[..., :32], dv=buf.view(-1)[8:8 + g.numel()].view_as(g))):
+        with pytest.raises(ValueError):
+            kn.cross_bwd(q, k, v, o, lse, d_o, 2, **kw)
+    for out in (buf[..., 24:56], buf.view(-1)[8:8 + q.numel()].view_as(q)):
+        with pytest.raises(ValueError):
+            kn.cross_fwd(buf[..., :32], k, v, 2, out=out)
+    want = kn.cross_bwd(q, k, v, o, lse, d_o, 2)
+    kn.cross_bwd(q, k, v, o, lse, d_o, 2, dq=buf[..., :32], dk=buf[..., 32:64], dv=buf[..., 64:])
+    assert all(torch.equal(a, b) for a, b in zip(want, buf.split(32, -1)))
