@@ -198,6 +198,7 @@ extern "C" int dm_rope(const dm_rope_args* a, dm_stream_t stream) {
   DM_REQUIRE(a->rot >= 2 && a->rot % 2 == 0 && a->rot <= a->hd);
   DM_REQUIRE(a->axes >= 1 && a->axes <= 3 && (a->dtype == 0 || a->dtype == 1) && (a->pairing == 0 || a->pairing == 1));
   DM_REQUIRE(a->ldx >= (long)a->heads * a->hd && a->ldy >= (long)a->heads * a->hd);
+  DM_REQUIRE(a->x != a->y || a->ldx == a->ldy);       // (in place: the same rows)
   if (!a->pos) {
     long n = 1;
     for (int i = 0; i < a->axes; ++i) {

@@ -755,7 +755,7 @@ def rope(x, heads: int, plan: RopePlan, *, grid=None, positions=None, inverse: b
     strided: the query and key slices of a fused projection are rotated in one call as x = qkv[..., :2C] with 2 * heads.
     Where the tokens sit: ``grid`` = the extents of the plan's axes, tokens in row-major order; or ``positions``, int32 or
     float32 [N, axes] or [B, N, axes] (crops, packed images, text tokens).  ``inverse=True`` turns back, which is the backward:
-    dx = rope(dy, ..., inverse=True).  ``out`` may be x itself."""
+    dx = rope(dy, ..., inverse=True).  ``out`` may be x itself, and otherwise shares no memory with it."""
     if x.dim() != 3 or x.dtype not in (BF16, F32):
         raise ValueError("rope: x must be a bf16 or float32 tensor [B, N, heads * head_dim]")
     B, N, Cc = x.shape
@@ -785,9 +785,12 @@ def rope(x, heads: int, plan: RopePlan, *, grid=None, positions=None, inverse: b
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("rope: out must have x's shape and type")
     _same_device("rope", x, out, plan.freq, plan.axis, positions)
+    ldx, ldy = _act(x, "x"), _act(out, "out")
+    if out is not x and (out.data_ptr() != x.data_ptr() or ldx != ldy) and _share(x, out):
+        raise ValueError("rope: out must be x's own rows or share no memory with x")
     if B == 0 or N == 0:
         return out
-    a = RopeArgs(x.data_ptr(), _act(x, "x"), out.data_ptr(), _act(out, "out"), int(x.dtype == F32), B, N, heads, plan.head_dim,
+    a = RopeArgs(x.data_ptr(), ldx, out.data_ptr(), ldy, int(x.dtype == F32), B, N, heads, plan.head_dim,
                  plan.rot, int(plan.pairing == "half"), plan.freq.data_ptr(), plan.axis.data_ptr(), nax, pos_ptr, pos_f32,
                  pos_stride, places, int(inverse))
     check(_lib.lib().dm_rope(C.byref(a), _stream()), "dm_rope")

@@ -273,7 +273,7 @@ int dm_cross_bwd(const dm_cross_args* args, dm_stream_t stream);
  * Rotary embedding with up to three position axes on every head of x [B, N, heads*hd] (an image or video's query / key
  * projection before dm_attn_fwd, reference unet.py:119-126, which has no positions): pair p turns by
  * position[axis[p]] * freq[p] TURNS (freq = theta^(-2i/d) / (2 pi), doubles); channels >= rot are copied.  Angles are reduced
- * in 64 bits.  inverse: the opposite angle, which is the backward.  y may be x itself, but not overlap it otherwise. */
+ * in 64 bits.  inverse: the opposite angle, which is the backward.  y may be x itself (with ldy = ldx), but not overlap it otherwise. */
 typedef struct dm_rope_args {
   const void* x; long ldx;        /* [B*N] rows of heads*hd */
   void* y; long ldy;

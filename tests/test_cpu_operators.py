@@ -251,3 +251,7 @@ def test_shared_memory_of_row_views():
             assert K._share(a, b) and K._share(b, a)
     assert min(both) > 300
     assert not K._share(buf[:0].view(1, 0, 4), buf.view(1, 100, 4)) and K._share(buf[:1].expand(2, 3, 1), buf.view(1, 100, 4))
+
+
+def test_rope_entry_point_refuses_other_rows_at_the_same_start():
+    assert _lib.lib().dm_rope(ctypes.byref(rope_struct(ldx=192)), None) == -1

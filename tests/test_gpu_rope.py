@@ -168,3 +168,20 @@ def test_rope_rows_past_32_bits():
     plan = k.rope_plan(32, (32,), device="cuda")
     k.rope(x, 2, plan, grid=(1100,), out=x)
     check(x, *reference(src, 2, 32, (32,), "interleaved", positions_of((1100,))), torch.bfloat16)
+
+
+def test_rope_refuses_an_output_that_overlaps():
+    """x's own rows or memory of its own: another start inside x's rows, or the same start with rows of another length, would be
+    written before they are read."""
+    k = K()
+    plan = k.rope_plan(32, (16, 16), device="cuda")
+    buf = torch.randn(2, 6, 192, device="cuda")
+    x = buf[..., :64]
+    for out in (buf[..., 32:96], buf.view(-1)[:x.numel()].view_as(x)):
+        with pytest.raises(ValueError):
+            k.rope(x, 2, plan, grid=(2, 3), out=out)
+    want = k.rope(x, 2, plan, grid=(2, 3))
+    k.rope(x, 2, plan, grid=(2, 3), out=buf[..., 64:128])
+    assert torch.equal(buf[..., 64:128], want)
+    k.rope(x, 2, plan, grid=(2, 3), out=buf[..., :64])
+    assert torch.equal(x, want)
