@@ -785,12 +785,12 @@ def rope(x, heads: int, plan: RopePlan, *, grid=None, positions=None, inverse: b
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("rope: out must have x's shape and type")
     _same_device("rope", x, out, plan.freq, plan.axis, positions)
-    ldx, ldy = _act(x, "x"), _act(out, "out")
-    if out is not x and (out.data_ptr() != x.data_ptr() or ldx != ldy) and _share(x, out):
+    (px, ldx), (py, ldy) = _rows("rope", "x", x), _rows("rope", "out", out)
+    if out is not x and (px != py or ldx != ldy) and _share(x, out):
         raise ValueError("rope: out must be x's own rows or share no memory with x")
     if B == 0 or N == 0:
         return out
-    a = RopeArgs(x.data_ptr(), ldx, out.data_ptr(), ldy, int(x.dtype == F32), B, N, heads, plan.head_dim,
+    a = RopeArgs(px, ldx, py, ldy, int(x.dtype == F32), B, N, heads, plan.head_dim,
                  plan.rot, int(plan.pairing == "half"), plan.freq.data_ptr(), plan.axis.data_ptr(), nax, pos_ptr, pos_f32,
                  pos_stride, places, int(inverse))
     check(_lib.lib().dm_rope(C.byref(a), _stream()), "dm_rope")
@@ -866,20 +866,24 @@ def _cross_check(what, q, k, v, heads, kv_heads, lens, mask, index, scale, drop_
     return B, Bc, kv_heads, Nq, Nk, hd, scale
 
 
-def _rows16(what, name, t, esize):
-    """(address, row stride) of [.., .., C] rows that start on 16-byte boundaries, samples densely packed."""
+def _rows(what, name, t):
+    """(address, row stride) of [.., .., C] rows, samples densely packed."""
     if t.is_contiguous():
-        ld = t.shape[-1]
-    else:
-        s0, ld, s2 = t.stride()
-        n0, n1, _ = t.shape
-        if n1 == 1:
-            ld = s0
-        elif n0 != 1 and s0 != ld * n1:
-            s2 = 0
-        if s2 != 1:
-            raise ValueError(f"{what}: unsupported strides {t.stride()} of {name} {tuple(t.shape)}")
-    ptr = t.data_ptr()
+        return t.data_ptr(), t.shape[-1]
+    s0, ld, s2 = t.stride()
+    n0, n1, _ = t.shape
+    if n1 == 1:
+        ld = s0
+    elif n0 != 1 and s0 != ld * n1:
+        s2 = 0
+    if s2 != 1:
+        raise ValueError(f"{what}: unsupported strides {t.stride()} of {name} {tuple(t.shape)}")
+    return t.data_ptr(), ld
+
+
+def _rows16(what, name, t, esize):
+    """_rows that start on 16-byte boundaries."""
+    ptr, ld = _rows(what, name, t)
     if (ptr | ld * esize) & 15:
         raise ValueError(f"{what}: the rows of {name} must be 16-byte aligned")
     return ptr, ld

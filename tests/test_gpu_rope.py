@@ -185,3 +185,17 @@ def test_rope_refuses_an_output_that_overlaps():
     assert torch.equal(buf[..., 64:128], want)
     k.rope(x, 2, plan, grid=(2, 3), out=buf[..., :64])
     assert torch.equal(x, want)
+
+
+def test_rope_one_token_of_many():
+    """A single token of every sample, as a view: its rows are a sample apart."""
+    k = K()
+    plan = k.rope_plan(32, (16, 16), device="cuda")
+    x = torch.randn(3, 6, 64, generator=torch.Generator().manual_seed(3)).cuda()
+    pos = torch.tensor([[3, 4]], dtype=torch.int32, device="cuda")
+    want = k.rope(x[:, 2:3].contiguous(), 2, plan, positions=pos)
+    assert torch.equal(k.rope(x[:, 2:3], 2, plan, positions=pos), want)
+    rest = x.clone()
+    k.rope(x[:, 2:3], 2, plan, positions=pos, out=x[:, 2:3])
+    rest[:, 2:3] = want
+    assert torch.equal(x, rest)
