@@ -208,14 +208,20 @@ class ContextMap(NamedTuple):
 
     @staticmethod
     def of(device, lens=None, mask=None, index=None) -> Optional["ContextMap"]:
-        """On ``device``, in the kernels' types; None when nothing is given."""
+        """On ``device``, in the kernels' types; None when nothing is given.  Lengths and indices are whole numbers and a mask is
+        bool (or 0 and 1): an additive mask of 0 and -infinity would mean the opposite."""
         if lens is None and mask is None and index is None:
             return None
 
-        def put(t, dtype):
-            return None if t is None else torch.as_tensor(t).to(device=device, dtype=dtype).contiguous()
+        def put(name, t, dtype):
+            if t is None:
+                return None
+            t = torch.as_tensor(t)
+            if t.numel() and (t.is_floating_point() or t.is_complex() or (t.dtype == torch.bool) > (dtype == torch.bool)):
+                raise ValueError(f"context_{name}: a {t.dtype} tensor is not {'a mask of valid tokens' if name == 'mask' else 'whole numbers'}")
+            return t.to(device=device, dtype=dtype).contiguous()
 
-        return ContextMap(put(lens, torch.int32), put(mask, torch.bool), put(index, torch.int32))
+        return ContextMap(put("lens", lens, torch.int32), put("mask", mask, torch.bool), put("index", index, torch.int32))
 
     def kw(self) -> dict:
         return dict(lens=self.lens, mask=self.mask, index=self.index)

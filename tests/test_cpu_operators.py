@@ -255,3 +255,19 @@ def test_shared_memory_of_row_views():
 
 def test_rope_entry_point_refuses_other_rows_at_the_same_start():
     assert _lib.lib().dm_rope(ctypes.byref(rope_struct(ldx=192)), None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(mask=torch.zeros(2, 7)), dict(mask=[[0.0, float("-inf")]]), dict(lens=torch.tensor([1.0, 2.0])),
+                                dict(lens=[True, False]), dict(index=torch.tensor([0.0])), dict(index=torch.zeros(2, dtype=torch.bool))])
+def test_context_map_refuses_other_kinds_of_numbers(kw):
+    from diffusion_model_amd.unet import ContextMap
+    with pytest.raises(ValueError):
+        ContextMap.of("cpu", **kw)
+
+
+def test_context_map_types():
+    from diffusion_model_amd.unet import ContextMap
+    m = ContextMap.of("cpu", [3, 0], torch.tensor([[1, 0], [0, 2]]), torch.tensor([1, 0, 1]))
+    assert (m.lens.dtype, m.mask.dtype, m.index.dtype) == (torch.int32, torch.bool, torch.int32)
+    assert m.mask.tolist() == [[True, False], [False, True]] and ContextMap.of("cpu") is None
+    assert ContextMap.of("cpu", lens=[]).lens.shape == (0,)
