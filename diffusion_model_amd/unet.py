@@ -226,6 +226,15 @@ class ContextMap(NamedTuple):
     def kw(self) -> dict:
         return dict(lens=self.lens, mask=self.mask, index=self.index)
 
+    def versions(self):
+        """The caller's tensors are used as they are, so a backward wants them unchanged: compare with the forward's."""
+        return tuple(None if t is None or t.is_inference() else t._version for t in self)
+
+
+def _unchanged(cmap: Optional[ContextMap], versions) -> None:
+    if cmap is not None and cmap.versions() != versions:
+        raise RuntimeError("context_lens, context_mask or context_index was modified in place between the forward and its backward")
+
 
 def _context_in(c, B, cmap: Optional[ContextMap]):
     """fp32 contexts [.., L, D] of B samples as an operand; with a map, tokens that no sample attends to become zeros."""
@@ -265,10 +274,13 @@ class _Fn(torch.autograd.Function):
         ctx.mod, ctx.saved, ctx.n_in = mod, saved, n_in
         ctx.params = args[n_in:]
         ctx.need_in = [torch.is_tensor(a) and a.requires_grad for a in ins]
+        ctx.cmap = next((a for a in ins if isinstance(a, ContextMap)), None)
+        ctx.versions = ctx.cmap and ctx.cmap.versions()
         return out
 
     @staticmethod
     def backward(ctx, dout):
+        _unchanged(ctx.cmap, ctx.versions)
         g = Grads()
         dins = ctx.mod._run_bwd(dout.contiguous(), ctx.saved, g, ctx.need_in)
         K.join_aux(dout.device)   # overlapped attention backward branches (UnetLayer._bwd)
@@ -1106,6 +1118,7 @@ class _UNetFn(torch.autograd.Function):
     def forward(ctx, mod, x, t, context, cmap, *params):
         y, saved = mod._fwd(x, t, context, cmap)
         ctx.mod, ctx.saved, ctx.params = mod, saved, params
+        ctx.cmap, ctx.versions = cmap, cmap and cmap.versions()
         ctx.need_dx = x.requires_grad
         ctx.need_dctx = torch.is_tensor(context) and torch.is_floating_point(context) and context.requires_grad
         ctx.ctx_shape = tuple(context.shape) if torch.is_tensor(context) else None
@@ -1113,6 +1126,7 @@ class _UNetFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        _unchanged(ctx.cmap, ctx.versions)
         g = Grads()
         dx = ctx.mod._bwd(dout.contiguous(), ctx.saved, g, need_dx=ctx.need_dx, need_dctx=ctx.need_dctx)
         pg = []

@@ -404,3 +404,24 @@ def test_partial_and_dpm_sampling_with_lengths(how):
 
     a, b = run(m), run(Copies)
     assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["lens", "mask", "index"])
+def test_a_map_changed_before_the_backward_is_refused(which):
+    """Lengths, masks and indices in the kernels' types are used where they are; a buffer that the next batch has already
+    overwritten would give gradients of another forward."""
+    from diffusion_model_amd.unet import CrossAttention
+    m, _ = network(False)
+    x, t, ctx = case(2, 2, 9)
+    c = CrossAttention(64, 48, HEADS, 0.0).to(dev()).eval()
+    runs = (lambda kw: m(x.to(dev()), t, ctx.to(dev()), **kw), lambda kw: c(torch.ones(2, 64, 4, 4, device=dev()), ctx.to(dev()), **kw))
+    for run in runs:
+        kw = dict(context_lens=torch.tensor([9, 4], dtype=torch.int32, device=dev()), context_mask=torch.ones(2, 9, dtype=torch.bool, device=dev()),
+                  context_index=torch.tensor([1, 0], dtype=torch.int32, device=dev()))
+        run(kw).sum().backward()                              # unchanged: fine
+        y = run(kw)
+        kw["context_" + which].zero_()
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+    with torch.inference_mode():
+        assert bool(torch.isfinite(runs[0](dict(context_lens=torch.tensor([9, 4], dtype=torch.int32, device=dev())))).all())
