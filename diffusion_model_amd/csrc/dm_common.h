@@ -53,6 +53,9 @@ static inline bool dm_first_on_device(unsigned long long& mask) {
   return true;
 }
 
+// HIP takes fewer than 2^32 threads along a grid dimension: the most workgroups of 256
+constexpr long DM_MAX_GRID256 = (1L << 24) - 1;
+
 static inline int dm_cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
 __device__ __forceinline__ float dm_silu(float x) { return x / (1.0f + __expf(-x)); }

@@ -440,6 +440,8 @@ BwdPlan bwd_plan(const dm_cross_args* a) {
 template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 int launch_dq(const CrossParams& p, hipStream_t st) {
   auto kern = cross_dq_kernel<T, HDP, RES, SPLIT, DROP>;
+  const long blocks = (long)p.B * p.qsplit * p.nqb * p.H;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -447,8 +449,6 @@ int launch_dq(const CrossParams& p, hipStream_t st) {
     return DM_ERR_LAUNCH;
   size_t lds = RES ? (size_t)p.kb * (2 * Geo<T, HDP>::SR + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
   if (SPLIT && lds < 4 * 32 * (HDP + 4) * 4) lds = 4 * 32 * (HDP + 4) * 4;
-  const long blocks = (long)p.B * p.qsplit * p.nqb * p.H;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   return p.qsplit > 1 ? dqsum_launch(p, sizeof(T) == 2 ? 0 : 1, st) : DM_OK;
@@ -457,20 +457,20 @@ template <typename T, int HDP, bool DROP>
 int launch_dkv(const CrossParams& p, hipStream_t st) {
   auto kern = cross_dkv_kernel<T, HDP, DROP>;
   const int lds = 2 * list_bytes<T, HDP>();
+  const long blocks = (long)p.Bc * p.nsplit * ((p.Nk + 127) / 128) * p.G;
+  if (blocks == 0) return DM_OK;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const long blocks = (long)p.Bc * p.nsplit * ((p.Nk + 127) / 128) * p.G;
-  if (blocks == 0) return DM_OK;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
   DM_LAUNCH_CHECK();
   if (p.nsplit > 1) {
     const long n = (long)2 * p.Bc * p.Nk * p.G * (p.hd >> 2);
     const bool wide = p.nsplit > 8;
     const long jb = (n + (wide ? 31 : 255)) / (wide ? 32 : 256);
-    if (jb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    if (jb > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
     if (wide) hipLaunchKernelGGL((cross_sum_kernel<T, 8>), dim3((unsigned)jb), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((cross_sum_kernel<T, 1>), dim3((unsigned)jb), dim3(256), 0, st, p);
     DM_LAUNCH_CHECK();

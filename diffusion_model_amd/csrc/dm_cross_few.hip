@@ -384,12 +384,12 @@ int launch(const CrossParams& p, hipStream_t st) {
   auto kern = cross_few_kernel<T, HDP, KT, DROP, HEADS>;
   constexpr int lds = few_lds<T, HDP, KT>();
   static_assert(lds <= 160 * 1024, "LDS");
+  const long blocks = (long)p.B * p.nqb * (HEADS ? p.G : p.H);
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const long blocks = (long)p.B * p.nqb * (HEADS ? p.G : p.H);
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_bwd_few<%s,%d,KT=%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, KT);
   dm_set_variant(nm.s);
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);
@@ -400,7 +400,7 @@ int launch(const CrossParams& p, hipStream_t st) {
     CrossParams g = p;
     g.iters = (int)((n + (wide ? 31 : 255)) / (wide ? 32 : 256));
     const long gb = (long)p.Bc * g.iters;
-    if (gb > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+    if (gb > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
     if (wide) hipLaunchKernelGGL((cross_gather_kernel<T, 8>), dim3((unsigned)gb), dim3(256), 0, st, g);
     else hipLaunchKernelGGL((cross_gather_kernel<T, 1>), dim3((unsigned)gb), dim3(256), 0, st, g);
     DM_LAUNCH_CHECK();

@@ -352,6 +352,8 @@ FwdPlan fwd_plan(const dm_cross_args* a) {
 template <typename T, int HDP, bool RES, bool SPLIT, bool DROP>
 int launch_fwd(const CrossParams& p, hipStream_t st) {
   auto kern = cross_fwd_kernel<T, HDP, RES, SPLIT, DROP>;
+  const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -359,8 +361,6 @@ int launch_fwd(const CrossParams& p, hipStream_t st) {
     return DM_ERR_LAUNCH;
   size_t lds = RES ? (size_t)p.kb * (Geo<T, HDP>::SR + Geo<T, HDP>::ST + 4) + (p.kb / 32 + 2) * 4 : 2 * image_bytes<T, HDP>();
   if (SPLIT && lds < 4 * 32 * ((HDP + 4) * 4 + 8)) lds = 4 * 32 * ((HDP + 4) * 4 + 8);
-  const long blocks = (long)p.B * p.nsplit * p.nqb * p.H;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_fwd<%s,%d,%s>", sizeof(T) == 2 ? "bf16" : "fp32", HDP, SPLIT ? "split" : (RES ? "resident" : "streamed"));
   dm_set_variant(nm.s);
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);

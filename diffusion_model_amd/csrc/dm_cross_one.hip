@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossParams p) {
 
 template <typename T, int LPR, int R> int launch(const CrossParams& p, hipStream_t st) {
   const long blocks = (long)p.B * p.nsplit * p.G;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_one<%s,LPR=%d,R=%d>", sizeof(T) == 2 ? "bf16" : "fp32", LPR, R);
   dm_set_variant(nm.s);
   hipLaunchKernelGGL((cross_one_kernel<T, LPR, R>), dim3((unsigned)blocks), dim3(256), 0, st, p);
@@ -239,7 +239,7 @@ int one_launch(const CrossParams& p, int dtype, hipStream_t st) {
 
 int join_launch(const CrossParams& p, int dtype, hipStream_t st) {
   const long blocks = ((long)p.B * p.H * p.Nq + 3) / 4;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   if (dtype == 0) hipLaunchKernelGGL((cross_join_kernel<bf16>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((cross_join_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   DM_LAUNCH_CHECK();

@@ -224,7 +224,7 @@ template <typename T> int launch_sum(const CrossParams& p, hipStream_t st) {
   const long n = (long)p.B * p.H * p.Nq * (p.hd >> 2);
   const bool wide = p.qsplit > 8;
   const long blocks = (n + (wide ? 31 : 255)) / (wide ? 32 : 256);
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   if (wide) hipLaunchKernelGGL((cross_dqsum_kernel<T, 8>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((cross_dqsum_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   DM_LAUNCH_CHECK();
@@ -233,7 +233,7 @@ template <typename T> int launch_sum(const CrossParams& p, hipStream_t st) {
 
 template <typename T, int LPR, bool DROP> int launch(const CrossParams& p, hipStream_t st) {
   const long blocks = (long)p.Bc * p.qsplit * p.G;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_bwd_one<%s,LPR=%d>", sizeof(T) == 2 ? "bf16" : "fp32", LPR);
   dm_set_variant(nm.s);
   hipLaunchKernelGGL((cross_onebwd_kernel<T, LPR, DROP>), dim3((unsigned)blocks), dim3(256), 0, st, p);

@@ -188,12 +188,12 @@ template <typename T, int HDP, bool DROP> int launch(const CrossParams& p, hipSt
   auto kern = cross_rows_kernel<T, HDP, DROP>;
   constexpr int lds = lds_bytes<T, HDP>();
   static_assert(lds <= 160 * 1024, "LDS");
+  const long blocks = (long)p.Bc * p.qsplit * p.G;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static unsigned long long attr_devs = 0ull;
   if (dm_first_on_device(attr_devs) &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return DM_ERR_LAUNCH;
-  const long blocks = (long)p.Bc * p.qsplit * p.G;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("cross_bwd_rows<%s,%d>", sizeof(T) == 2 ? "bf16" : "fp32", HDP);
   dm_set_variant(nm.s);
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, p);

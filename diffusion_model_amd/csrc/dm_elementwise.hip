@@ -590,7 +590,7 @@ extern "C" int dm_context_rows(const float* x, void* y, int y_is_f32, int Bc, in
                                const unsigned char* mask, const int* index, int B, dm_stream_t stream) {
   DM_REQUIRE(x && y && Bc > 0 && L > 0 && D > 0 && (!index || B > 0));
   const long rows = (long)Bc * L, blocks = (rows + 3) / 4;
-  if (blocks >= (1L << 24)) return DM_ERR_TOO_LARGE;      // (a grid has fewer than 2^32 threads)
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   if (y_is_f32)
     hipLaunchKernelGGL(context_rows_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, x, (float*)y, rows, L, D,
                        lens, mask, index, B);

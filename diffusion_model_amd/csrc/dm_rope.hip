@@ -181,7 +181,7 @@ int launch(RopeParams& p, int heads, hipStream_t st) {
   p.by_uph = fast_div(p.uph);
   p.by_np = fast_div(p.np);
   const long blocks = (p.rows + rt - 1) / rt;
-  if (blocks > 0x7FFFFFFFL) return DM_ERR_TOO_LARGE;
+  if (blocks > DM_MAX_GRID256) return DM_ERR_TOO_LARGE;
   static const DmVariantName nm("rope<%s,%s,V=%d>", sizeof(T) == 2 ? "bf16" : "fp32", HALF ? "half" : "interleaved", V);
   dm_set_variant(nm.s);
   hipLaunchKernelGGL((rope_kernel<T, HALF, V>), dim3((unsigned)blocks), dim3(256), (size_t)rt * p.np * 8, st, p);

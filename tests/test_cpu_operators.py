@@ -271,3 +271,18 @@ def test_context_map_types():
     assert (m.lens.dtype, m.mask.dtype, m.index.dtype) == (torch.int32, torch.bool, torch.int32)
     assert m.mask.tolist() == [[True, False], [False, True]] and ContextMap.of("cpu") is None
     assert ContextMap.of("cpu", lens=[]).lens.shape == (0,)
+
+
+@pytest.mark.parametrize("kw", [dict(Nq=1), dict(Nq=1, Nk=600), dict(Nq=5), dict(Nq=20, Nk=600), dict(Nq=40, Nk=600, ldq=128),
+                                dict(Nq=40, Nk=20), dict(Nq=200, Nk=600, Bc=1)])
+def test_cross_grids_that_hip_does_not_take(kw):
+    """A launch holds fewer than 2^32 threads along its grid: more samples and heads than 2^24 workgroups of 256 are refused."""
+    L = _lib.lib()
+    a = cross_struct(**{**dict(B=1 << 23, Bc=1 << 23, ws_bytes=1 << 62), **kw})
+    assert L.dm_cross_fwd(ctypes.byref(a), None) == -3
+    assert L.dm_cross_bwd(ctypes.byref(a), None) == -3
+
+
+def test_rope_grids_that_hip_does_not_take():
+    a = rope_struct(B=1 << 20, N=1 << 10, heads=32, ldx=1024, ldy=1024, axes=1, grid=(1 << 10, 0))
+    assert _lib.lib().dm_rope(ctypes.byref(a), None) == -3
