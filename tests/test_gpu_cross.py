@@ -557,3 +557,43 @@ def test_cross_refuses_outputs_that_share_memory():
     want = kn.cross_bwd(q, k, v, o, lse, d_o, 2)
     kn.cross_bwd(q, k, v, o, lse, d_o, 2, dq=buf[..., :32], dk=buf[..., 32:64], dv=buf[..., 64:])
     assert all(torch.equal(a, b) for a, b in zip(want, buf.split(32, -1)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,Nk", [(130, 130), (130, 70), (20, 130), (1, 130)])
+def test_cross_rows_far_apart(Nq, Nk, dtype):
+    """Rows so far apart (24 MiB in bf16, 40 MiB in fp32; 64 MiB is the limit) that 32 bits do not hold a step of the staging
+    loads, which then go by plain addresses: queries, states, gradients and results, with masked states."""
+    kn = K()
+    ld = (24 << 20) // 2 if dtype == BF16 else (40 << 20) // 4
+    base = torch.empty(1, max(Nq, Nk), ld, dtype=dtype, device="cuda")      # 3.0 and 5.1 GiB
+    q, k, v, d_o, _, M, _ = inputs(dtype, 1, 1, Nq, Nk, 1, 1, 16, None, True, False, seed=Nq + Nk)
+    val, tol = reference(q, k, v, 1, 1, None, M, d_o=d_o)
+    at = {}
+    for i, (name, t) in enumerate((("q", q), ("k", k), ("v", v), ("d_o", d_o), ("o", q), ("dq", q), ("dk", k), ("dv", k))):
+        at[name] = base[:, :t.shape[1], 64 * i:64 * i + 16]
+        at[name].copy_(t)
+    o, lse = kn.cross_fwd(at["q"], at["k"], at["v"], 1, mask=M.cuda(), out=at["o"])
+    grads = kn.cross_bwd(at["q"], at["k"], at["v"], o, lse, at["d_o"], 1, mask=M.cuda(), dq=at["dq"], dk=at["dk"], dv=at["dv"])
+    for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *grads)):
+        check(name, t, val, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Nq,Nk,hd,variant", [(1, 300, 64, "cross_bwd_one"), (20, 150, 64, "cross_bwd_rows"), (70, 150, 64, "cross_bwd<"),
+                                              (70, 40, 32, "cross_bwd_few")])
+def test_cross_half_of_the_samples_on_one_context(Nq, Nk, hd, variant, dtype):
+    """The form goes by the average list; one list of 33 samples among lists of one or none."""
+    kn = K()
+    B = 66
+    q, k, v, d_o, L, _, I = inputs(dtype, B, B, Nq, Nk, 1, 1, hd, "ragged", False, True, seed=Nq)
+    I[:] = torch.arange(B, dtype=torch.int32)
+    I[::2] = 5
+    L[5] = Nk
+    val, tol = reference(q, k, v, 1, 1, L, None, I, d_o=d_o)
+    dq_, dk_, dv_, do_, dL, dI = cuda(q, *poison(k, v, L, None), d_o, L, I)
+    o, lse = kn.cross_fwd(dq_, dk_, dv_, 1, lens=dL, index=dI)
+    grads = kn.cross_bwd(dq_, dk_, dv_, o, lse, do_, 1, lens=dL, index=dI)
+    assert kn.last_variant().startswith(variant)
+    for name, t in zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *grads)):
+        check(name, t, val, tol)
