@@ -352,6 +352,9 @@ class Trainer:
             gt.copy_(t, non_blocking=True)
             if gc is not None:
                 gc.copy_(context, non_blocking=True)
+            # an eager micro-step of this window (a map of contexts, another shape) may have left weight gradients on the side
+            # stream: the graph adds to the same gradients and writes the same scratch
+            K.join_side(x.device)
             self._graph.replay()
             self.last_skipped = False
             self.micro = 0 if last else self.micro + 1

@@ -425,3 +425,69 @@ def test_a_map_changed_before_the_backward_is_refused(which):
             y.sum().backward()
     with torch.inference_mode():
         assert bool(torch.isfinite(runs[0](dict(context_lens=torch.tensor([9, 4], dtype=torch.int32, device=dev())))).all())
+
+
+def test_micro_steps_with_lengths_beside_a_captured_one():
+    """One accumulation window of eager micro-steps with lengths and replayed ones without: each replay finds the eager weight
+    gradients joined, and the sums are those of a trainer without a graph."""
+    from diffusion_model_amd import kernels as K
+    from diffusion_model_amd.trainer import Trainer
+    from diffusion_model_amd.utils import DDPM_beta_t_cosine_scheduler
+    x, t, ctx = case(4, 4, 9)
+    x, t, ctx = x.to(dev()), t.to(dev()), ctx.to(dev())
+    es = [torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).to(dev()) for i in range(5)]
+    grads = []
+    for captured in (False, True):
+        m, _ = network(True)
+        tr = Trainer(m.train(), DDPM_beta_t_cosine_scheduler(500), accum=8)
+        if captured:
+            tr.enable_graph(x, ctx, t, es[0])
+            replay = tr._graph.replay
+
+            class Joined:
+                """The captured step, replayed only with nothing left on the side stream."""
+                @staticmethod
+                def replay():
+                    assert not K._PENDING and not K._SIDE_DIRTY
+                    replay()
+
+            tr._graph = Joined
+        for i, e in enumerate(es):
+            tr.micro_step(x, ctx, t, e, **(dict(context_lens=torch.tensor([9, 4, 0, 1])) if i % 2 == 0 else {}))
+        K.join_side(dev())
+        grads.append(tr.fp.grad.clone())
+        tr.disable_graph()
+    assert float(grads[0].abs().max()) > 0 and torch.equal(*grads)
+
+
+def test_captured_network_with_a_map():
+    """UNET.forward in a graph, replayed with other lengths, masks and indices in the same buffers, eager calls in between."""
+    m, _ = network(True)
+    x, t, ctx = case(4, 3, 9)
+    x, t, ctx = x.to(dev()), t.to(dev()), ctx.to(dev())
+    lens, mask = torch.tensor([9, 4, 0], dtype=torch.int32, device=dev()), torch.ones(3, 9, dtype=torch.bool, device=dev())
+    index = torch.tensor([0, 1, 1, 2], dtype=torch.int32, device=dev())
+
+    def run():
+        with torch.no_grad():
+            return m(x, t, ctx, context_lens=lens, context_mask=mask, context_index=index)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for i in range(4):
+        g = torch.Generator().manual_seed(i)
+        lens.copy_(torch.randint(0, 10, (3,), generator=g, dtype=torch.int32))
+        mask.copy_(torch.rand(3, 9, generator=g) < 0.7)
+        index.copy_(torch.randint(-1, 4, (4,), generator=g, dtype=torch.int32))
+        x.copy_(torch.randn(x.shape, generator=g))
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
