@@ -8,7 +8,8 @@
 // A 32x32 result tile puts column l % 32 and rows 8 i + 4 (l / 32) + r (register 4 i + r) into lane l.  Scores are computed
 // with the softmax axis on the registers (forward, dq) or the lanes (dk, dv), and the probability tile is then, register by
 // register, already the second product's operand over the reduction order "rows 8 i + 4 half + r"; the other operand takes
-// that order through the row addresses of its transposing LDS reads (tr_frag).  Where one pass computes the products of both axes, a probability tile is also turned through LDS.
+// that order through the row addresses of its transposing LDS reads (tr_frag).  Where one pass computes the products of both axes,
+// a probability tile is also turned through LDS.
 #pragma once
 #include "dm_common.h"
 
@@ -58,7 +59,8 @@ template <> struct Cr<bf16> {
   static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // operand fragment f of a result tile (its rows are the reduction axis)
+  // operand fragment f of a result tile (its rows are the reduction axis); in bf16 the probabilities and the score gradients are
+  // rounded here, half a step (2^-8) of each value: the matrix units take no wider operand at their rate, and fp32 sums follow
   static __device__ __forceinline__ frag pack(const f32x16& s, int f) {
     frag r;
 #pragma unroll

@@ -3,12 +3,12 @@
 //   P = exp2(c S - lse log2(e)),  dP = dO V^T,  dS = P (dP - delta),  delta = sum_d dO * O,
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
 // dQ runs with the queries on the lanes (as the forward), dK / dV with the keys on the lanes; each probability tile is then
-// already the operand of the product that reduces over its rows.  S and dP are computed in
-// both kernels, seven products in all: one kernel for both sides would have to add dQ up over its key blocks in memory, 4
-// bytes per channel and block.
-// The pipes (matrix, vector, LDS) are each about a third busy at two waves per SIMD; more waves, or two tiles at a time, were
-// not faster.  bf16, 16 x 1024 queries, 8 heads of 64 on 333 states (2 key / value heads, a tenth masked): dQ 36 us, dK and dV
-// 41 us; fp32, 8 key / value heads: 477 us together (82 TFLOP/s).
+// already the operand of the product that reduces over its rows.  S and dP are computed in both kernels, seven products in all:
+// one kernel for both sides would have to add dQ up over its key blocks in memory, 4 bytes per channel and block. The pipes
+// (vector, matrix, LDS) are 40, 25 and 26 % busy in dQ, 33, 31 and 35 % in dK / dV at two waves per SIMD; more waves, or two
+// query tiles at a time, were not faster.  delta reads O as the forward rounded it.  bf16, 16 x 1024 queries, 8 heads of 64 on
+// 333 states (2 key / value heads, a tenth masked): dQ 36 us, dK and dV 41 us; fp32, 8 key / value heads: 477 us together (82
+// TFLOP/s).
 #include "dm_cross.h"
 
 namespace {

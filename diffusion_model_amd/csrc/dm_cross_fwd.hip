@@ -5,10 +5,11 @@
 // The row sum takes the fp32 probabilities before they are rounded for the second product, so lse is an fp32 value.
 //
 // Narrow heads are bound by the vector work per score (an exponential, a maximum, two adds and half a conversion against 64
-// matrix flops), which is why masks cost none of it and empty half tiles are left out; wide ones by the matrix units and the
-// LDS reads that feed them.  bf16, ragged lengths: 64 x 2304 queries, 8 heads of 16, 77 tokens 27 us; 64 x 576, 8 heads of 32,
-// 77 tokens 12.5 us (3.3 TB/s); 16 x 1024, 8 heads of 128, 512 states 49 us (700 TFLOP/s).  fp32: 16 x 1024, 8 heads of 64, 333
-// states 118 us (95 TFLOP/s).
+// matrix flops; vector units 67 % busy at 16-wide heads), which is why masks cost none of it and empty half tiles are left out;
+// wide ones by the chain of scores, softmax and products of the one tile that a wave has (vector units 40 % busy, matrix units
+// 32, LDS 28 at 128-wide heads).  bf16, ragged lengths: 64 x 2304 queries, 8 heads of 16, 77 tokens 27 us; 64 x 576, 8 heads of
+// 32, 77 tokens 12.5 us (3.3 TB/s); 16 x 1024, 8 heads of 128, 512 states 49 us (700 TFLOP/s).  fp32: 16 x 1024, 8 heads of 64,
+// 333 states 118 us (95 TFLOP/s).
 #include "dm_cross.h"
 
 namespace {

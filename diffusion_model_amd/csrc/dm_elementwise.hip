@@ -81,7 +81,8 @@ __global__ void cast_bf16_f32_kernel(const bf16* __restrict__ x, float* __restri
 
 // Context rows as operands: the ones that some sample attends to are cast, the others become zeros by a select (their
 // gradients are exact zeros, and a product with what padding holds -- NaN, infinities -- would not be).  One wave per row;
-// whether the row's context has a sample is looked up in the index 64 entries at a time.
+// whether the row's context has a sample is looked up in the index 64 entries at a time.  64 x 77 tokens of 512 channels to bf16:
+// 4.2 us with lengths, 4.5 with an index of 64, too (the cast alone 3.7).
 template <typename T>
 __global__ __launch_bounds__(256) void context_rows_kernel(const float* __restrict__ x, T* __restrict__ y, long rows, int L, int D,
                                                            const int* __restrict__ lens, const unsigned char* __restrict__ mask,

@@ -5,12 +5,13 @@
 //   (u cos t - w sin t,  w cos t + u sin t),   t = x_a f(p)       (t -> -t: the inverse, which is also the backward),
 // channels past the rotated width are copied.  Pairs are neighbours (2p, 2p+1) or half the rotated width apart (p, p + R/2).
 //
-// Angles: far positions lose their fraction in 32 bits (x = 1e5 leaves 2^-7 of a radian), so the frequency is kept in
-// TURNS per unit of position as a double; x f is reduced to a fraction of a turn in 64 bits and only then goes to
-// sincospif.  A workgroup computes each (token, pair) angle ONCE into an LDS table and uses it for every head, so the
-// 64-bit work is 1/heads of the elements and the kernel is a pure stream: one 16-byte load, one 16-byte store.
-// bf16, 64 x 576 tokens, 16 heads of 32: 14.3 us (5.3 TB/s); 2 x 16384 tokens, 16 heads of 128, forward and inverse: 103 us
-// (5.2 TB/s); fp32, 8 x 1371 tokens, 16 heads of 40, positions of their own per sample, both ways: 30 us (3.8 TB/s).
+// Angles: far positions lose their fraction in 32 bits (x = 1e5 leaves 2^-7 of a radian), so the frequency is kept in TURNS per
+// unit of position as a double; x f is reduced to a fraction of a turn in 64 bits and only then rounded to 32 (at most pi 2^-24
+// of a radian, of the size of sincospif's own error) for sincospif.  A workgroup computes each (token, pair) angle ONCE into an
+// LDS table and uses it for every head, so the 64-bit work is 1/heads of the elements and the kernel is a pure stream: one
+// 16-byte load, one 16-byte store. bf16, 64 x 576 tokens, 16 heads of 32: 14.3 us (5.3 TB/s; a copy of these 75 MB, which the
+// last-level cache holds, 11.7 us); 2 x 16384 tokens, 16 heads of 128, forward and inverse: 103 us (5.2 TB/s; two such copies
+// 75 us); fp32, 8 x 1371 tokens, 16 heads of 40, positions of their own per sample, both ways: 30 us (3.8 TB/s).
 #include "dm_common.h"
 
 namespace {

@@ -242,9 +242,10 @@ long dm_cross1_bwd_workspace_bytes(int B, int heads, int C);
  *   - key j of context c is valid iff j < lens[c] (NULL: Nk; values are clamped to [0, Nk]) and mask[c][j] != 0 (NULL: all).
  *     What invalid rows of k and v hold does not matter (NaN and infinities included).
  *   - a query with no valid key: o = 0, lse = -infinity, and no gradient flows.
- * hd: a multiple of 8 up to 128.  Rows of every activation are 16-byte aligned and less than 64 MiB apart, and no output
- * shares memory with an input or another output.  Scores, softmax statistics and accumulators are fp32; with dtype 0 the probabilities (and in the backward the score gradients) are rounded to bf16 for the second
- * matrix product, like the inputs.  Dropout words as dm_attn_fwd's for 64- and 128-wide heads. */
+ * hd: a multiple of 8 up to 128.  Rows of every activation are 16-byte aligned and less than 64 MiB apart, and no output shares
+ * memory with an input or another output.  Scores, softmax statistics and accumulators are fp32; with dtype 0 the probabilities
+ * (and in the backward the score gradients) are rounded to bf16 for the second matrix product, like the inputs.  Dropout words
+ * as dm_attn_fwd's for 64- and 128-wide heads. */
 typedef struct dm_cross_args {
   const void* q; long ldq;        /* [B, Nq, heads*hd] */
   const void* k; long ldk;        /* [Bc, Nk, kv_heads*hd] */
